@@ -51,6 +51,7 @@ extern "C" {
 #define PLORA_DEV_IMAGE_RANGE 8  /* a slot-image record pointed outside the image: rank 0  */
 #define PLORA_DEV_PADDING 16     /* an attention mask was not right-padded                */
 #define PLORA_DEV_TOKEN_RANGE 32 /* a segment-table token id outside [0, num_tokens) skipped */
+#define PLORA_DEV_PAGE_RANGE 64  /* a cached token without a page in [0, num_pages): see below */
 
 /* Library version string. */
 const char* plora_version(void);
@@ -310,6 +311,80 @@ int plora_slot_fill(const plora_slot_module* modules, int32_t num_modules, int32
 int plora_peft_pack(const char* path, const char* const* modules, int32_t num_modules,
                     const char* adapter_name, int32_t dtype, double lora_alpha, void* image,
                     size_t capacity, size_t* image_bytes, int64_t* dims);
+
+/* ---------------------------------------------------------------------------
+ * Paged key-value cache (no counterpart in the reference).
+ *
+ * k_cache, v_cache: (num_pages, kv_heads, page_size, head_dim), dense within a
+ * page, k_page_stride / v_page_stride elements between pages; position p of
+ * row b is slot p % page_size of page page_table[b * table_stride + p / page_size]
+ * (max_pages int32 entries a row; entries past a row's tokens are not read).
+ * head_dim is a multiple of 8 up to 256, page_size any positive number, and
+ * heads a multiple of kv_heads: query head h reads key-value head
+ * h / (heads / kv_heads).  Strides are in elements and, like all pointers to
+ * heads and pages, multiples of 16 bytes.  Rows must not share a page that
+ * plora_paged_append writes; pages that are only read may be shared.
+ *
+ * plora_paged_append: new token m < new_lens[b] (null: max_new each) of row b
+ * takes position past_lens[b] + m.  q (rows, max_new, q_heads, head_dim; null:
+ * none) and k (.., kv_heads, ..) are rotated, k and v written to their pages,
+ * rotated queries to q_out and, if k_out is not null, rotated keys to k_out,
+ * both dense; padded tokens (m >= new_lens[b]) are zeros there and leave the
+ * cache alone.  The first 2 * pairs elements of a head rotate, element i with
+ * i + pairs, or 2i with 2i + 1 when interleaved != 0, by position * f_i;
+ * phases[i] = round(f_i / (2 pi) * 2^64) mod 2^64, cosines and sines times
+ * rotary_scale.  pairs 0: no rotation.  A token whose position has no page in
+ * [0, num_pages) is not cached and raises PLORA_DEV_PAGE_RANGE.
+ *
+ * plora_paged_attention: out[b, h] = softmax(scale * q[b, h] . k) v over row
+ * b's last min(window, seq_lens[b]) of seq_lens[b] cached tokens (window 0:
+ * all of them); zeros where there are none.  out is dense (rows, heads,
+ * head_dim).  A token on a page outside [0, num_pages) reads as zeros, and
+ * seq_lens beyond the table's reach are clamped to it; the first raises
+ * PLORA_DEV_PAGE_RANGE.  Sums in fp32; repeated calls agree bit for bit.  The
+ * workspace (plora_paged_attention_workspace bytes, 256-byte aligned; 0 for
+ * arguments the call rejects) needs no initialisation; calls that may overlap
+ * need one each. */
+int plora_paged_append(const void* q, int64_t q_row_stride, int64_t q_token_stride, int64_t q_head_stride,
+                       const void* k, int64_t k_row_stride, int64_t k_token_stride, int64_t k_head_stride,
+                       const void* v, int64_t v_row_stride, int64_t v_token_stride, int64_t v_head_stride,
+                       void* q_out, void* k_out, void* k_cache, void* v_cache, int64_t k_page_stride,
+                       int64_t v_page_stride, const int32_t* page_table, int64_t table_stride,
+                       const int32_t* past_lens, const int32_t* new_lens, const int64_t* phases, int32_t pairs,
+                       int32_t interleaved, float rotary_scale, int64_t rows, int64_t max_new, int32_t q_heads,
+                       int32_t kv_heads, int32_t head_dim, int32_t page_size, int64_t num_pages, int64_t max_pages,
+                       int32_t dtype, void* stream);
+
+size_t plora_paged_attention_workspace(int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t dtype);
+
+int plora_paged_attention(const void* q, int64_t q_row_stride, int64_t q_head_stride, const void* k_cache,
+                          const void* v_cache, int64_t k_page_stride, int64_t v_page_stride,
+                          const int32_t* page_table, int64_t table_stride, const int32_t* seq_lens, void* out,
+                          float scale, int64_t window, int64_t rows, int32_t heads, int32_t kv_heads,
+                          int32_t head_dim, int32_t page_size, int64_t num_pages, int64_t max_pages, int32_t dtype,
+                          void* workspace, size_t workspace_size, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Each row's own rules on its logits (no counterpart in the reference).
+ *
+ * logits, out: (rows, vocab) of dtype, *_stride elements between rows; out may
+ * be logits.  In fp32, rounded once, in this order:
+ *   x > 0 ? x / repetition[b] : x * repetition[b]  for tokens of row b's history,
+ *       tokens[b, i], i < token_lens[b] (null: history each);
+ *   x - frequency[b] * count - presence[b]         for tokens found count > 0 times
+ *       among i >= prompt_lens[b] (null: 0);
+ *   x + bias_values[b, j]                          for each j with bias_tokens[b, j];
+ *   -infinity                                      where bit t % 32 of
+ *       allowed[b, t / 32] is 0 (null: all are allowed).
+ * Null repetition / presence / frequency mean 1 / 0 / 0.  Token ids are
+ * int32 or int64 (token_bytes 4 or 8); ids outside [0, vocab) are skipped. */
+int plora_logit_rules(const void* logits, int64_t logits_stride, void* out, int64_t out_stride, int64_t rows,
+                      int64_t vocab, int32_t dtype, const void* tokens, int64_t tokens_stride, int64_t history,
+                      const int32_t* token_lens, const int32_t* prompt_lens, const float* repetition,
+                      const float* presence, const float* frequency, const void* bias_tokens,
+                      int64_t bias_tokens_stride, const float* bias_values, int64_t bias_values_stride,
+                      int64_t biases, const int32_t* allowed, int64_t allowed_stride, int32_t token_bytes,
+                      void* stream);
 
 #ifdef __cplusplus
 }

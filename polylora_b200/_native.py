@@ -30,6 +30,7 @@ DEV_RANK_RANGE = 4
 DEV_IMAGE_RANGE = 8
 DEV_PADDING = 16
 DEV_TOKEN_RANGE = 32
+DEV_PAGE_RANGE = 64
 
 NOALLOC_SCRATCH_BYTES = 8 << 20  # PLORA_NOALLOC_SCRATCH_BYTES
 
@@ -152,6 +153,29 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [
             _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
             _i64, _i64, _i64, _i64, _i32, _i32, _i32, _c_void_p,
+        ],
+    ),
+    "plora_paged_append": (
+        ctypes.c_int,
+        [
+            _c_void_p, _i64, _i64, _i64, _c_void_p, _i64, _i64, _i64, _c_void_p, _i64, _i64, _i64,
+            _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i64, _c_void_p, _i64, _c_void_p, _c_void_p, _c_void_p,
+            _i32, _i32, ctypes.c_float, _i64, _i64, _i32, _i32, _i32, _i32, _i64, _i64, _i32, _c_void_p,
+        ],
+    ),
+    "plora_paged_attention_workspace": (_size, [_i32, _i32, _i32, _i32]),
+    "plora_paged_attention": (
+        ctypes.c_int,
+        [
+            _c_void_p, _i64, _i64, _c_void_p, _c_void_p, _i64, _i64, _c_void_p, _i64, _c_void_p, _c_void_p,
+            ctypes.c_float, _i64, _i64, _i32, _i32, _i32, _i32, _i64, _i64, _i32, _c_void_p, _size, _c_void_p,
+        ],
+    ),
+    "plora_logit_rules": (
+        ctypes.c_int,
+        [
+            _c_void_p, _i64, _c_void_p, _i64, _i64, _i64, _i32, _c_void_p, _i64, _i64, _c_void_p, _c_void_p,
+            _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p, _i64, _i64, _c_void_p, _i64, _i32, _c_void_p,
         ],
     ),
     "plora_slot_fill": (

@@ -1,0 +1,710 @@
+// Paged key-value cache: appending new tokens with their position rotation,
+// and attention of one new token per row over the cache.
+//
+// Cache layout: k and v are (num_pages, kv_heads, page_size, head_dim), so the
+// tokens of one head in one page are one contiguous run; a row's tokens are
+// found through its page table, position p at slot p % page_size of page
+// table[p / page_size].
+#pragma once
+
+#include "common.cuh"
+#include "sgmv_grid.cuh"
+#include "sgmv_stream.cuh"
+
+namespace plora {
+
+// n / d for 0 <= n < 2^31 by a multiplication (Granlund and Montgomery, 1994).
+struct FastDiv {
+  uint32_t d, m, s;
+  __host__ void set(uint32_t div) {
+    d = div;
+    s = 0;
+    while ((1ull << s) < div) ++s;
+    m = (uint32_t)(((1ull << 32) * ((1ull << s) - div)) / div + 1);
+  }
+  __device__ __forceinline__ uint32_t div(uint32_t n) const { return (__umulhi(m, n) + n) >> s; }
+};
+
+struct PagedView {
+  void *k, *v;
+  const int32_t* table;   // (rows, max_pages)
+  int64_t table_stride;   // entries between rows
+  int64_t k_page, v_page; // elements between pages
+  int64_t capacity;       // positions a row's table reaches: max_pages * page_size
+  int32_t num_pages, kv_heads, page_size, dim;
+  FastDiv page;
+};
+
+// Elements of one 16-byte chunk as floats.
+template <typename T>
+struct Chunk;
+template <>
+struct Chunk<float> {
+  static constexpr int N = 4;
+  static __device__ __forceinline__ void load(const uint4& u, float* f) {
+    f[0] = __uint_as_float(u.x), f[1] = __uint_as_float(u.y), f[2] = __uint_as_float(u.z), f[3] = __uint_as_float(u.w);
+  }
+  static __device__ __forceinline__ uint4 store(const float* f) {
+    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  }
+  static __device__ __forceinline__ float get(float v) { return v; }
+  static __device__ __forceinline__ float put(float f) { return f; }
+};
+template <>
+struct Chunk<__nv_bfloat16> {
+  static constexpr int N = 8;
+  static __device__ __forceinline__ void load(const uint4& u, float* f) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[2 * i] = __uint_as_float(w[i] << 16), f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+  static __device__ __forceinline__ uint4 store(const float* f) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  static __device__ __forceinline__ float get(__nv_bfloat16 v) { return __bfloat162float(v); }
+  static __device__ __forceinline__ __nv_bfloat16 put(float f) { return __float2bfloat16_rn(f); }
+};
+template <>
+struct Chunk<__half> {
+  static constexpr int N = 8;
+  static __device__ __forceinline__ void load(const uint4& u, float* f) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      f[2 * i] = p.x, f[2 * i + 1] = p.y;
+    }
+  }
+  static __device__ __forceinline__ uint4 store(const float* f) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __half2 h = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  static __device__ __forceinline__ float get(__half v) { return __half2float(v); }
+  static __device__ __forceinline__ __half put(float f) { return __float2half_rn(f); }
+};
+
+// ---------------------------------------------------------------- append
+// Token (b, m), m < new_lens[b], has position past_lens[b] + m.  Its queries
+// and keys are rotated by the angle position * f_i of each pair i of head
+// elements, (x, y) -> (x cos - y sin, y cos + x sin), keys and values go to the
+// row's pages, rotated queries (and keys, if wanted) to dense outputs.
+//
+// The angle is kept as a fraction of a turn: phases[i] = round(f_i / 2 pi * 2^64),
+// and position * phases[i] mod 2^64 is an exact integer product, so far
+// positions lose nothing (a 32-bit float product is off by 2^-24 of the angle,
+// 0.008 rad at position 131072).
+constexpr int kAppendThreads = 256;
+constexpr int kAppendTokens = 4;   // most tokens of a CTA
+constexpr int kAppendPairs = 128;  // most rotated pairs of a head (head_dim <= 256)
+
+struct AppendParams {
+  PagedView c;
+  const void *q, *k, *v;
+  void *q_out, *k_out;  // dense (rows, max_new, heads, dim); q_out null when q is, k_out may be null
+  int64_t q_row, q_tok, q_head, k_row, k_tok, k_head, v_row, v_tok, v_head;  // strides in elements
+  const int32_t *past, *news;  // news null: every row has max_new tokens
+  const uint64_t* phases;      // null: no rotation (pairs 0)
+  int32_t q_heads, pairs, interleaved, max_new, tokens, cta_tokens;
+  float scale;
+  FastDiv by_new, by_item, by_head;  // max_new; items of a token; items of a head
+};
+
+// Rotates element j of a head vector from its parts (the slow path: pairs that
+// do not fill 16-byte chunks).
+template <typename T>
+__device__ __forceinline__ float rotated_at(const T* x, int j, const float2* cs, int pairs, int interleaved) {
+  const float a = Chunk<T>::get(x[j]);
+  if (j >= 2 * pairs) return a;
+  const int i = interleaved ? j >> 1 : (j < pairs ? j : j - pairs);
+  const bool first = interleaved ? !(j & 1) : j < pairs;
+  const float b = Chunk<T>::get(x[interleaved ? j ^ 1 : (first ? j + pairs : j - pairs)]);
+  return first ? a * cs[i].x - b * cs[i].y : a * cs[i].x + b * cs[i].y;
+}
+
+// One CTA takes cta_tokens tokens; a thread's item is two 16-byte chunks of a
+// head vector, which hold whole pairs when VEC (each element is then read
+// once): chunks c and c + pairs / N in halves, 2c and 2c + 1 interleaved.  The
+// cosines of a token are computed once and shared by all of its heads.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const AppendParams p) {
+  constexpr int N = Chunk<T>::N;
+  __shared__ float2 cs[kAppendTokens][kAppendPairs];
+  __shared__ int32_t s_page[kAppendTokens];  // -2: padding; -1: no place in the cache
+  __shared__ int32_t s_slot[kAppendTokens];
+  griddep_wait();
+  griddep_launch();
+  const int tid = threadIdx.x;
+  const int t0 = blockIdx.x * p.cta_tokens;
+  const int nt = min(p.cta_tokens, p.tokens - t0);
+  const int pairs = p.pairs, dim = p.c.dim;
+
+  for (int i = tid; i < nt * max(pairs, 1); i += kAppendThreads) {
+    const int tok = pairs ? i / pairs : i, pr = pairs ? i - tok * pairs : 0;
+    const int b = p.by_new.div(t0 + tok), m = t0 + tok - b * p.max_new;
+    const int64_t pos = (int64_t)p.past[b] + m;
+    if (pairs) {
+      const uint64_t turn = (uint64_t)pos * p.phases[pr];
+      float s, c;
+      sincospif((float)(int32_t)(turn >> 32) * 0x1p-31f, &s, &c);  // half turns in [-1, 1]
+      cs[tok][pr] = make_float2(c * p.scale, s * p.scale);
+    }
+    if (pr == 0) {
+      int page = -2, slot = 0;
+      if (m < (p.news ? min(p.news[b], p.max_new) : p.max_new)) {
+        page = -1;
+        if (pos >= 0 && pos < p.c.capacity) {
+          const uint32_t e = p.c.page.div((uint32_t)pos);
+          slot = (int)((uint32_t)pos - e * p.c.page.d);
+          page = p.c.table[b * p.c.table_stride + e];
+          if ((uint32_t)page >= (uint32_t)p.c.num_pages) page = -1;
+        }
+        if (page < 0) raise_status(PLORA_DEV_PAGE_RANGE);
+      }
+      s_page[tok] = page;
+      s_slot[tok] = slot;
+    }
+  }
+  __syncthreads();
+
+  const int per_token = (int)p.by_item.d, per_head = (int)p.by_head.d;
+  const int rot = VEC && !p.interleaved ? pairs / N : 0;  // items of a head that hold both halves of their pairs
+  for (int i = tid; i < nt * per_token; i += kAppendThreads) {
+    const int tok = p.by_item.div(i);
+    int r = i - tok * per_token;
+    int head = p.by_head.div(r);
+    const int c = r - head * per_head;
+    const int t = t0 + tok, b = p.by_new.div(t), m = t - b * p.max_new;
+    const int page = s_page[tok];
+    // which tensor: q heads, then k heads, then v heads
+    const T* x;
+    T *dense = nullptr, *cache = nullptr;
+    bool turn = pairs > 0;
+    if (head < p.q_heads) {
+      x = (const T*)p.q + b * p.q_row + m * p.q_tok + head * p.q_head;
+      dense = (T*)p.q_out + ((int64_t)t * p.q_heads + head) * dim;
+    } else {
+      head -= p.q_heads;
+      const bool key = head < p.c.kv_heads;
+      if (!key) head -= p.c.kv_heads;
+      const int64_t at = ((int64_t)head * p.c.page_size + s_slot[tok]) * dim;
+      if (key) {
+        x = (const T*)p.k + b * p.k_row + m * p.k_tok + head * p.k_head;
+        if (p.k_out) dense = (T*)p.k_out + ((int64_t)t * p.c.kv_heads + head) * dim;
+        if (page >= 0) cache = (T*)p.c.k + page * p.c.k_page + at;
+      } else {
+        x = (const T*)p.v + b * p.v_row + m * p.v_tok + head * p.v_head;
+        if (page >= 0) cache = (T*)p.c.v + page * p.c.v_page + at;
+        turn = false;
+      }
+    }
+    const int first = c < rot ? c * N : 2 * c * N, e1 = first + (c < rot ? pairs : N);
+    const bool two = e1 < dim;
+    uint4 u0 = make_uint4(0, 0, 0, 0), u1 = u0;
+    if (page != -2) {
+      if (VEC || !turn) {
+        u0 = *reinterpret_cast<const uint4*>(x + first);
+        if (two) u1 = *reinterpret_cast<const uint4*>(x + e1);
+        if (turn) {
+          float a[N], d[N], y0[N], y1[N];
+          Chunk<T>::load(u0, a);
+          Chunk<T>::load(u1, d);
+          if (p.interleaved) {
+#pragma unroll
+            for (int j = 0; j < N; j += 2) {
+              const float2 w = first < 2 * pairs ? cs[tok][(first + j) >> 1] : make_float2(1.f, 0.f);
+              const float2 z = e1 < 2 * pairs ? cs[tok][(e1 + j) >> 1] : make_float2(1.f, 0.f);
+              y0[j] = a[j] * w.x - a[j + 1] * w.y, y0[j + 1] = a[j + 1] * w.x + a[j] * w.y;
+              y1[j] = d[j] * z.x - d[j + 1] * z.y, y1[j + 1] = d[j + 1] * z.x + d[j] * z.y;
+            }
+            if (first < 2 * pairs) u0 = Chunk<T>::store(y0);
+            if (e1 < 2 * pairs) u1 = Chunk<T>::store(y1);
+          } else if (c < rot) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+              const float2 w = cs[tok][first + j];
+              y0[j] = a[j] * w.x - d[j] * w.y;
+              y1[j] = d[j] * w.x + a[j] * w.y;
+            }
+            u0 = Chunk<T>::store(y0);
+            u1 = Chunk<T>::store(y1);
+          }
+        }
+      } else {
+        float y[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) y[j] = rotated_at(x, first + j, cs[tok], pairs, p.interleaved);
+        u0 = Chunk<T>::store(y);
+        if (two) {
+#pragma unroll
+          for (int j = 0; j < N; ++j) y[j] = rotated_at(x, e1 + j, cs[tok], pairs, p.interleaved);
+          u1 = Chunk<T>::store(y);
+        }
+      }
+    }
+    if (dense) {
+      *reinterpret_cast<uint4*>(dense + first) = u0;
+      if (two) *reinterpret_cast<uint4*>(dense + e1) = u1;
+    }
+    if (cache) {
+      *reinterpret_cast<uint4*>(cache + first) = u0;
+      if (two) *reinterpret_cast<uint4*>(cache + e1) = u1;
+    }
+  }
+}
+
+// ---------------------------------------------------------------- attention
+// out[b, h] = sum_j softmax_j(scale * q[b, h] . k_j) v_j over the last
+// min(window, seq_lens[b]) of a row's seq_lens[b] cached tokens; zeros where
+// there are none.  One pass over the cache with a running maximum and sum.
+//
+// Bound by HBM: the cache is read once, 4 * group flops for each 2 * elem
+// bytes.  The rows' lengths are known on the device only, so the work is cut
+// there: an item is a row and a key-value head (or a block of its query
+// heads), a tile 16 of its tokens, and the tiles of all items in order are
+// dealt in equal contiguous shares to the grid's warps, each of which streams
+// its share through a ring of shared-memory stages of its own (cp.async, no
+// barrier between warps).  An item cut by a share's end leaves partial sums in
+// the workspace, which attn_join_kernel adds in the order of the shares; every
+// item has at least one (empty) tile, so rows without tokens are written too.
+constexpr int kAttnTile = 16;
+
+struct AttnParams {
+  PagedView c;
+  const void* q;
+  void* out;  // dense (rows, heads, dim)
+  const int32_t* seq_lens;
+  int64_t q_row, q_head;
+  int32_t rows, group, blocks, block_heads, window;  // blocks of block_heads query heads cover a group
+  float scale_log2;                                  // scale * log2(e)
+  // workspace: two partials a worker (slot 0: its first item, begun by another; 1: its last, that goes on)
+  float* part_o;    // (workers, 2, block_heads, dim)
+  float2* part_ml;  // (workers, 2, block_heads): maximum (in units of scale_log2), sum
+  int4* desc;       // (workers): row, head block, pieces of the item that begins and is cut here (pieces 0: none)
+};
+
+struct AttnRow {
+  int lo, n;   // tokens [lo, n)
+  int t0, t1;  // tiles [t0, t1), at least one
+};
+__device__ __forceinline__ AttnRow attn_row(const AttnParams& p, int row) {
+  AttnRow r;
+  int64_t n = p.seq_lens[row];
+  n = n < 0 ? 0 : (n > p.c.capacity ? p.c.capacity : n);
+  r.n = (int)n;
+  r.lo = p.window > 0 ? max(0, r.n - p.window) : 0;
+  r.t0 = r.lo / kAttnTile;
+  r.t1 = max(r.t0 + 1, (r.n + kAttnTile - 1) / kAttnTile);
+  return r;
+}
+
+// A position in the list of all tiles.
+struct AttnCursor {
+  int row, head, tile;  // head: head block of the row, kv_head * blocks + block
+  AttnRow r;
+  __device__ __forceinline__ void next(const AttnParams& p) {
+    if (++tile < r.t1) return;
+    if (++head == p.c.kv_heads * p.blocks) {
+      head = 0;
+      if (++row < p.rows) r = attn_row(p, row);
+    }
+    tile = r.t0;
+  }
+};
+
+struct AttnShare {
+  int64_t begin, end;   // tiles of this warp
+  int64_t total;        // tiles of all items
+  int workers, worker;  // warps with a share
+  AttnCursor at;        // at `begin`
+};
+
+// Sum over the CTA's threads before this one (exclusive) and over all of them.
+template <int WARPS>
+__device__ __forceinline__ int block_scan(int v, int* s_warp, int* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int incl = v;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, incl, d);
+    if (lane >= d) incl += u;
+  }
+  __syncthreads();
+  if (lane == 31) s_warp[warp] = incl;
+  __syncthreads();
+  int before = 0, sum = 0;
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) {
+    if (w < warp) before += s_warp[w];
+    sum += s_warp[w];
+  }
+  *total = sum;
+  return before + incl - v;
+}
+
+// The calling warp's share.  Block-collective; warps without one get begin == end.
+template <int WARPS>
+__device__ __forceinline__ AttnShare attn_share(const AttnParams& p) {
+  constexpr int THREADS = WARPS * 32;
+  __shared__ int s_warp[WARPS];
+  __shared__ int s_row[WARPS];
+  __shared__ int64_t s_before[WARPS], s_begin[WARPS];
+  const int tid = threadIdx.x, warp = tid >> 5;
+  const int per_row = p.c.kv_heads * p.blocks;
+  int64_t tiles = 0;
+  for (int base = 0; base < p.rows; base += THREADS) {
+    int n = 0, sum;
+    if (base + tid < p.rows) {
+      const AttnRow r = attn_row(p, base + tid);
+      n = r.t1 - r.t0;
+    }
+    block_scan<WARPS>(n, s_warp, &sum);
+    tiles += sum;
+  }
+  AttnShare s;
+  s.total = tiles * per_row;
+  // worker w of the grid is warp w / gridDim.x of CTA w % gridDim.x: few shares spread over the SMs
+  const int all = gridDim.x * WARPS;
+  s.workers = s.total < all ? (int)s.total : all;
+  s.worker = warp * gridDim.x + blockIdx.x;
+  s.begin = s.end = 0;
+  if (s.worker < s.workers) {
+    s.begin = s.total * s.worker / s.workers;
+    s.end = s.total * (s.worker + 1) / s.workers;
+  }
+  if ((tid & 31) == 0) s_begin[warp] = s.begin < s.end ? s.begin : -1;  // the scan's barriers publish it
+  int64_t before = 0;
+  for (int base = 0; base < p.rows; base += THREADS) {
+    int n = 0, sum;
+    if (base + tid < p.rows) {
+      const AttnRow r = attn_row(p, base + tid);
+      n = r.t1 - r.t0;
+    }
+    const int64_t mine = before + block_scan<WARPS>(n, s_warp, &sum);
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      const int64_t x = s_begin[w];
+      if (x >= mine * per_row && x < (mine + n) * per_row) {
+        s_row[w] = base + tid;
+        s_before[w] = mine;
+      }
+    }
+    before += sum;
+  }
+  __syncthreads();
+  if (s.begin < s.end) {
+    s.at.row = s_row[warp];
+    s.at.r = attn_row(p, s.at.row);
+    const int n = s.at.r.t1 - s.at.r.t0;
+    const int rest = (int)(s.begin - s_before[warp] * per_row);
+    s.at.head = rest / n;
+    s.at.tile = s.at.r.t0 + rest - s.at.head * n;
+  }
+  return s;
+}
+
+// cp_async16 that writes zeros instead where `ok` is false.
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool ok) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Shared-memory layout of a tile: 16 rows of DP elements, 16-byte chunks of a
+// row exchanged by row & 7, so that 8 rows of one chunk lie in 8 bank groups.
+template <int EB, int DP>
+struct AttnTileCfg {
+  static constexpr int kChunks = DP * EB / 16;         // of a padded row
+  static constexpr int kRowBytes = DP * EB;
+  static constexpr int kTileBytes = kAttnTile * kRowBytes;
+  static constexpr int kStageBytes = 2 * kTileBytes;   // keys, values
+  static __device__ __forceinline__ uint32_t offset(int row, int chunk) {
+    return row * kRowBytes + ((chunk ^ (row & 7)) << 4);
+  }
+};
+
+// Copies the tiles of a share into a warp's stages.  The page of a tile's
+// tokens is looked up one tile ahead (lane l: token l & 15).
+template <int EB, int DP>
+struct AttnLoader {
+  using Cfg = AttnTileCfg<EB, DP>;
+  AttnCursor at;
+  int64_t left;
+  int page, inner;  // of this lane's token of tile `at`; page -1: reads as zeros
+
+  __device__ __forceinline__ void look_up(const AttnParams& p) {
+    page = -1, inner = 0;
+    if (left <= 0) return;
+    const int pos = at.tile * kAttnTile + (threadIdx.x & 15);
+    if (pos >= at.r.lo && pos < at.r.n) {
+      const int e = p.c.page.div(pos);
+      page = p.c.table[at.row * p.c.table_stride + e];
+      if ((uint32_t)page >= (uint32_t)p.c.num_pages) {
+        raise_status(PLORA_DEV_PAGE_RANGE);
+        page = -1;
+      }
+      inner = ((at.head / p.blocks) * p.c.page_size + pos - e * p.c.page_size) * p.c.dim;
+    }
+  }
+  // Starts the copies of tile `at` (none past the share's end) and steps on.
+  __device__ __forceinline__ void issue(const AttnParams& p, uint32_t stage) {
+    if (left > 0) {
+      constexpr int LANES = Cfg::kChunks < 32 ? Cfg::kChunks : 32;  // lanes of a row
+      const int lane = threadIdx.x & 31, lc = lane % LANES;
+#pragma unroll
+      for (int r0 = 0; r0 < kAttnTile; r0 += 32 / LANES) {
+        const int row = r0 + lane / LANES;
+        const int pg = __shfl_sync(0xffffffffu, page, row), in = __shfl_sync(0xffffffffu, inner, row);
+        const bool ok = pg >= 0;
+        const char* k = (const char*)p.c.k + (ok ? (pg * p.c.k_page + in) * EB : 0);
+        const char* v = (const char*)p.c.v + (ok ? (pg * p.c.v_page + in) * EB : 0);
+#pragma unroll
+        for (int c = lc; c < Cfg::kChunks; c += LANES) {
+          if (c * (16 / EB) < p.c.dim) {  // columns past dim stay zero
+            const uint32_t d = stage + Cfg::offset(row, c);
+            cp_async16_or_zero(d, k + c * 16, ok);
+            cp_async16_or_zero(d + Cfg::kTileBytes, v + c * 16, ok);
+          }
+        }
+      }
+      at.next(p);
+      --left;
+      look_up(p);
+    }
+    cp_async_commit();
+  }
+};
+
+// Where a warp leaves the sums of the item it has finished its part of:
+// `begun` / `done`: the part holds the item's first / last tile.
+struct AttnPlace {
+  bool whole;
+  int64_t part;  // row of part_ml: ((worker * 2 + slot) * block_heads)
+};
+__device__ __forceinline__ AttnPlace attn_place(const AttnParams& p, const AttnShare& s, const AttnCursor& at,
+                                                int64_t pos, bool begun, bool done) {
+  AttnPlace o;
+  o.whole = begun && done;
+  o.part = (s.worker * 2ll + (begun ? 1 : 0)) * p.block_heads;
+  if (begun && !done && (threadIdx.x & 31) == 0) {  // the item goes on in later shares
+    const int64_t last = pos + (at.r.t1 - 1 - at.tile);  // its last tile
+    const int w = (int)(((last + 1) * s.workers - 1) / s.total);  // the worker whose share holds it
+    p.desc[s.worker] = make_int4(at.row, at.head, w - s.worker + 1, 0);
+  }
+  return o;
+}
+
+template <int EB, int DP>
+struct AttnSimtCfg {
+  using Tile = AttnTileCfg<EB, DP>;
+  static constexpr int kHeads = 8;  // query heads of a block
+  static constexpr int kStages = DP == 256 ? 2 : 3;
+  static constexpr int kWarps = DP == 256 ? 3 : (DP == 128 ? 4 : 8);
+  static constexpr int kQBytes = kHeads * DP * 4, kPBytes = kAttnTile * kHeads * 4;
+  static constexpr int kWarpBytes = kStages * Tile::kStageBytes + kQBytes + kPBytes;
+  static constexpr int kSmemBytes = kWarps * kWarpBytes;
+};
+
+// CUDA-core attention.  Scores: lanes l and l + 16 take token l & 15, each half
+// of the head's elements.  Sums: a lane owns DP / 32 elements of all heads.
+template <typename T, int DP>
+__global__ void __launch_bounds__(AttnSimtCfg<sizeof(T), DP>::kWarps * 32, 1) attn_simt_kernel(const AttnParams p) {
+  using Cfg = AttnSimtCfg<sizeof(T), DP>;
+  using Tile = AttnTileCfg<sizeof(T), DP>;
+  constexpr int H = Cfg::kHeads, N = Chunk<T>::N, E = DP / 32;
+  extern __shared__ __align__(128) unsigned char attn_smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  unsigned char* mine = attn_smem + warp * Cfg::kWarpBytes;
+  float* sq = reinterpret_cast<float*>(mine + Cfg::kStages * Tile::kStageBytes);  // [H][DP]
+  float* sp = sq + H * DP;                                                        // [16][H]
+  for (int i = lane; i < Cfg::kWarpBytes / 16; i += 32) reinterpret_cast<uint4*>(mine)[i] = make_uint4(0, 0, 0, 0);
+  griddep_wait();
+  griddep_launch();
+  const AttnShare s = attn_share<Cfg::kWarps>(p);
+  if (s.worker < gridDim.x * Cfg::kWarps && lane == 0) p.desc[s.worker] = make_int4(0, 0, 0, 0);
+  __syncwarp();
+  if (s.begin == s.end) return;
+
+  AttnLoader<sizeof(T), DP> load;
+  load.at = s.at;
+  load.left = s.end - s.begin;
+  load.look_up(p);
+  const uint32_t ring = smem_u32(mine);
+#pragma unroll
+  for (int i = 0; i < Cfg::kStages - 1; ++i) load.issue(p, ring + i * Tile::kStageBytes);
+
+  AttnCursor at = s.at;
+  bool begun = at.tile == at.r.t0, fresh = true;
+  float m[H], l[H], o[H][E];
+  int stage = 0;
+  for (int64_t pos = s.begin; pos < s.end; ++pos) {
+    const int kv = at.head / p.blocks, blk = at.head - kv * p.blocks;
+    const int h0 = blk * p.block_heads, nh = min(p.block_heads, p.group - h0);
+    if (fresh) {
+      const T* q = (const T*)p.q + at.row * p.q_row + (kv * p.group + h0) * p.q_head;
+      for (int h = 0; h < H; ++h)
+        for (int d = lane; d < p.c.dim; d += 32) sq[h * DP + d] = h < nh ? Chunk<T>::get(q[h * p.q_head + d]) * p.scale_log2 : 0.f;
+#pragma unroll
+      for (int h = 0; h < H; ++h) {
+        m[h] = -INFINITY, l[h] = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[h][e] = 0.f;
+      }
+      fresh = false;
+    }
+    cp_async_wait<Cfg::kStages - 2>();
+    __syncwarp();
+    // the stage read in the last round is free again
+    const int ahead = stage == 0 ? Cfg::kStages - 1 : stage - 1;
+    load.issue(p, ring + ahead * Tile::kStageBytes);
+
+    const unsigned char* ks = mine + stage * Tile::kStageBytes;
+    const int tok = lane & 15, half = lane >> 4;
+    float acc[H];
+#pragma unroll
+    for (int h = 0; h < H; ++h) acc[h] = 0.f;
+#pragma unroll 4
+    for (int c = half * (Tile::kChunks / 2); c < (half + 1) * (Tile::kChunks / 2); ++c) {
+      float kf[N];
+      Chunk<T>::load(*reinterpret_cast<const uint4*>(ks + Tile::offset(tok, c)), kf);
+#pragma unroll
+      for (int h = 0; h < H; ++h) {
+#pragma unroll
+        for (int j = 0; j < N; j += 4) {
+          const float4 qv = *reinterpret_cast<const float4*>(sq + h * DP + c * N + j);
+          acc[h] = fmaf(qv.x, kf[j], fmaf(qv.y, kf[j + 1], fmaf(qv.z, kf[j + 2], fmaf(qv.w, kf[j + 3], acc[h]))));
+        }
+      }
+    }
+    const int at_pos = at.tile * kAttnTile + tok;
+    const bool live = at_pos >= at.r.lo && at_pos < at.r.n;
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+      float x = acc[h] + __shfl_xor_sync(0xffffffffu, acc[h], 16);
+      x = live ? x : -INFINITY;
+      float mx = x;
+#pragma unroll
+      for (int d = 8; d; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+      const float m2 = fmaxf(m[h], mx), base = m2 == -INFINITY ? 0.f : m2;
+      const float keep = exp2f(m[h] - base), pr = exp2f(x - base);
+      m[h] = m2;
+      l[h] = l[h] * keep + (half ? 0.f : pr);  // per lane; added over the lanes at the item's end
+      if (half == 0) sp[tok * H + h] = pr;
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[h][e] *= keep;
+    }
+    __syncwarp();
+    const unsigned char* vs = ks + Tile::kTileBytes;
+#pragma unroll 2
+    for (int t = 0; t < kAttnTile; ++t) {
+      float vf[E];
+#pragma unroll
+      for (int e = 0; e < E; e += 2) {  // elements 2 lane, 2 lane + 1 of every 64
+        const int d = e * 32 + 2 * lane;
+        const T* src = reinterpret_cast<const T*>(vs + Tile::offset(t, d / N)) + d % N;
+        vf[e] = Chunk<T>::get(src[0]), vf[e + 1] = Chunk<T>::get(src[1]);
+      }
+#pragma unroll
+      for (int h = 0; h < H; ++h) {
+        const float pr = sp[t * H + h];
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[h][e] = fmaf(pr, vf[e], o[h][e]);
+      }
+    }
+    stage = stage + 1 == Cfg::kStages ? 0 : stage + 1;
+
+    const bool done = at.tile + 1 == at.r.t1;
+    if (done || pos + 1 == s.end) {
+      const AttnPlace to = attn_place(p, s, at, pos, begun, done);
+#pragma unroll
+      for (int h = 0; h < H; ++h) {
+#pragma unroll
+        for (int d = 16; d; d >>= 1) l[h] += __shfl_xor_sync(0xffffffffu, l[h], d);
+        if (h >= nh) continue;
+        const float f = to.whole ? (l[h] > 0.f ? 1.f / l[h] : 0.f) : 1.f;
+        if (!to.whole && lane == 0) p.part_ml[to.part + h] = make_float2(m[h], l[h]);
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+          const int d = e * 32 + 2 * lane;
+          if (d >= p.c.dim) continue;
+          if (to.whole) {
+            T* out = (T*)p.out + ((int64_t)at.row * p.c.kv_heads * p.group + kv * p.group + h0 + h) * p.c.dim + d;
+            out[0] = Chunk<T>::put(o[h][e] * f), out[1] = Chunk<T>::put(o[h][e + 1] * f);
+          } else {
+            float* out = p.part_o + (to.part + h) * p.c.dim + d;
+            out[0] = o[h][e], out[1] = o[h][e + 1];
+          }
+        }
+      }
+      begun = true, fresh = true;
+    }
+    at.next(p);
+    __syncwarp();
+  }
+}
+
+// Joins the parts of the items that share ends cut.  CTA (w, h): head h of the
+// item that begins in worker w's share and goes on in the next ones, if there
+// is one; its warps take the parts in turn, a lane four elements.
+constexpr int kJoinWarps = 8;
+template <typename T>
+__global__ void __launch_bounds__(kJoinWarps * 32) attn_join_kernel(const AttnParams p) {
+  __shared__ float s_o[kJoinWarps][256];
+  __shared__ float s_l[kJoinWarps], s_m[kJoinWarps];
+  griddep_wait();
+  griddep_launch();
+  const int4 d = p.desc[blockIdx.x];
+  const int h = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (d.z == 0) return;
+  const int kv = d.y / p.blocks, blk = d.y - kv * p.blocks;
+  const int h0 = blk * p.block_heads, dim = p.c.dim;
+  if (h0 + h >= p.group) return;
+  float m = -INFINITY, l = 0.f, o[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) o[e] = 0.f;
+  for (int i = warp; i < d.z; i += kJoinWarps) {
+    const int64_t part = ((blockIdx.x + i) * 2ll + (i == 0 ? 1 : 0)) * p.block_heads + h;
+    const float2 ml = p.part_ml[part];
+    float4 a = make_float4(0, 0, 0, 0), b = a;
+    if (lane * 4 < dim) a = *reinterpret_cast<const float4*>(p.part_o + part * dim + lane * 4);
+    if (128 + lane * 4 < dim) b = *reinterpret_cast<const float4*>(p.part_o + part * dim + 128 + lane * 4);
+    const float m2 = fmaxf(m, ml.x), base = m2 == -INFINITY ? 0.f : m2;
+    const float keep = exp2f(m - base), f = exp2f(ml.x - base);
+    m = m2;
+    l = l * keep + ml.y * f;
+    o[0] = o[0] * keep + a.x * f, o[1] = o[1] * keep + a.y * f, o[2] = o[2] * keep + a.z * f, o[3] = o[3] * keep + a.w * f;
+    o[4] = o[4] * keep + b.x * f, o[5] = o[5] * keep + b.y * f, o[6] = o[6] * keep + b.z * f, o[7] = o[7] * keep + b.w * f;
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) s_o[warp][lane * 4 + e] = o[e], s_o[warp][128 + lane * 4 + e] = o[4 + e];
+  if (lane == 0) s_m[warp] = m, s_l[warp] = l;
+  __syncthreads();
+  float top = -INFINITY, sum = 0.f, f[kJoinWarps];
+#pragma unroll
+  for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, s_m[w]);
+  const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+  for (int w = 0; w < kJoinWarps; ++w) f[w] = exp2f(s_m[w] - base), sum += s_l[w] * f[w];
+  const float inv = sum > 0.f ? 1.f / sum : 0.f;
+  T* out = (T*)p.out + ((int64_t)d.x * p.c.kv_heads * p.group + kv * p.group + h0 + h) * dim;
+  for (int e = threadIdx.x; e < dim; e += kJoinWarps * 32) {
+    float x = 0.f;
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) x += s_o[w][e] * f[w];
+    out[e] = Chunk<T>::put(x * inv);
+  }
+}
+
+}  // namespace plora

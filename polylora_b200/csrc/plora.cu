@@ -16,6 +16,8 @@
 #include "sgmv_grid.cuh"
 #include "host_rows.cuh"
 #include "sgmv_stream.cuh"
+#include "paged.cuh"
+#include "logits.cuh"
 #include "peft_pack.h"
 
 using namespace plora;
@@ -147,6 +149,19 @@ int device_info(DeviceInfo** out) {
     SET_GRID((sgmv_expand_stream_kernel<true>), kStreamSmemLimit)
     SET_GRID((sgmv_expand_stream_kernel<false>), kStreamSmemLimit)
     SET_GRID(seg_scan_place_kernel, (kSegScanPlaceMaxInts + kSegMaxSlots + 1) * 4)
+#define SET_ATTN(T, DP) SET_GRID((attn_simt_kernel<T, DP>), (AttnSimtCfg<sizeof(T), DP>::kSmemBytes))
+#define SET_PAGED(T)                                     \
+  SET_ATTN(T, 64)                                        \
+  SET_ATTN(T, 128)                                       \
+  SET_ATTN(T, 256)                                       \
+  SET_GRID((logit_rules_kernel<T, int32_t>), kRulesSmem) \
+  SET_GRID((logit_rules_kernel<T, int64_t>), kRulesSmem)
+    constexpr int kRulesSmem = kRulesChunk * 6 + kRulesMaxBiases * 5;
+    SET_PAGED(float)
+    SET_PAGED(__half)
+    SET_PAGED(__nv_bfloat16)
+#undef SET_PAGED
+#undef SET_ATTN
 #undef SET_GRID
     // the row copies use no shared memory; an SM running them keeps its largest
     // shared-memory carveout, so the segment-table kernels of the next rows of
@@ -623,6 +638,104 @@ int token_rows_impl(const void* host_rows, void* device_rows, bool to_host, int6
   return PLORA_OK;
 }
 
+// ---------------------------------------------------------------- paged cache
+// SMs of a B200: the attention grid, so that its workspace does not depend on the device.
+constexpr int kAttnGrid = 148;
+constexpr int64_t kPagedMaxRows = 1 << 20;
+
+int attn_padded_dim(int64_t dim) { return dim <= 64 ? 64 : (dim <= 128 ? 128 : 256); }
+
+// Query heads of a block and warps of a CTA of the kernel that runs a call.
+struct AttnPlan {
+  int blocks, block_heads, warps;
+  size_t ml_offset, desc_offset, bytes;
+};
+AttnPlan attn_plan(int32_t heads, int32_t kv_heads, int32_t dim, int dtype) {
+  AttnPlan a;
+  const int group = heads / kv_heads;
+  const int dp = attn_padded_dim(dim);
+  const int most = 8;
+  if (dtype == PLORA_DTYPE_F32)
+    a.warps = dp == 64 ? AttnSimtCfg<4, 64>::kWarps : (dp == 128 ? AttnSimtCfg<4, 128>::kWarps : AttnSimtCfg<4, 256>::kWarps);
+  else
+    a.warps = dp == 64 ? AttnSimtCfg<2, 64>::kWarps : (dp == 128 ? AttnSimtCfg<2, 128>::kWarps : AttnSimtCfg<2, 256>::kWarps);
+  a.blocks = (group + most - 1) / most;
+  a.block_heads = (group + a.blocks - 1) / a.blocks;
+  a.blocks = (group + a.block_heads - 1) / a.block_heads;
+  const size_t workers = (size_t)kAttnGrid * a.warps, parts = workers * 2 * a.block_heads;
+  a.ml_offset = align256(parts * dim * 4);
+  a.desc_offset = a.ml_offset + align256(parts * 8);
+  a.bytes = a.desc_offset + align256(workers * 16);
+  return a;
+}
+
+// Arguments that both paged entry points share.
+int paged_view(PagedView* c, const void* k_cache, const void* v_cache, int64_t k_page_stride, int64_t v_page_stride,
+               const int32_t* page_table, int64_t table_stride, int64_t rows, int32_t heads, int32_t kv_heads,
+               int32_t head_dim, int32_t page_size, int64_t num_pages, int64_t max_pages, int32_t dtype) {
+  if (!valid_dtype(dtype)) return fail(PLORA_ERR_INVALID_ARGUMENT, "unknown dtype %d", dtype);
+  if (rows < 0 || kv_heads < 1 || heads < 0 || head_dim < 1 || page_size < 1 || num_pages < 1 || max_pages < 1)
+    return fail(PLORA_ERR_INVALID_ARGUMENT, "rows, heads, head_dim, page_size or page counts not positive");
+  if (heads % kv_heads) return fail(PLORA_ERR_INVALID_ARGUMENT, "%d heads over %d kv heads", heads, kv_heads);
+  if (head_dim % 8 || head_dim > 256)
+    return fail(PLORA_ERR_UNSUPPORTED, "head_dim %d is no multiple of 8 up to 256", head_dim);
+  if (rows > kPagedMaxRows || heads > 65535 || kv_heads > 65535)
+    return fail(PLORA_ERR_UNSUPPORTED, "%lld rows, %d heads", (long long)rows, heads);
+  if (num_pages > INT32_MAX || max_pages > INT32_MAX / page_size)
+    return fail(PLORA_ERR_UNSUPPORTED, "num_pages, or positions of max_pages pages, beyond int32");
+  const int64_t page_elems = (int64_t)kv_heads * head_dim;  // kv_heads <= 65535, head_dim <= 256
+  if (page_elems > INT32_MAX / page_size) return fail(PLORA_ERR_UNSUPPORTED, "elements of a page beyond int32");
+  if (k_page_stride < page_elems * page_size || v_page_stride < page_elems * page_size || table_stride < max_pages)
+    return fail(PLORA_ERR_INVALID_ARGUMENT, "page or page-table stride below its extent");
+  const int64_t vec = 16 / (int64_t)elem_size(dtype);
+  if (k_page_stride % vec || v_page_stride % vec || !aligned16(k_cache) || !aligned16(v_cache))
+    return fail(PLORA_ERR_INVALID_ARGUMENT, "cache pages must be 16-byte aligned");
+  if (num_pages > INT64_MAX / 16 / std::max(k_page_stride, v_page_stride))
+    return fail(PLORA_ERR_INVALID_ARGUMENT, "cache size overflows");
+  if (rows > 0 && (!k_cache || !v_cache || !page_table)) return fail(PLORA_ERR_INVALID_ARGUMENT, "null pointer");
+  c->k = const_cast<void*>(k_cache);
+  c->v = const_cast<void*>(v_cache);
+  c->table = page_table;
+  c->table_stride = table_stride;
+  c->k_page = k_page_stride;
+  c->v_page = v_page_stride;
+  c->capacity = max_pages * page_size;
+  c->num_pages = (int32_t)num_pages;
+  c->kv_heads = kv_heads;
+  c->page_size = page_size;
+  c->dim = head_dim;
+  c->page.set((uint32_t)page_size);
+  return PLORA_OK;
+}
+
+template <typename T>
+cudaError_t launch_append(const AppendParams& p, bool vec, unsigned grid, cudaStream_t s) {
+  return vec ? launch_kernel(paged_append_kernel<T, true>, dim3(grid), dim3(kAppendThreads), 0, s, true, 0, p)
+             : launch_kernel(paged_append_kernel<T, false>, dim3(grid), dim3(kAppendThreads), 0, s, true, 0, p);
+}
+
+template <typename T, int DP>
+cudaError_t launch_attn_simt(const AttnParams& p, cudaStream_t s) {
+  using Cfg = AttnSimtCfg<sizeof(T), DP>;
+  return launch_kernel(attn_simt_kernel<T, DP>, dim3(kAttnGrid), dim3(Cfg::kWarps * 32), Cfg::kSmemBytes, s, true, 0, p);
+}
+template <typename T>
+cudaError_t launch_attn(const AttnParams& p, const AttnPlan& a, cudaStream_t s) {
+  const int dp = attn_padded_dim(p.c.dim);
+  cudaError_t e = dp == 64 ? launch_attn_simt<T, 64>(p, s)
+                           : (dp == 128 ? launch_attn_simt<T, 128>(p, s) : launch_attn_simt<T, 256>(p, s));
+  if (e != cudaSuccess) return e;
+  return launch_kernel(attn_join_kernel<T>, dim3((unsigned)(kAttnGrid * a.warps), (unsigned)a.block_heads),
+                       dim3(kJoinWarps * 32), 0, s, true, 0, p);
+}
+
+template <typename T>
+cudaError_t launch_rules(const RulesParams& p, bool wide, int64_t rows, size_t smem, cudaStream_t s) {
+  const dim3 grid((unsigned)((p.vocab + kRulesChunk - 1) / kRulesChunk), (unsigned)rows);
+  return wide ? launch_kernel(logit_rules_kernel<T, int64_t>, grid, dim3(kRulesThreads), smem, s, true, 0, p)
+              : launch_kernel(logit_rules_kernel<T, int32_t>, grid, dim3(kRulesThreads), smem, s, true, 0, p);
+}
+
 }  // namespace
 
 extern "C" {
@@ -921,6 +1034,156 @@ int plora_slot_fill(const plora_slot_module* modules, int32_t num_modules, int32
   else
     slot_fill_kernel<__half><<<grid, block, 0, s>>>(modules, num_modules, slot, max_rank, img, nbytes);
   return check_launch("slot_fill_kernel");
+}
+
+int plora_paged_append(const void* q, int64_t q_row_stride, int64_t q_token_stride, int64_t q_head_stride,
+                       const void* k, int64_t k_row_stride, int64_t k_token_stride, int64_t k_head_stride,
+                       const void* v, int64_t v_row_stride, int64_t v_token_stride, int64_t v_head_stride,
+                       void* q_out, void* k_out, void* k_cache, void* v_cache, int64_t k_page_stride,
+                       int64_t v_page_stride, const int32_t* page_table, int64_t table_stride,
+                       const int32_t* past_lens, const int32_t* new_lens, const int64_t* phases, int32_t pairs,
+                       int32_t interleaved, float rotary_scale, int64_t rows, int64_t max_new, int32_t q_heads,
+                       int32_t kv_heads, int32_t head_dim, int32_t page_size, int64_t num_pages, int64_t max_pages,
+                       int32_t dtype, void* stream) {
+  g_last_error.clear();
+  AppendParams p = {};
+  int st = paged_view(&p.c, k_cache, v_cache, k_page_stride, v_page_stride, page_table, table_stride, rows,
+                      q ? q_heads : 0, kv_heads, head_dim, page_size, num_pages, max_pages, dtype);
+  if (st) return st;
+  if (max_new < 0 || pairs < 0 || 2 * (int64_t)pairs > head_dim)
+    return fail(PLORA_ERR_INVALID_ARGUMENT, "max_new negative, or %d rotated pairs in a head of %d", pairs, head_dim);
+  if (!token_count_ok(rows, max_new)) return fail(PLORA_ERR_UNSUPPORTED, "rows * max_new beyond int32");
+  if (rows == 0 || max_new == 0) return PLORA_OK;
+  if (!k || !v || !past_lens || (q && !q_out) || (pairs && !phases))
+    return fail(PLORA_ERR_INVALID_ARGUMENT, "null pointer");
+  const int64_t vec = 16 / (int64_t)elem_size(dtype);
+  const int64_t strides[9] = {q ? q_row_stride : 0, q ? q_token_stride : 0, q ? q_head_stride : 0,
+                              k_row_stride, k_token_stride, k_head_stride, v_row_stride, v_token_stride, v_head_stride};
+  for (int64_t x : strides)
+    if (x < 0 || x % vec) return fail(PLORA_ERR_INVALID_ARGUMENT, "token strides must be multiples of 16 bytes");
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(q_out) || !aligned16(k_out))
+    return fail(PLORA_ERR_INVALID_ARGUMENT, "token pointers must be 16-byte aligned");
+  DeviceInfo* di = nullptr;
+  if ((st = device_info(&di))) return st;
+  p.q = q, p.k = k, p.v = v, p.q_out = q_out, p.k_out = k_out;
+  p.q_row = strides[0], p.q_tok = strides[1], p.q_head = strides[2];
+  p.k_row = strides[3], p.k_tok = strides[4], p.k_head = strides[5];
+  p.v_row = strides[6], p.v_tok = strides[7], p.v_head = strides[8];
+  p.past = past_lens, p.news = new_lens;
+  p.phases = reinterpret_cast<const uint64_t*>(phases);
+  p.q_heads = q ? q_heads : 0;
+  p.pairs = pairs, p.interleaved = interleaved != 0, p.scale = rotary_scale;
+  p.max_new = (int32_t)max_new, p.tokens = (int32_t)(rows * max_new);
+  // one token a CTA until that fills the SMs
+  p.cta_tokens = p.tokens <= 8 * di->sm_count ? 1 : kAppendTokens;
+  const int n = (int)vec, per_head = (head_dim / n + 1) / 2;
+  p.by_new.set((uint32_t)max_new);
+  p.by_head.set((uint32_t)per_head);
+  p.by_item.set((uint32_t)(per_head * (p.q_heads + 2 * kv_heads)));
+  const bool whole = interleaved ? 2 * pairs % n == 0 : pairs % n == 0;
+  const unsigned grid = (unsigned)((p.tokens + p.cta_tokens - 1) / p.cta_tokens);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t e = dtype == PLORA_DTYPE_F32   ? launch_append<float>(p, whole, grid, s)
+                  : dtype == PLORA_DTYPE_F16 ? launch_append<__half>(p, whole, grid, s)
+                                             : launch_append<__nv_bfloat16>(p, whole, grid, s);
+  PLORA_CUDA(e, "launch paged_append_kernel");
+  return PLORA_OK;
+}
+
+size_t plora_paged_attention_workspace(int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t dtype) {
+  if (!valid_dtype(dtype) || kv_heads < 1 || heads < 1 || heads % kv_heads || heads > 65535 || head_dim < 1 ||
+      head_dim > 256 || head_dim % 8)
+    return 0;
+  return attn_plan(heads, kv_heads, head_dim, dtype).bytes;
+}
+
+int plora_paged_attention(const void* q, int64_t q_row_stride, int64_t q_head_stride, const void* k_cache,
+                          const void* v_cache, int64_t k_page_stride, int64_t v_page_stride,
+                          const int32_t* page_table, int64_t table_stride, const int32_t* seq_lens, void* out,
+                          float scale, int64_t window, int64_t rows, int32_t heads, int32_t kv_heads,
+                          int32_t head_dim, int32_t page_size, int64_t num_pages, int64_t max_pages, int32_t dtype,
+                          void* workspace, size_t workspace_size, void* stream) {
+  g_last_error.clear();
+  AttnParams p = {};
+  int st = paged_view(&p.c, k_cache, v_cache, k_page_stride, v_page_stride, page_table, table_stride, rows, heads,
+                      kv_heads, head_dim, page_size, num_pages, max_pages, dtype);
+  if (st) return st;
+  if (heads < 1) return fail(PLORA_ERR_INVALID_ARGUMENT, "no heads");
+  if (window < 0) return fail(PLORA_ERR_INVALID_ARGUMENT, "window %lld is negative", (long long)window);
+  if (rows == 0) return PLORA_OK;
+  if (!q || !seq_lens || !out) return fail(PLORA_ERR_INVALID_ARGUMENT, "null pointer");
+  const size_t elem = elem_size(dtype);
+  if (q_row_stride < 0 || q_head_stride < 0 || q_row_stride * elem % 16 || q_head_stride * elem % 16 ||
+      !aligned16(q) || !aligned16(out))
+    return fail(PLORA_ERR_INVALID_ARGUMENT, "q and out must be 16-byte aligned, with q's strides multiples of 16 bytes");
+  const AttnPlan a = attn_plan(heads, kv_heads, head_dim, dtype);
+  if (!workspace || workspace_size < a.bytes)
+    return fail(PLORA_ERR_WORKSPACE, "attention workspace %zu < %zu bytes", workspace_size, a.bytes);
+  if (reinterpret_cast<uintptr_t>(workspace) % 256)
+    return fail(PLORA_ERR_INVALID_ARGUMENT, "workspace must be 256-byte aligned");
+  DeviceInfo* di = nullptr;
+  if ((st = device_info(&di))) return st;
+  p.q = q, p.out = out, p.seq_lens = seq_lens;
+  p.q_row = q_row_stride, p.q_head = q_head_stride;
+  p.rows = (int32_t)rows, p.group = heads / kv_heads, p.blocks = a.blocks, p.block_heads = a.block_heads;
+  p.window = (int32_t)std::min<int64_t>(window, INT32_MAX);
+  p.scale_log2 = scale * 1.4426950408889634f;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  p.part_o = reinterpret_cast<float*>(ws);
+  p.part_ml = reinterpret_cast<float2*>(ws + a.ml_offset);
+  p.desc = reinterpret_cast<int4*>(ws + a.desc_offset);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t e = dtype == PLORA_DTYPE_F32   ? launch_attn<float>(p, a, s)
+                  : dtype == PLORA_DTYPE_F16 ? launch_attn<__half>(p, a, s)
+                                             : launch_attn<__nv_bfloat16>(p, a, s);
+  PLORA_CUDA(e, "launch paged attention");
+  return PLORA_OK;
+}
+
+int plora_logit_rules(const void* logits, int64_t logits_stride, void* out, int64_t out_stride, int64_t rows,
+                      int64_t vocab, int32_t dtype, const void* tokens, int64_t tokens_stride, int64_t history,
+                      const int32_t* token_lens, const int32_t* prompt_lens, const float* repetition,
+                      const float* presence, const float* frequency, const void* bias_tokens,
+                      int64_t bias_tokens_stride, const float* bias_values, int64_t bias_values_stride,
+                      int64_t biases, const int32_t* allowed, int64_t allowed_stride, int32_t token_bytes,
+                      void* stream) {
+  g_last_error.clear();
+  if (!valid_dtype(dtype)) return fail(PLORA_ERR_INVALID_ARGUMENT, "unknown dtype %d", dtype);
+  if (rows < 0 || vocab < 0 || history < 0 || biases < 0)
+    return fail(PLORA_ERR_INVALID_ARGUMENT, "negative rows, vocab, history or biases");
+  if (token_bytes != 4 && token_bytes != 8) return fail(PLORA_ERR_INVALID_ARGUMENT, "token ids of %d bytes", token_bytes);
+  if (rows > 65535 || vocab > INT32_MAX || history > (1 << 30) - 1 || biases > kRulesMaxBiases)
+    return fail(PLORA_ERR_UNSUPPORTED, "rows > 65535, vocab or history beyond 2^30, or more than %d biases a row",
+                kRulesMaxBiases);
+  if (rows == 0 || vocab == 0) return PLORA_OK;
+  if (!logits || !out || (history && !tokens) || (biases && (!bias_tokens || !bias_values)))
+    return fail(PLORA_ERR_INVALID_ARGUMENT, "null pointer");
+  if (logits_stride < vocab || out_stride < vocab || (history && tokens_stride < 0) ||
+      (biases && (bias_tokens_stride < 0 || bias_values_stride < 0)) ||
+      (allowed && allowed_stride < 0))
+    return fail(PLORA_ERR_INVALID_ARGUMENT, "row strides below the vocabulary, or negative");
+  const uintptr_t el = elem_size(dtype) - 1;
+  if ((reinterpret_cast<uintptr_t>(logits) & el) || (reinterpret_cast<uintptr_t>(out) & el))
+    return fail(PLORA_ERR_INVALID_ARGUMENT, "logits or out not aligned to its type");
+  DeviceInfo* di = nullptr;
+  int st = device_info(&di);
+  if (st) return st;
+  RulesParams p = {};
+  p.x = logits, p.y = out, p.x_row = logits_stride, p.y_row = out_stride, p.vocab = vocab;
+  p.tokens = tokens, p.token_row = tokens_stride, p.history = (int32_t)history;
+  p.token_lens = token_lens, p.prompt_lens = prompt_lens;
+  p.repetition = repetition, p.presence = presence, p.frequency = frequency;
+  p.bias_tokens = bias_tokens, p.bias_row = bias_tokens_stride;
+  p.bias_values = bias_values, p.value_row = bias_values_stride, p.biases = (int32_t)biases;
+  p.allowed = reinterpret_cast<const uint32_t*>(allowed), p.mask_row = allowed_stride;
+  const size_t smem = history || biases ? (size_t)kRulesChunk * 6 + (size_t)biases * 5 : 0;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool wide = token_bytes == 8;
+  cudaError_t e = dtype == PLORA_DTYPE_F32   ? launch_rules<float>(p, wide, rows, smem, s)
+                  : dtype == PLORA_DTYPE_F16 ? launch_rules<__half>(p, wide, rows, smem, s)
+                                             : launch_rules<__nv_bfloat16>(p, wide, rows, smem, s);
+  PLORA_CUDA(e, "launch logit_rules_kernel");
+  return PLORA_OK;
 }
 
 // Device address of g_noalloc_scratch, looked up once per device and CUDA

@@ -1,0 +1,124 @@
+"""Each row's own rules on its logits: penalties, biases and masks.
+
+As every row of a batch picks its own adapter, every row carries its own
+sampling rules: :class:`LogitRules` holds them as device tensors and
+:func:`apply_logit_rules` applies all of them in one pass over the logits.
+The reference has no counterpart (it ends at the base model's output).
+"""
+
+from __future__ import annotations
+
+from dataclasses import dataclass, fields
+
+import torch
+
+from .paged import _call, _no_grad
+from .sgmv import _as, _require_cuda, dtype_code
+
+
+@dataclass
+class LogitRules:
+    """Rules of a batch of B rows; None leaves a rule out.
+
+    ``tokens`` (B, L) int32 or int64 with the first ``token_lens[b]`` (None: L)
+    of each row its history, of which the first ``prompt_lens[b]`` (None: 0)
+    are the prompt.  For a token of the history, x -> x / r where positive, else
+    x * r, with r = ``repetition_penalty[b]``; for one that the answer (the
+    history past the prompt) holds n > 0 times, x -> x - n *
+    ``frequency_penalty[b]`` - ``presence_penalty[b]``.  Then
+    ``bias_values[b, j]`` is added to token ``bias_tokens[b, j]`` (ids outside the
+    vocabulary, such as -1 for padding, are skipped, as in ``tokens``; biases of
+    one token add up), and tokens whose bit t % 32 of ``allowed[b, t // 32]``
+    (int32) is 0 become -inf.
+    """
+
+    tokens: torch.Tensor | None = None
+    token_lens: torch.Tensor | None = None
+    prompt_lens: torch.Tensor | None = None
+    repetition_penalty: torch.Tensor | None = None
+    presence_penalty: torch.Tensor | None = None
+    frequency_penalty: torch.Tensor | None = None
+    bias_tokens: torch.Tensor | None = None
+    bias_values: torch.Tensor | None = None
+    allowed: torch.Tensor | None = None
+
+    def tensors(self) -> list[torch.Tensor]:
+        return [t for t in (getattr(self, f.name) for f in fields(self)) if t is not None]
+
+
+def _rows_of(t: torch.Tensor, rows: int, name: str) -> torch.Tensor:
+    if t.dim() != 2 or t.shape[0] != rows:
+        raise ValueError(f"{name} must be 2D with {rows} rows, got {tuple(t.shape)}")
+    return t if t.shape[1] <= 1 or t.stride(1) == 1 else t.contiguous()
+
+
+def _per_row(t: torch.Tensor | None, rows: int, dtype: torch.dtype, name: str) -> torch.Tensor | None:
+    if t is None:
+        return None
+    if t.shape != (rows,):
+        raise ValueError(f"{name} must have shape ({rows},), got {tuple(t.shape)}")
+    return _as(t, dtype)
+
+
+def _ptr(t: torch.Tensor | None) -> int:
+    return t.data_ptr() if t is not None else 0
+
+
+def _row_stride(t: torch.Tensor | None) -> int:
+    return 0 if t is None else (t.stride(0) if t.shape[0] > 1 else t.shape[1])
+
+
+def apply_logit_rules(logits: torch.Tensor, rules: LogitRules, out: torch.Tensor | None = None) -> torch.Tensor:
+    """``rules`` on logits (B, V), computed in fp32 and rounded once to the
+    logits' dtype; into ``out`` (which may be ``logits``) or a new tensor."""
+    dev = _require_cuda(logits, *rules.tensors())
+    _no_grad(logits)
+    if logits.dim() != 2:
+        raise ValueError("logits must be (B, V)")
+    rows, vocab = logits.shape
+    if logits.shape[1] > 1 and logits.stride(1) != 1:
+        raise ValueError("logits rows must be contiguous")
+    if out is None:
+        out = torch.empty((rows, vocab), dtype=logits.dtype, device=dev)
+    elif out.shape != logits.shape or out.dtype != logits.dtype or out.device != dev or (vocab > 1 and out.stride(1) != 1):
+        raise ValueError("out must have the logits' shape, dtype and device, with contiguous rows")
+    tokens, bias_tokens, bias_values, allowed = rules.tokens, rules.bias_tokens, rules.bias_values, rules.allowed
+    width = None
+    for name, t in (("tokens", tokens), ("bias_tokens", bias_tokens)):
+        if t is not None and t.dtype not in (torch.int32, torch.int64):
+            raise TypeError(f"{name} must be int32 or int64, got {t.dtype}")
+    if tokens is not None:
+        tokens = _rows_of(tokens, rows, "tokens")
+        width = tokens.dtype
+    elif any(t is not None for t in (rules.token_lens, rules.prompt_lens, rules.repetition_penalty,
+                                     rules.presence_penalty, rules.frequency_penalty)):
+        raise ValueError("penalties and lengths need tokens")
+    if (bias_tokens is None) != (bias_values is None):
+        raise ValueError("bias_tokens and bias_values go together")
+    if bias_tokens is not None:
+        if bias_tokens.shape != bias_values.shape:
+            raise ValueError("bias_tokens and bias_values must have one shape")
+        bias_tokens = _rows_of(bias_tokens, rows, "bias_tokens")
+        if width is not None and bias_tokens.dtype != width:  # both as the wider: narrowing could alias ids
+            tokens, bias_tokens = tokens.to(torch.int64), bias_tokens.to(torch.int64)
+        width = bias_tokens.dtype
+        bias_values = _rows_of(bias_values.to(torch.float32), rows, "bias_values")
+    if allowed is not None:
+        if allowed.dtype != torch.int32 or allowed.dim() != 2 or allowed.shape[1] < (vocab + 31) // 32:
+            raise ValueError(f"allowed must be int32 ({rows}, at least {(vocab + 31) // 32})")
+        allowed = _rows_of(allowed, rows, "allowed")
+    lens = _per_row(rules.token_lens, rows, torch.int32, "token_lens")
+    prompt = _per_row(rules.prompt_lens, rows, torch.int32, "prompt_lens")
+    rep = _per_row(rules.repetition_penalty, rows, torch.float32, "repetition_penalty")
+    pres = _per_row(rules.presence_penalty, rows, torch.float32, "presence_penalty")
+    freq = _per_row(rules.frequency_penalty, rows, torch.float32, "frequency_penalty")
+    _call(
+        dev, "plora_logit_rules",
+        logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, out.data_ptr(),
+        out.stride(0) if rows > 1 else vocab, rows, vocab, dtype_code(logits.dtype), _ptr(tokens),
+        _row_stride(tokens), tokens.shape[1] if tokens is not None else 0, _ptr(lens), _ptr(prompt), _ptr(rep),
+        _ptr(pres), _ptr(freq), _ptr(bias_tokens), _row_stride(bias_tokens), _ptr(bias_values),
+        _row_stride(bias_values), bias_tokens.shape[1] if bias_tokens is not None else 0, _ptr(allowed),
+        _row_stride(allowed), 4 if width == torch.int32 else 8,
+    )
+    return out

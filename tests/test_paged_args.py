@@ -1,0 +1,134 @@
+"""Refusals of the paged-cache and logit operators, and the rotation phases,
+on a machine without a GPU."""
+
+import math
+
+import pytest
+import torch
+
+from polylora_b200.logits import LogitRules, apply_logit_rules
+from polylora_b200.paged import _heads, paged_append, paged_attention, rotary_phases
+
+D = 0x1000  # stands for a device pointer; never dereferenced on the host
+
+
+def _append(lib, native, **kw):
+    a = dict(q=D, qs=(2048, 1024, 64), k=D, ks=(512, 256, 64), v=D, vs=(512, 256, 64), q_out=D, k_out=None, kc=D, vc=D,
+             kp=4096, vp=4096, table=D, ts=4, past=D, news=None, phases=D, pairs=32, inter=0, scale=1.0, rows=2, new=2,
+             heads=16, kv=4, dim=64, page=16, pages=8, width=4, dtype=native.DTYPE_BF16)
+    a.update(kw)
+    return lib.plora_paged_append(a["q"], *a["qs"], a["k"], *a["ks"], a["v"], *a["vs"], a["q_out"], a["k_out"], a["kc"],
+                                  a["vc"], a["kp"], a["vp"], a["table"], a["ts"], a["past"], a["news"], a["phases"],
+                                  a["pairs"], a["inter"], a["scale"], a["rows"], a["new"], a["heads"], a["kv"], a["dim"],
+                                  a["page"], a["pages"], a["width"], a["dtype"], None)
+
+
+def _attend(lib, native, **kw):
+    a = dict(q=D, qs=(1024, 64), kc=D, vc=D, kp=4096, vp=4096, table=D, ts=4, lens=D, out=D, scale=0.125, window=0,
+             rows=2, heads=16, kv=4, dim=64, page=16, pages=8, width=4, dtype=native.DTYPE_BF16, ws=D, wb=1 << 30)
+    a.update(kw)
+    return lib.plora_paged_attention(a["q"], *a["qs"], a["kc"], a["vc"], a["kp"], a["vp"], a["table"], a["ts"], a["lens"],
+                                     a["out"], a["scale"], a["window"], a["rows"], a["heads"], a["kv"], a["dim"],
+                                     a["page"], a["pages"], a["width"], a["dtype"], a["ws"], a["wb"], None)
+
+
+SHARED = [
+    (dict(dtype=9), "INVALID"), (dict(rows=-1), "INVALID"), (dict(kv=0), "INVALID"), (dict(heads=10), "INVALID"),
+    (dict(dim=60), "UNSUPPORTED"), (dict(dim=264), "UNSUPPORTED"), (dict(page=0), "INVALID"), (dict(pages=0), "INVALID"),
+    (dict(width=0), "INVALID"), (dict(rows=1 << 21), "UNSUPPORTED"), (dict(pages=1 << 32), "UNSUPPORTED"),
+    (dict(width=1 << 28, ts=1 << 28), "UNSUPPORTED"), (dict(kp=4095), "INVALID"), (dict(vp=4100), "INVALID"),
+    (dict(ts=3), "INVALID"), (dict(kc=D + 8), "INVALID"), (dict(kc=None), "INVALID"), (dict(table=None), "INVALID"),
+    (dict(q=D + 2), "INVALID"), (dict(kv=60000, heads=60000, page=1 << 20), "UNSUPPORTED"),
+    (dict(pages=1 << 30, kp=1 << 40, vp=1 << 40), "INVALID"),
+]
+
+
+@pytest.mark.parametrize("kw,status", SHARED)
+@pytest.mark.parametrize("call", [_append, _attend])
+def test_cache_arguments_rejected_before_cuda(native, call, kw, status):
+    want = {"INVALID": native.ERR_INVALID_ARGUMENT, "UNSUPPORTED": native.ERR_UNSUPPORTED}[status]
+    assert call(native.load(), native, **kw) == want, native.last_error()
+    assert native.last_error()
+
+
+def test_append_arguments_rejected_before_cuda(native):
+    lib = native.load()
+    for kw in (dict(pairs=33), dict(pairs=-1), dict(new=-1), dict(k=None), dict(v=None), dict(past=None), dict(q_out=None),
+               dict(phases=None), dict(qs=(2048, 1024, 63)), dict(ks=(-512, 256, 64)), dict(vs=(512, 4, 64)),
+               dict(k_out=D + 4)):
+        assert _append(lib, native, **kw) == native.ERR_INVALID_ARGUMENT, kw
+    assert _append(lib, native, rows=1 << 16, new=1 << 16) == native.ERR_UNSUPPORTED
+    assert _append(lib, native, rows=0) == native.OK
+    assert _append(lib, native, new=0) == native.OK
+
+
+def test_attention_arguments_rejected_before_cuda(native):
+    lib = native.load()
+    for kw in (dict(heads=0), dict(window=-1), dict(q=None), dict(lens=None), dict(out=None), dict(out=D + 8),
+               dict(qs=(1024, 4)), dict(ws=D + 16)):
+        assert _attend(lib, native, **kw) == native.ERR_INVALID_ARGUMENT, kw
+    need = lib.plora_paged_attention_workspace(16, 4, 64, native.DTYPE_BF16)
+    assert need > 0
+    assert _attend(lib, native, wb=need - 1) == native.ERR_WORKSPACE
+    assert _attend(lib, native, ws=None) == native.ERR_WORKSPACE
+    assert _attend(lib, native, rows=0) == native.OK
+    for bad in ((16, 5, 64, 2), (0, 4, 64, 2), (16, 4, 65, 2), (16, 4, 512, 2), (16, 4, 64, 7)):
+        assert lib.plora_paged_attention_workspace(*bad) == 0
+
+
+def test_rules_arguments_rejected_before_cuda(native):
+    lib = native.load()
+
+    def rules(**kw):
+        a = dict(x=D, xs=100, y=D, ys=100, rows=2, vocab=100, dtype=native.DTYPE_BF16, tok=D, tr=8, hist=8, bt=D, br=4,
+                 bv=D, vr=4, k=4, mask=None, mr=0, tb=8)
+        a.update(kw)
+        return lib.plora_logit_rules(a["x"], a["xs"], a["y"], a["ys"], a["rows"], a["vocab"], a["dtype"], a["tok"], a["tr"],
+                                     a["hist"], None, None, None, None, None, a["bt"], a["br"], a["bv"], a["vr"], a["k"],
+                                     a["mask"], a["mr"], a["tb"], None)
+
+    for kw in (dict(dtype=3), dict(rows=-1), dict(vocab=-1), dict(hist=-1), dict(k=-1), dict(tb=2), dict(x=None),
+               dict(y=None), dict(tok=None), dict(bt=None), dict(bv=None), dict(xs=99), dict(ys=99), dict(tr=-1),
+               dict(br=-1), dict(mask=D, mr=-1), dict(x=D + 1)):
+        assert rules(**kw) == native.ERR_INVALID_ARGUMENT, kw
+    for kw in (dict(rows=70000), dict(vocab=1 << 31, xs=1 << 31, ys=1 << 31), dict(hist=1 << 30), dict(k=4097)):
+        assert rules(**kw) == native.ERR_UNSUPPORTED, kw
+    assert rules(rows=0) == native.OK and rules(vocab=0) == native.OK
+
+
+def test_cpu_tensors_are_refused():
+    kc, table, lens = torch.zeros(1, 1, 4, 8), torch.zeros(1, 1, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        paged_attention(torch.zeros(1, 1, 8), kc, kc, table, lens)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        paged_append(None, torch.zeros(1, 1, 1, 8), torch.zeros(1, 1, 1, 8), kc, kc, table, lens)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        apply_logit_rules(torch.zeros(1, 5), LogitRules())
+
+
+def test_rotary_phases_are_exact_fractions():
+    """Position * phase mod 2^64 is the angle's fraction of a turn to 2^-36 of a
+    turn at positions of millions; a phase is off by half a unit of 2^-64 and by
+    64-bit division, 2^-52 of a fraction below one."""
+    freq = torch.cat([500000.0 ** -(torch.arange(0, 128, 2) / 128), torch.tensor([0.0, 3.0, 6.5, -0.25, 1e-9])])
+    for f, p in zip(freq.tolist(), rotary_phases(freq).tolist()):
+        for pos in (0, 1, 8191, 131071, 5_000_000):
+            turn = ((pos * p) % (1 << 64)) / 2.0**64
+            want = math.fmod(pos * math.fmod(f, 2 * math.pi), 2 * math.pi) / (2 * math.pi)
+            off = (turn - want) % 1.0
+            assert min(off, 1 - off) < (pos + 1) * 2.0**-50, (f, pos)
+    assert rotary_phases(torch.zeros(0)).shape == (0,)
+    for bad in (torch.zeros(2, 2), torch.zeros(2, dtype=torch.int64), torch.tensor([math.inf])):
+        with pytest.raises(ValueError):
+            rotary_phases(bad)
+
+
+def test_heads_copies_only_what_it_must():
+    t = torch.zeros(2, 3, 4, 16, dtype=torch.bfloat16)
+    for same in (t, t.transpose(0, 1), t[:, :, 1:3], t[:, :, :1].expand(2, 3, 4, 16)):
+        assert _heads(same)[0].data_ptr() == same.data_ptr()
+    for other in (t.transpose(-1, -2), t[..., 1:9], torch.zeros(2, 3, 4, 12, dtype=torch.bfloat16)[..., :8]):
+        got, st = _heads(other)
+        assert got.is_contiguous() and got.data_ptr() % 16 == 0
+        assert other.shape[-1] % 8 or all(s % 8 == 0 for s in st[:-1])  # heads that the operators take
+    assert _heads(t[:1])[1][0] == 0
