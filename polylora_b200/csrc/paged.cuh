@@ -506,9 +506,9 @@ __device__ __forceinline__ AttnPlace attn_place(const AttnParams& p, const AttnS
   return o;
 }
 
-template <int EB, int DP>
+template <int DP>
 struct AttnSimtCfg {
-  using Tile = AttnTileCfg<EB, DP>;
+  using Tile = AttnTileCfg<4, DP>;
   static constexpr int kHeads = 8;  // query heads of a block
   static constexpr int kStages = DP == 256 ? 2 : 3;
   static constexpr int kWarps = DP == 256 ? 3 : (DP == 128 ? 4 : 8);
@@ -517,12 +517,14 @@ struct AttnSimtCfg {
   static constexpr int kSmemBytes = kWarps * kWarpBytes;
 };
 
-// CUDA-core attention.  Scores: lanes l and l + 16 take token l & 15, each half
-// of the head's elements.  Sums: a lane owns DP / 32 elements of all heads.
-template <typename T, int DP>
-__global__ void __launch_bounds__(AttnSimtCfg<sizeof(T), DP>::kWarps * 32, 1) attn_simt_kernel(const AttnParams p) {
-  using Cfg = AttnSimtCfg<sizeof(T), DP>;
-  using Tile = AttnTileCfg<sizeof(T), DP>;
+// CUDA-core attention for fp32 (TF32 products would lose 13 bits of it).
+// Scores: lanes l and l + 16 take token l & 15, each half of the head's
+// elements.  Sums: a lane owns DP / 32 elements of all heads.
+template <int DP>
+__global__ void __launch_bounds__(AttnSimtCfg<DP>::kWarps * 32, 1) attn_simt_kernel(const AttnParams p) {
+  using T = float;
+  using Cfg = AttnSimtCfg<DP>;
+  using Tile = AttnTileCfg<4, DP>;
   constexpr int H = Cfg::kHeads, N = Chunk<T>::N, E = DP / 32;
   extern __shared__ __align__(128) unsigned char attn_smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -533,11 +535,11 @@ __global__ void __launch_bounds__(AttnSimtCfg<sizeof(T), DP>::kWarps * 32, 1) at
   griddep_wait();
   griddep_launch();
   const AttnShare s = attn_share<Cfg::kWarps>(p);
-  if (s.worker < gridDim.x * Cfg::kWarps && lane == 0) p.desc[s.worker] = make_int4(0, 0, 0, 0);
+  if (lane == 0) p.desc[s.worker] = make_int4(0, 0, 0, 0);
   __syncwarp();
   if (s.begin == s.end) return;
 
-  AttnLoader<sizeof(T), DP> load;
+  AttnLoader<4, DP> load;
   load.at = s.at;
   load.left = s.end - s.begin;
   load.look_up(p);
@@ -646,6 +648,215 @@ __global__ void __launch_bounds__(AttnSimtCfg<sizeof(T), DP>::kWarps * 32, 1) at
             float* out = p.part_o + (to.part + h) * p.c.dim + d;
             out[0] = o[h][e], out[1] = o[h][e + 1];
           }
+        }
+      }
+      begun = true, fresh = true;
+    }
+    at.next(p);
+    __syncwarp();
+  }
+}
+
+template <int DP, int NT>
+struct AttnMmaCfg {
+  using Tile = AttnTileCfg<2, DP>;
+  static constexpr int kHeads = 8 * NT;             // query heads of a block
+  static constexpr bool kQShared = NT * DP > 256;   // query fragments in shared memory, not registers
+  static constexpr int kQBytes = kQShared ? kHeads * DP * 2 : 0;
+  static constexpr int kStages = DP == 256 ? 2 : (DP == 128 ? 3 : 6);
+  static constexpr int kWarpBytes = kStages * Tile::kStageBytes + kQBytes;
+  static constexpr int kFit = 224 * 1024 / kWarpBytes;
+  static constexpr int kWarps = kFit < 8 ? kFit : 8;
+  static constexpr int kSmemBytes = kWarps * kWarpBytes;
+};
+
+// Tensor-core attention for 16-bit types, 8 * NT query heads at a time.  A tile's
+// keys are the rows of S^T = K Q^T (m16n8k16: 16 tokens by 8 heads, so a group
+// of up to eight heads fills the instruction), its values those of
+// O^T += V^T P^T; both come from shared memory by ldmatrix, and P^T is S^T's own
+// fragment, transposed in registers by movmatrix.
+//
+// Probabilities enter the second product as a 16-bit number and a 16-bit
+// remainder: with the first alone the sums would be off by as much as the
+// rounding of the result (1.7e-3 becomes 2.3e-3 of a bf16 output); the second
+// costs one more instruction where memory is the bound.
+template <bool BF16, int DP, int NT>
+__global__ void __launch_bounds__(AttnMmaCfg<DP, NT>::kWarps * 32, 1) attn_mma_kernel(const AttnParams p) {
+  using Cfg = AttnMmaCfg<DP, NT>;
+  using Tile = AttnTileCfg<2, DP>;
+  using T = typename Elem<BF16>::T;
+  constexpr int KS = DP / 16;
+  extern __shared__ __align__(128) unsigned char attn_smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  unsigned char* mine = attn_smem + warp * Cfg::kWarpBytes;
+  const uint32_t ring = smem_u32(mine), sq = ring + Cfg::kStages * Tile::kStageBytes;
+  for (int i = lane; i < Cfg::kWarpBytes / 16; i += 32) reinterpret_cast<uint4*>(mine)[i] = make_uint4(0, 0, 0, 0);
+  griddep_wait();
+  griddep_launch();
+  const AttnShare s = attn_share<Cfg::kWarps>(p);
+  if (lane == 0) p.desc[s.worker] = make_int4(0, 0, 0, 0);
+  __syncwarp();
+  if (s.begin == s.end) return;
+
+  AttnLoader<2, DP> load;
+  load.at = s.at;
+  load.left = s.end - s.begin;
+  load.look_up(p);
+#pragma unroll
+  for (int i = 0; i < Cfg::kStages - 1; ++i) load.issue(p, ring + i * Tile::kStageBytes);
+
+  // ldmatrix rows of this lane: keys (token l & 15, chunk 2 ks + l / 16), values
+  // transposed (token (l & 7) + 8 (l / 16), chunk 2 mt + (l / 8) % 2)
+  const int krow = lane & 15, kchunk = lane >> 4;
+  const int vrow = (lane & 7) + ((lane >> 4) << 3), vchunk = (lane >> 3) & 1;
+  AttnCursor at = s.at;
+  bool begun = at.tile == at.r.t0, fresh = true;
+  uint32_t qf[Cfg::kQShared ? 1 : NT][Cfg::kQShared ? 1 : KS][2];
+  float m[NT][2], l[NT][2], o[NT][KS][4];
+  int stage = 0;
+  for (int64_t pos = s.begin; pos < s.end; ++pos) {
+    const int kv = at.head / p.blocks, blk = at.head - kv * p.blocks;
+    const int h0 = blk * p.block_heads, nh = min(p.block_heads, p.group - h0);
+    if (fresh) {
+      const T* q = (const T*)p.q + at.row * p.q_row + (kv * p.group + h0) * p.q_head;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        if constexpr (Cfg::kQShared) {
+          for (int i = lane; i < 8 * Tile::kChunks; i += 32) {
+            const int h = i / Tile::kChunks, c = i % Tile::kChunks;
+            uint4 u = make_uint4(0, 0, 0, 0);
+            if (nt * 8 + h < nh && c * 8 < p.c.dim) u = *reinterpret_cast<const uint4*>(q + (nt * 8 + h) * p.q_head + c * 8);
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(sq + Tile::offset(nt * 8 + h, c)), "r"(u.x),
+                         "r"(u.y), "r"(u.z), "r"(u.w)
+                         : "memory");
+          }
+        } else {
+          const int h = nt * 8 + (lane >> 2);
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const int d = ks * 16 + j * 8 + (lane & 3) * 2;
+              qf[nt][ks][j] = h < nh && d < p.c.dim ? *reinterpret_cast<const uint32_t*>(q + h * p.q_head + d) : 0u;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) m[nt][j] = -INFINITY, l[nt][j] = 0.f;
+#pragma unroll
+        for (int mt = 0; mt < KS; ++mt)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[nt][mt][j] = 0.f;
+      }
+      fresh = false;
+    }
+    cp_async_wait<Cfg::kStages - 2>();
+    __syncwarp();
+    // the stage read in the last round is free again
+    load.issue(p, ring + (stage == 0 ? Cfg::kStages - 1 : stage - 1) * Tile::kStageBytes);
+    const uint32_t ks0 = ring + stage * Tile::kStageBytes, vs0 = ks0 + Tile::kTileBytes;
+
+    float sc[NT][2][4];  // two chains of sums, even and odd steps
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sc[nt][0][j] = sc[nt][1][j] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      if (ks * 16 >= p.c.dim) break;
+      uint32_t a[4];
+      ldsm_x4(ks0 + Tile::offset(krow, 2 * ks + kchunk), a);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        if constexpr (Cfg::kQShared) {
+          uint32_t b[4];  // the lower lanes' two matrices are the step's, so both halves name them
+          ldsm_x4(sq + Tile::offset(nt * 8 + (lane & 7), 2 * ks + ((lane >> 3) & 1)), b);
+          mma_16816<BF16>(sc[nt][ks & 1], a, b[0], b[1]);
+        } else {
+          mma_16816<BF16>(sc[nt][ks & 1], a, qf[nt][ks][0], qf[nt][ks][1]);
+        }
+      }
+    }
+    const int p0 = at.tile * kAttnTile + (lane >> 2);  // this lane's tokens: p0, p0 + 8
+    const bool inner = at.tile * kAttnTile >= at.r.lo && (at.tile + 1) * kAttnTile <= at.r.n;
+    const bool live0 = inner || (p0 >= at.r.lo && p0 < at.r.n), live1 = inner || (p0 + 8 >= at.r.lo && p0 + 8 < at.r.n);
+    uint32_t hi[NT][2], lo[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float x[4], keep[2];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        x[j] = (sc[nt][0][j] + sc[nt][1][j]) * p.scale_log2;
+        if (!(j < 2 ? live0 : live1)) x[j] = -INFINITY;
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {  // the lane's two heads
+        float mx = fmaxf(x[j], x[j + 2]);
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+        const float m2 = fmaxf(m[nt][j], mx), base = m2 == -INFINITY ? 0.f : m2;
+        keep[j] = exp2f(m[nt][j] - base);
+        m[nt][j] = m2;
+        x[j] = exp2f(x[j] - base);
+        x[j + 2] = exp2f(x[j + 2] - base);
+        l[nt][j] = l[nt][j] * keep[j] + x[j] + x[j + 2];  // of this lane's tokens; added over lanes at the end
+      }
+      if (__any_sync(0xffffffffu, keep[0] != 1.f || keep[1] != 1.f)) {
+#pragma unroll
+        for (int mt = 0; mt < KS; ++mt)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[nt][mt][j] *= keep[j & 1];
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const uint32_t w = pack2<BF16>(x[2 * j], x[2 * j + 1]);
+        const float r0 = x[2 * j] - Elem<BF16>::to_f((uint16_t)w), r1 = x[2 * j + 1] - Elem<BF16>::to_f((uint16_t)(w >> 16));
+        hi[nt][j] = movmatrix_t(w);
+        lo[nt][j] = movmatrix_t(pack2<BF16>(r0, r1));
+      }
+    }
+#pragma unroll
+    for (int mt = 0; mt < KS; ++mt) {
+      if (mt * 16 >= p.c.dim) break;
+      uint32_t a[4];
+      ldsm_x4_trans(vs0 + Tile::offset(vrow, 2 * mt + vchunk), a);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        mma_16816<BF16>(o[nt][mt], a, hi[nt][0], hi[nt][1]);
+        mma_16816<BF16>(o[nt][mt], a, lo[nt][0], lo[nt][1]);
+      }
+    }
+    stage = stage + 1 == Cfg::kStages ? 0 : stage + 1;
+
+    const bool done = at.tile + 1 == at.r.t1;
+    if (done || pos + 1 == s.end) {
+      const AttnPlace to = attn_place(p, s, at, pos, begun, done);
+      const int64_t head0 = (int64_t)at.row * p.c.kv_heads * p.group + kv * p.group + h0;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float sum = l[nt][j];
+          sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+          const int h = nt * 8 + (lane & 3) * 2 + j;
+          if (h >= nh) continue;
+          const float f = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
+          if (!to.whole && lane < 4) p.part_ml[to.part + h] = make_float2(m[nt][j], sum);
+          T* out = (T*)p.out + (head0 + h) * p.c.dim;
+          float* part = p.part_o + (to.part + h) * p.c.dim;
+#pragma unroll
+          for (int mt = 0; mt < KS; ++mt)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const int d = mt * 16 + i * 8 + (lane >> 2);
+              if (d >= p.c.dim) continue;
+              if (to.whole)
+                out[d] = Chunk<T>::put(o[nt][mt][2 * i + j] * f);
+              else
+                part[d] = o[nt][mt][2 * i + j];
+            }
         }
       }
       begun = true, fresh = true;

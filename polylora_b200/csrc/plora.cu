@@ -149,19 +149,29 @@ int device_info(DeviceInfo** out) {
     SET_GRID((sgmv_expand_stream_kernel<true>), kStreamSmemLimit)
     SET_GRID((sgmv_expand_stream_kernel<false>), kStreamSmemLimit)
     SET_GRID(seg_scan_place_kernel, (kSegScanPlaceMaxInts + kSegMaxSlots + 1) * 4)
-#define SET_ATTN(T, DP) SET_GRID((attn_simt_kernel<T, DP>), (AttnSimtCfg<sizeof(T), DP>::kSmemBytes))
-#define SET_PAGED(T)                                     \
-  SET_ATTN(T, 64)                                        \
-  SET_ATTN(T, 128)                                       \
-  SET_ATTN(T, 256)                                       \
+#define SET_ATTN(DP, NT)                                                       \
+  SET_GRID((attn_mma_kernel<true, DP, NT>), (AttnMmaCfg<DP, NT>::kSmemBytes))  \
+  SET_GRID((attn_mma_kernel<false, DP, NT>), (AttnMmaCfg<DP, NT>::kSmemBytes))
+    SET_ATTN(64, 1)
+    SET_ATTN(64, 2)
+    SET_ATTN(64, 4)
+    SET_ATTN(128, 1)
+    SET_ATTN(128, 2)
+    SET_ATTN(128, 4)
+    SET_ATTN(256, 1)
+    SET_ATTN(256, 2)
+#undef SET_ATTN
+    SET_GRID(attn_simt_kernel<64>, AttnSimtCfg<64>::kSmemBytes)
+    SET_GRID(attn_simt_kernel<128>, AttnSimtCfg<128>::kSmemBytes)
+    SET_GRID(attn_simt_kernel<256>, AttnSimtCfg<256>::kSmemBytes)
+    constexpr int kRulesSmem = kRulesChunk * 6 + kRulesMaxBiases * 5;
+#define SET_RULES(T)                                     \
   SET_GRID((logit_rules_kernel<T, int32_t>), kRulesSmem) \
   SET_GRID((logit_rules_kernel<T, int64_t>), kRulesSmem)
-    constexpr int kRulesSmem = kRulesChunk * 6 + kRulesMaxBiases * 5;
-    SET_PAGED(float)
-    SET_PAGED(__half)
-    SET_PAGED(__nv_bfloat16)
-#undef SET_PAGED
-#undef SET_ATTN
+    SET_RULES(float)
+    SET_RULES(__half)
+    SET_RULES(__nv_bfloat16)
+#undef SET_RULES
 #undef SET_GRID
     // the row copies use no shared memory; an SM running them keeps its largest
     // shared-memory carveout, so the segment-table kernels of the next rows of
@@ -643,25 +653,33 @@ int token_rows_impl(const void* host_rows, void* device_rows, bool to_host, int6
 constexpr int kAttnGrid = 148;
 constexpr int64_t kPagedMaxRows = 1 << 20;
 
-int attn_padded_dim(int64_t dim) { return dim <= 64 ? 64 : (dim <= 128 ? 128 : 256); }
-
-// Query heads of a block and warps of a CTA of the kernel that runs a call.
+// The attention kernel of a call: padded head size, query heads of a block (in
+// eights for the tensor cores, 0: CUDA cores) and warps of a CTA.  Blocks are as
+// large as registers allow, for a second block reads the cache again.
 struct AttnPlan {
-  int blocks, block_heads, warps;
+  int dp, eights, blocks, block_heads, warps;
   size_t ml_offset, desc_offset, bytes;
 };
 AttnPlan attn_plan(int32_t heads, int32_t kv_heads, int32_t dim, int dtype) {
   AttnPlan a;
   const int group = heads / kv_heads;
-  const int dp = attn_padded_dim(dim);
-  const int most = 8;
-  if (dtype == PLORA_DTYPE_F32)
-    a.warps = dp == 64 ? AttnSimtCfg<4, 64>::kWarps : (dp == 128 ? AttnSimtCfg<4, 128>::kWarps : AttnSimtCfg<4, 256>::kWarps);
-  else
-    a.warps = dp == 64 ? AttnSimtCfg<2, 64>::kWarps : (dp == 128 ? AttnSimtCfg<2, 128>::kWarps : AttnSimtCfg<2, 256>::kWarps);
+  a.dp = dim <= 64 ? 64 : (dim <= 128 ? 128 : 256);
+  const int most = dtype == PLORA_DTYPE_F32 ? 8 : (a.dp == 256 ? 16 : 32);
   a.blocks = (group + most - 1) / most;
   a.block_heads = (group + a.blocks - 1) / a.blocks;
   a.blocks = (group + a.block_heads - 1) / a.block_heads;
+  if (dtype == PLORA_DTYPE_F32) {
+    a.eights = 0;
+    a.warps = a.dp == 64 ? AttnSimtCfg<64>::kWarps : (a.dp == 128 ? AttnSimtCfg<128>::kWarps : AttnSimtCfg<256>::kWarps);
+  } else {
+    a.eights = a.block_heads <= 8 ? 1 : (a.block_heads <= 16 ? 2 : 4);
+#define PLORA_WARPS(DP, NT) \
+  if (a.dp == DP && a.eights == NT) a.warps = AttnMmaCfg<DP, NT>::kWarps;
+    PLORA_WARPS(64, 1) PLORA_WARPS(64, 2) PLORA_WARPS(64, 4)
+    PLORA_WARPS(128, 1) PLORA_WARPS(128, 2) PLORA_WARPS(128, 4)
+    PLORA_WARPS(256, 1) PLORA_WARPS(256, 2)
+#undef PLORA_WARPS
+  }
   const size_t workers = (size_t)kAttnGrid * a.warps, parts = workers * 2 * a.block_heads;
   a.ml_offset = align256(parts * dim * 4);
   a.desc_offset = a.ml_offset + align256(parts * 8);
@@ -714,19 +732,29 @@ cudaError_t launch_append(const AppendParams& p, bool vec, unsigned grid, cudaSt
              : launch_kernel(paged_append_kernel<T, false>, dim3(grid), dim3(kAppendThreads), 0, s, true, 0, p);
 }
 
-template <typename T, int DP>
-cudaError_t launch_attn_simt(const AttnParams& p, cudaStream_t s) {
-  using Cfg = AttnSimtCfg<sizeof(T), DP>;
-  return launch_kernel(attn_simt_kernel<T, DP>, dim3(kAttnGrid), dim3(Cfg::kWarps * 32), Cfg::kSmemBytes, s, true, 0, p);
-}
-template <typename T>
-cudaError_t launch_attn(const AttnParams& p, const AttnPlan& a, cudaStream_t s) {
-  const int dp = attn_padded_dim(p.c.dim);
-  cudaError_t e = dp == 64 ? launch_attn_simt<T, 64>(p, s)
-                           : (dp == 128 ? launch_attn_simt<T, 128>(p, s) : launch_attn_simt<T, 256>(p, s));
+cudaError_t launch_attn(const AttnParams& p, const AttnPlan& a, int dtype, cudaStream_t s) {
+  cudaError_t e = cudaErrorInvalidValue;
+#define PLORA_SIMT(DP)                                                                                          \
+  if (a.eights == 0 && a.dp == DP)                                                                              \
+    e = launch_kernel(attn_simt_kernel<DP>, dim3(kAttnGrid), dim3(a.warps * 32), AttnSimtCfg<DP>::kSmemBytes, s, \
+                      true, 0, p);
+#define PLORA_MMA(BF16, DP, NT)                                                                           \
+  if (a.eights == NT && a.dp == DP && BF16 == (dtype == PLORA_DTYPE_BF16))                                \
+    e = launch_kernel(attn_mma_kernel<BF16, DP, NT>, dim3(kAttnGrid), dim3(a.warps * 32),                 \
+                      AttnMmaCfg<DP, NT>::kSmemBytes, s, true, 0, p);
+#define PLORA_MMA_BOTH(DP, NT) PLORA_MMA(true, DP, NT) PLORA_MMA(false, DP, NT)
+  PLORA_SIMT(64) PLORA_SIMT(128) PLORA_SIMT(256)
+  PLORA_MMA_BOTH(64, 1) PLORA_MMA_BOTH(64, 2) PLORA_MMA_BOTH(64, 4)
+  PLORA_MMA_BOTH(128, 1) PLORA_MMA_BOTH(128, 2) PLORA_MMA_BOTH(128, 4)
+  PLORA_MMA_BOTH(256, 1) PLORA_MMA_BOTH(256, 2)
+#undef PLORA_MMA_BOTH
+#undef PLORA_MMA
+#undef PLORA_SIMT
   if (e != cudaSuccess) return e;
-  return launch_kernel(attn_join_kernel<T>, dim3((unsigned)(kAttnGrid * a.warps), (unsigned)a.block_heads),
-                       dim3(kJoinWarps * 32), 0, s, true, 0, p);
+  const dim3 grid((unsigned)(kAttnGrid * a.warps), (unsigned)a.block_heads), block(kJoinWarps * 32);
+  return dtype == PLORA_DTYPE_F32   ? launch_kernel(attn_join_kernel<float>, grid, block, 0, s, true, 0, p)
+         : dtype == PLORA_DTYPE_F16 ? launch_kernel(attn_join_kernel<__half>, grid, block, 0, s, true, 0, p)
+                                    : launch_kernel(attn_join_kernel<__nv_bfloat16>, grid, block, 0, s, true, 0, p);
 }
 
 template <typename T>
@@ -1133,10 +1161,7 @@ int plora_paged_attention(const void* q, int64_t q_row_stride, int64_t q_head_st
   p.part_ml = reinterpret_cast<float2*>(ws + a.ml_offset);
   p.desc = reinterpret_cast<int4*>(ws + a.desc_offset);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  cudaError_t e = dtype == PLORA_DTYPE_F32   ? launch_attn<float>(p, a, s)
-                  : dtype == PLORA_DTYPE_F16 ? launch_attn<__half>(p, a, s)
-                                             : launch_attn<__nv_bfloat16>(p, a, s);
-  PLORA_CUDA(e, "launch paged attention");
+  PLORA_CUDA(launch_attn(p, a, dtype, s), "launch paged attention");
   return PLORA_OK;
 }
 
