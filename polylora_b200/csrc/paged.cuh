@@ -279,6 +279,13 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const Appe
 // item has at least one (empty) tile, so rows without tokens are written too.
 constexpr int kAttnTile = 16;
 
+// 2^x to 2 ulp; results below 2^-126 are zero, next to a largest term of 1.
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 struct AttnParams {
   PagedView c;
   const void* q;
@@ -290,7 +297,7 @@ struct AttnParams {
   // workspace: two partials a worker (slot 0: its first item, begun by another; 1: its last, that goes on)
   float* part_o;    // (workers, 2, block_heads, dim)
   float2* part_ml;  // (workers, 2, block_heads): maximum (in units of scale_log2), sum
-  int4* desc;       // (workers): row, head block, pieces of the item that begins and is cut here (pieces 0: none)
+  int4* desc;       // (workers): row, kv head, head block, parts of the item that begins and is cut here (0: none)
 };
 
 struct AttnRow {
@@ -308,22 +315,27 @@ __device__ __forceinline__ AttnRow attn_row(const AttnParams& p, int row) {
   return r;
 }
 
-// A position in the list of all tiles.
+// A position in the list of all tiles: rows, their key-value heads, blocks of
+// a group's query heads, tiles.
 struct AttnCursor {
-  int row, head, tile;  // head: head block of the row, kv_head * blocks + block
+  int row, kv, blk, tile;
   AttnRow r;
   __device__ __forceinline__ void next(const AttnParams& p) {
     if (++tile < r.t1) return;
-    if (++head == p.c.kv_heads * p.blocks) {
-      head = 0;
-      if (++row < p.rows) r = attn_row(p, row);
+    if (++blk == p.blocks) {
+      blk = 0;
+      if (++kv == p.c.kv_heads) {
+        kv = 0;
+        if (++row < p.rows) r = attn_row(p, row);
+      }
     }
     tile = r.t0;
   }
 };
 
 struct AttnShare {
-  int64_t begin, end;   // tiles of this warp
+  int64_t begin;        // first tile of this warp in the list
+  int count;            // its tiles
   int64_t total;        // tiles of all items
   int workers, worker;  // warps with a share
   AttnCursor at;        // at `begin`
@@ -352,7 +364,7 @@ __device__ __forceinline__ int block_scan(int v, int* s_warp, int* total) {
   return before + incl - v;
 }
 
-// The calling warp's share.  Block-collective; warps without one get begin == end.
+// The calling warp's share.  Block-collective; warps without one get count 0.
 template <int WARPS>
 __device__ __forceinline__ AttnShare attn_share(const AttnParams& p) {
   constexpr int THREADS = WARPS * 32;
@@ -377,12 +389,12 @@ __device__ __forceinline__ AttnShare attn_share(const AttnParams& p) {
   const int all = gridDim.x * WARPS;
   s.workers = s.total < all ? (int)s.total : all;
   s.worker = warp * gridDim.x + blockIdx.x;
-  s.begin = s.end = 0;
+  s.begin = 0, s.count = 0;
   if (s.worker < s.workers) {
     s.begin = s.total * s.worker / s.workers;
-    s.end = s.total * (s.worker + 1) / s.workers;
+    s.count = (int)(s.total * (s.worker + 1) / s.workers - s.begin);
   }
-  if ((tid & 31) == 0) s_begin[warp] = s.begin < s.end ? s.begin : -1;  // the scan's barriers publish it
+  if ((tid & 31) == 0) s_begin[warp] = s.count ? s.begin : -1;  // the scan's barriers publish it
   int64_t before = 0;
   for (int base = 0; base < p.rows; base += THREADS) {
     int n = 0, sum;
@@ -402,13 +414,15 @@ __device__ __forceinline__ AttnShare attn_share(const AttnParams& p) {
     before += sum;
   }
   __syncthreads();
-  if (s.begin < s.end) {
+  if (s.count) {
     s.at.row = s_row[warp];
     s.at.r = attn_row(p, s.at.row);
     const int n = s.at.r.t1 - s.at.r.t0;
     const int rest = (int)(s.begin - s_before[warp] * per_row);
-    s.at.head = rest / n;
-    s.at.tile = s.at.r.t0 + rest - s.at.head * n;
+    const int item = rest / n;
+    s.at.kv = item / p.blocks;
+    s.at.blk = item - s.at.kv * p.blocks;
+    s.at.tile = s.at.r.t0 + rest - item * n;
   }
   return s;
 }
@@ -422,26 +436,27 @@ __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// Shared-memory layout of a tile: 16 rows of DP elements, 16-byte chunks of a
-// row exchanged by row & 7, so that 8 rows of one chunk lie in 8 bank groups.
+// Shared-memory layout of a tile: blocks of 128 bytes of its 16 rows, block by
+// block; within a block the 16-byte chunks of a row are exchanged by row & 7 (the
+// TMA's 128-byte swizzle), so that 8 rows of one chunk lie in 8 bank groups.
 template <int EB, int DP>
 struct AttnTileCfg {
-  static constexpr int kChunks = DP * EB / 16;         // of a padded row
-  static constexpr int kRowBytes = DP * EB;
-  static constexpr int kTileBytes = kAttnTile * kRowBytes;
-  static constexpr int kStageBytes = 2 * kTileBytes;   // keys, values
+  static constexpr int kChunks = DP * EB / 16;  // of a padded row
+  static constexpr int kTileBytes = kAttnTile * DP * EB;
+  static constexpr int kStageBytes = 2 * kTileBytes;  // keys, values
   static __device__ __forceinline__ uint32_t offset(int row, int chunk) {
-    return row * kRowBytes + ((chunk ^ (row & 7)) << 4);
+    return (chunk >> 3) * (kAttnTile * 128) + row * 128 + (((chunk ^ row) & 7) << 4);
   }
 };
 
-// Copies the tiles of a share into a warp's stages.  The page of a tile's
-// tokens is looked up one tile ahead (lane l: token l & 15).
+// Copies the tiles of a share into a warp's stages, any page size and head
+// size: 16 bytes a lane (cp.async).  The page of a tile's tokens is looked up one
+// tile ahead (lane l: token l & 15).
 template <int EB, int DP>
-struct AttnLoader {
-  using Cfg = AttnTileCfg<EB, DP>;
+struct AttnCopyLoader {
+  using Tile = AttnTileCfg<EB, DP>;
   AttnCursor at;
-  int64_t left;
+  int left;
   int page, inner;  // of this lane's token of tile `at`; page -1: reads as zeros
 
   __device__ __forceinline__ void look_up(const AttnParams& p) {
@@ -455,13 +470,13 @@ struct AttnLoader {
         raise_status(PLORA_DEV_PAGE_RANGE);
         page = -1;
       }
-      inner = ((at.head / p.blocks) * p.c.page_size + pos - e * p.c.page_size) * p.c.dim;
+      inner = (at.kv * p.c.page_size + pos - e * p.c.page_size) * p.c.dim;
     }
   }
   // Starts the copies of tile `at` (none past the share's end) and steps on.
   __device__ __forceinline__ void issue(const AttnParams& p, uint32_t stage) {
     if (left > 0) {
-      constexpr int LANES = Cfg::kChunks < 32 ? Cfg::kChunks : 32;  // lanes of a row
+      constexpr int LANES = Tile::kChunks < 32 ? Tile::kChunks : 32;  // lanes of a row
       const int lane = threadIdx.x & 31, lc = lane % LANES;
 #pragma unroll
       for (int r0 = 0; r0 < kAttnTile; r0 += 32 / LANES) {
@@ -471,11 +486,11 @@ struct AttnLoader {
         const char* k = (const char*)p.c.k + (ok ? (pg * p.c.k_page + in) * EB : 0);
         const char* v = (const char*)p.c.v + (ok ? (pg * p.c.v_page + in) * EB : 0);
 #pragma unroll
-        for (int c = lc; c < Cfg::kChunks; c += LANES) {
+        for (int c = lc; c < Tile::kChunks; c += LANES) {
           if (c * (16 / EB) < p.c.dim) {  // columns past dim stay zero
-            const uint32_t d = stage + Cfg::offset(row, c);
+            const uint32_t d = stage + Tile::offset(row, c);
             cp_async16_or_zero(d, k + c * 16, ok);
-            cp_async16_or_zero(d + Cfg::kTileBytes, v + c * 16, ok);
+            cp_async16_or_zero(d + Tile::kTileBytes, v + c * 16, ok);
           }
         }
       }
@@ -487,6 +502,53 @@ struct AttnLoader {
   }
 };
 
+// The same by TMA, for pages of whole tiles and heads of DP elements: one lane
+// starts two copies a tile, where the copies above cost the warp ~250
+// instructions.  The maps view the cache as (64 elements, slot, 64-element block,
+// kv head, page); a page outside the cache is an out-of-range coordinate, which
+// reads as zeros.
+template <int DP>
+struct AttnTmaLoader {
+  using Tile = AttnTileCfg<2, DP>;
+  AttnCursor at;
+  int left;
+  int page, slot;  // of tile `at`
+
+  __device__ __forceinline__ void look_up(const AttnParams& p) {
+    if (left <= 0) return;
+    page = p.c.num_pages, slot = 0;
+    const int pos = at.tile * kAttnTile;
+    if (pos < at.r.n) {
+      const int e = p.c.page.div(pos);
+      slot = pos - e * p.c.page_size;
+      page = p.c.table[at.row * p.c.table_stride + e];
+      if ((uint32_t)page >= (uint32_t)p.c.num_pages) {
+        raise_status(PLORA_DEV_PAGE_RANGE);
+        page = p.c.num_pages;
+      }
+    }
+  }
+  // One lane's: starts the copies of tile `at`, completing on `bar`, and steps on.
+  __device__ __forceinline__ void issue(const AttnParams& p, const CUtensorMap* mk, const CUtensorMap* mv,
+                                        uint32_t stage, uint64_t* bar) {
+    if (left <= 0) return;
+    mbar_arrive_expect_tx(bar, Tile::kStageBytes);
+    tma_load_tile(stage, mk, bar, slot, at.kv, page);
+    tma_load_tile(stage + Tile::kTileBytes, mv, bar, slot, at.kv, page);
+    at.next(p);
+    --left;
+    look_up(p);
+  }
+  static __device__ __forceinline__ void tma_load_tile(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int slot,
+                                                       int kv, int page) {
+    asm volatile(
+        "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %3, %5, %6}], [%2];" ::"r"(dst),
+        "l"(map), "r"(smem_u32(bar)), "r"(0), "r"(slot), "r"(kv), "r"(page)
+        : "memory");
+  }
+};
+
 // Where a warp leaves the sums of the item it has finished its part of:
 // `begun` / `done`: the part holds the item's first / last tile.
 struct AttnPlace {
@@ -494,14 +556,14 @@ struct AttnPlace {
   int64_t part;  // row of part_ml: ((worker * 2 + slot) * block_heads)
 };
 __device__ __forceinline__ AttnPlace attn_place(const AttnParams& p, const AttnShare& s, const AttnCursor& at,
-                                                int64_t pos, bool begun, bool done) {
+                                                int64_t pos, bool begun, bool done) {  // pos: of tile `at`
   AttnPlace o;
   o.whole = begun && done;
   o.part = (s.worker * 2ll + (begun ? 1 : 0)) * p.block_heads;
   if (begun && !done && (threadIdx.x & 31) == 0) {  // the item goes on in later shares
     const int64_t last = pos + (at.r.t1 - 1 - at.tile);  // its last tile
     const int w = (int)(((last + 1) * s.workers - 1) / s.total);  // the worker whose share holds it
-    p.desc[s.worker] = make_int4(at.row, at.head, w - s.worker + 1, 0);
+    p.desc[s.worker] = make_int4(at.row, at.kv, at.blk, w - s.worker + 1);
   }
   return o;
 }
@@ -537,11 +599,11 @@ __global__ void __launch_bounds__(AttnSimtCfg<DP>::kWarps * 32, 1) attn_simt_ker
   const AttnShare s = attn_share<Cfg::kWarps>(p);
   if (lane == 0) p.desc[s.worker] = make_int4(0, 0, 0, 0);
   __syncwarp();
-  if (s.begin == s.end) return;
+  if (s.count == 0) return;
 
-  AttnLoader<4, DP> load;
+  AttnCopyLoader<4, DP> load;
   load.at = s.at;
-  load.left = s.end - s.begin;
+  load.left = s.count;
   load.look_up(p);
   const uint32_t ring = smem_u32(mine);
 #pragma unroll
@@ -551,9 +613,8 @@ __global__ void __launch_bounds__(AttnSimtCfg<DP>::kWarps * 32, 1) attn_simt_ker
   bool begun = at.tile == at.r.t0, fresh = true;
   float m[H], l[H], o[H][E];
   int stage = 0;
-  for (int64_t pos = s.begin; pos < s.end; ++pos) {
-    const int kv = at.head / p.blocks, blk = at.head - kv * p.blocks;
-    const int h0 = blk * p.block_heads, nh = min(p.block_heads, p.group - h0);
+  for (int i = 0; i < s.count; ++i) {
+    const int kv = at.kv, h0 = at.blk * p.block_heads, nh = min(p.block_heads, p.group - h0);
     if (fresh) {
       const T* q = (const T*)p.q + at.row * p.q_row + (kv * p.group + h0) * p.q_head;
       for (int h = 0; h < H; ++h)
@@ -600,7 +661,7 @@ __global__ void __launch_bounds__(AttnSimtCfg<DP>::kWarps * 32, 1) attn_simt_ker
 #pragma unroll
       for (int d = 8; d; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
       const float m2 = fmaxf(m[h], mx), base = m2 == -INFINITY ? 0.f : m2;
-      const float keep = exp2f(m[h] - base), pr = exp2f(x - base);
+      const float keep = exp2_fast(m[h] - base), pr = exp2_fast(x - base);
       m[h] = m2;
       l[h] = l[h] * keep + (half ? 0.f : pr);  // per lane; added over the lanes at the item's end
       if (half == 0) sp[tok * H + h] = pr;
@@ -628,8 +689,8 @@ __global__ void __launch_bounds__(AttnSimtCfg<DP>::kWarps * 32, 1) attn_simt_ker
     stage = stage + 1 == Cfg::kStages ? 0 : stage + 1;
 
     const bool done = at.tile + 1 == at.r.t1;
-    if (done || pos + 1 == s.end) {
-      const AttnPlace to = attn_place(p, s, at, pos, begun, done);
+    if (done || i + 1 == s.count) {
+      const AttnPlace to = attn_place(p, s, at, s.begin + i, begun, done);
 #pragma unroll
       for (int h = 0; h < H; ++h) {
 #pragma unroll
@@ -660,14 +721,14 @@ __global__ void __launch_bounds__(AttnSimtCfg<DP>::kWarps * 32, 1) attn_simt_ker
 template <int DP, int NT>
 struct AttnMmaCfg {
   using Tile = AttnTileCfg<2, DP>;
-  static constexpr int kHeads = 8 * NT;             // query heads of a block
-  static constexpr bool kQShared = NT * DP > 256;   // query fragments in shared memory, not registers
+  static constexpr int kHeads = 8 * NT;            // query heads of a block
+  static constexpr bool kQShared = NT * DP > 256;  // query fragments in shared memory, not registers
   static constexpr int kQBytes = kQShared ? kHeads * DP * 2 : 0;
   static constexpr int kStages = DP == 256 ? 2 : (DP == 128 ? 3 : 6);
   static constexpr int kWarpBytes = kStages * Tile::kStageBytes + kQBytes;
   static constexpr int kFit = 224 * 1024 / kWarpBytes;
   static constexpr int kWarps = kFit < 8 ? kFit : 8;
-  static constexpr int kSmemBytes = kWarps * kWarpBytes;
+  static constexpr int kSmemBytes = 1024 + kWarps * kWarpBytes;  // aligned to 1024 bytes
 };
 
 // Tensor-core attention for 16-bit types, 8 * NT query heads at a time.  A tile's
@@ -680,54 +741,83 @@ struct AttnMmaCfg {
 // remainder: with the first alone the sums would be off by as much as the
 // rounding of the result (1.7e-3 becomes 2.3e-3 of a bf16 output); the second
 // costs one more instruction where memory is the bound.
-template <bool BF16, int DP, int NT>
-__global__ void __launch_bounds__(AttnMmaCfg<DP, NT>::kWarps * 32, 1) attn_mma_kernel(const AttnParams p) {
+template <bool BF16, int DP, int NT, bool TMA>
+__global__ void __launch_bounds__(AttnMmaCfg<DP, NT>::kWarps * 32, 1)
+    attn_mma_kernel(const AttnParams p, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv) {
   using Cfg = AttnMmaCfg<DP, NT>;
   using Tile = AttnTileCfg<2, DP>;
   using T = typename Elem<BF16>::T;
-  constexpr int KS = DP / 16;
+  constexpr int KS = DP / 16, STAGES = Cfg::kStages;
   extern __shared__ __align__(128) unsigned char attn_smem[];
+  __shared__ uint64_t bars[TMA ? Cfg::kWarps * STAGES : 1];
+  __shared__ int abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  unsigned char* mine = attn_smem + warp * Cfg::kWarpBytes;
-  const uint32_t ring = smem_u32(mine), sq = ring + Cfg::kStages * Tile::kStageBytes;
-  for (int i = lane; i < Cfg::kWarpBytes / 16; i += 32) reinterpret_cast<uint4*>(mine)[i] = make_uint4(0, 0, 0, 0);
+  unsigned char* mine = attn_smem + ((1024 - (smem_u32(attn_smem) & 1023)) & 1023) + warp * Cfg::kWarpBytes;
+  const uint32_t ring = smem_u32(mine), sq = ring + STAGES * Tile::kStageBytes;
+  uint64_t* bar = bars + (TMA ? warp * STAGES : 0);
+  if constexpr (TMA) {
+    if (threadIdx.x == 0) abort_flag = 0;
+    if (lane == 0) {
+      for (int i = 0; i < STAGES; ++i) mbar_init(bar + i, 1);
+      fence_barrier_init();
+      prefetch_tmap(&mk);
+      prefetch_tmap(&mv);
+    }
+  } else if (p.c.dim < DP) {  // columns that no copy fills
+    for (int i = lane; i < STAGES * Tile::kStageBytes / 16; i += 32) reinterpret_cast<uint4*>(mine)[i] = make_uint4(0, 0, 0, 0);
+  }
   griddep_wait();
   griddep_launch();
   const AttnShare s = attn_share<Cfg::kWarps>(p);
   if (lane == 0) p.desc[s.worker] = make_int4(0, 0, 0, 0);
   __syncwarp();
-  if (s.begin == s.end) return;
+  if (s.count == 0) return;
 
-  AttnLoader<2, DP> load;
-  load.at = s.at;
-  load.left = s.end - s.begin;
-  load.look_up(p);
+  AttnCopyLoader<2, DP> copy;
+  AttnTmaLoader<DP> tma;
+  if constexpr (TMA) {
+    tma.at = s.at, tma.left = s.count;
+    if (lane == 0) {
+      tma.look_up(p);
 #pragma unroll
-  for (int i = 0; i < Cfg::kStages - 1; ++i) load.issue(p, ring + i * Tile::kStageBytes);
+      for (int i = 0; i < STAGES - 1; ++i) tma.issue(p, &mk, &mv, ring + i * Tile::kStageBytes, bar + i);
+    }
+  } else {
+    copy.at = s.at, copy.left = s.count;
+    copy.look_up(p);
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i) copy.issue(p, ring + i * Tile::kStageBytes);
+  }
 
   // ldmatrix rows of this lane: keys (token l & 15, chunk 2 ks + l / 16), values
-  // transposed (token (l & 7) + 8 (l / 16), chunk 2 mt + (l / 8) % 2)
-  const int krow = lane & 15, kchunk = lane >> 4;
-  const int vrow = (lane & 7) + ((lane >> 4) << 3), vchunk = (lane >> 3) & 1;
+  // transposed (token (l & 7) + 8 (l / 16), chunk 2 mt + (l / 8) % 2); four chunk
+  // pairs make a block, so step j adds a block and one of four offsets
+  const int krow = lane & 15, vrow = (lane & 7) + ((lane >> 4) << 3);
+  uint32_t koff[4], voff[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    koff[j] = Tile::offset(krow, 2 * j + (lane >> 4));
+    voff[j] = Tile::kTileBytes + Tile::offset(vrow, 2 * j + ((lane >> 3) & 1));
+  }
   AttnCursor at = s.at;
   bool begun = at.tile == at.r.t0, fresh = true;
   uint32_t qf[Cfg::kQShared ? 1 : NT][Cfg::kQShared ? 1 : KS][2];
   float m[NT][2], l[NT][2], o[NT][KS][4];
   int stage = 0;
-  for (int64_t pos = s.begin; pos < s.end; ++pos) {
-    const int kv = at.head / p.blocks, blk = at.head - kv * p.blocks;
-    const int h0 = blk * p.block_heads, nh = min(p.block_heads, p.group - h0);
+  uint32_t parity = 0;
+  for (int i = 0; i < s.count; ++i) {
     if (fresh) {
-      const T* q = (const T*)p.q + at.row * p.q_row + (kv * p.group + h0) * p.q_head;
+      const int h0 = at.blk * p.block_heads, nh = min(p.block_heads, p.group - h0);
+      const T* q = (const T*)p.q + at.row * p.q_row + (at.kv * p.group + h0) * p.q_head;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         if constexpr (Cfg::kQShared) {
-          for (int i = lane; i < 8 * Tile::kChunks; i += 32) {
-            const int h = i / Tile::kChunks, c = i % Tile::kChunks;
+          for (int j = lane; j < 8 * Tile::kChunks; j += 32) {
+            const int h = nt * 8 + j / Tile::kChunks, c = j % Tile::kChunks;
             uint4 u = make_uint4(0, 0, 0, 0);
-            if (nt * 8 + h < nh && c * 8 < p.c.dim) u = *reinterpret_cast<const uint4*>(q + (nt * 8 + h) * p.q_head + c * 8);
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(sq + Tile::offset(nt * 8 + h, c)), "r"(u.x),
-                         "r"(u.y), "r"(u.z), "r"(u.w)
+            if (h < nh && c * 8 < p.c.dim) u = *reinterpret_cast<const uint4*>(q + h * p.q_head + c * 8);
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(sq + h * (DP * 2) + ((c ^ (h & 7)) << 4)),
+                         "r"(u.x), "r"(u.y), "r"(u.z), "r"(u.w)
                          : "memory");
           }
         } else {
@@ -749,11 +839,39 @@ __global__ void __launch_bounds__(AttnMmaCfg<DP, NT>::kWarps * 32, 1) attn_mma_k
       }
       fresh = false;
     }
-    cp_async_wait<Cfg::kStages - 2>();
-    __syncwarp();
-    // the stage read in the last round is free again
-    load.issue(p, ring + (stage == 0 ? Cfg::kStages - 1 : stage - 1) * Tile::kStageBytes);
-    const uint32_t ks0 = ring + stage * Tile::kStageBytes, vs0 = ks0 + Tile::kTileBytes;
+    const int ahead = stage == 0 ? STAGES - 1 : stage - 1;  // read in the last round: free again
+    if constexpr (TMA) {
+      if (lane == 0) tma.issue(p, &mk, &mv, ring + ahead * Tile::kStageBytes, bar + ahead);
+      if (!mbar_wait_warp(bar + stage, parity, &abort_flag)) {
+        // let this warp's copies land before the CTA's memory goes
+        const int flying = min(STAGES, s.count - i);
+        for (int j = 0; j < flying; ++j) {
+          mbar_drain(bar + stage, parity);
+          if (++stage == STAGES) stage = 0, parity ^= 1;
+        }
+        return;
+      }
+    } else {
+      cp_async_wait<STAGES - 2>();
+      __syncwarp();
+      copy.issue(p, ring + ahead * Tile::kStageBytes);
+    }
+    const uint32_t base = ring + stage * Tile::kStageBytes;
+    const bool inner = at.tile * kAttnTile >= at.r.lo && (at.tile + 1) * kAttnTile <= at.r.n;
+    if (TMA && !inner) {
+      // the copy brought whole pages: values outside the row's tokens must not
+      // meet a zero probability as NaN or infinity
+      for (int j = lane; j < kAttnTile * Tile::kChunks; j += 32) {
+        const int row = j / Tile::kChunks, ps = at.tile * kAttnTile + row;
+        if (ps < at.r.lo || ps >= at.r.n)
+          asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(base + Tile::kTileBytes +
+                                                                       Tile::offset(row, j % Tile::kChunks)),
+                       "r"(0)
+                       : "memory");
+      }
+      fence_proxy_async_smem();  // before a later copy lands here
+      __syncwarp();
+    }
 
     float sc[NT][2][4];  // two chains of sums, even and odd steps
 #pragma unroll
@@ -762,14 +880,15 @@ __global__ void __launch_bounds__(AttnMmaCfg<DP, NT>::kWarps * 32, 1) attn_mma_k
       for (int j = 0; j < 4; ++j) sc[nt][0][j] = sc[nt][1][j] = 0.f;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
-      if (ks * 16 >= p.c.dim) break;
+      if (!TMA && ks * 16 >= p.c.dim) break;
       uint32_t a[4];
-      ldsm_x4(ks0 + Tile::offset(krow, 2 * ks + kchunk), a);
+      ldsm_x4(base + koff[ks & 3] + (ks >> 2) * (kAttnTile * 128), a);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         if constexpr (Cfg::kQShared) {
-          uint32_t b[4];  // the lower lanes' two matrices are the step's, so both halves name them
-          ldsm_x4(sq + Tile::offset(nt * 8 + (lane & 7), 2 * ks + ((lane >> 3) & 1)), b);
+          uint32_t b[4];  // two matrices, named by both halves of the warp
+          const int h = nt * 8 + (lane & 7);
+          ldsm_x4(sq + h * (DP * 2) + (((2 * ks + ((lane >> 3) & 1)) ^ (h & 7)) << 4), b);
           mma_16816<BF16>(sc[nt][ks & 1], a, b[0], b[1]);
         } else {
           mma_16816<BF16>(sc[nt][ks & 1], a, qf[nt][ks][0], qf[nt][ks][1]);
@@ -777,7 +896,6 @@ __global__ void __launch_bounds__(AttnMmaCfg<DP, NT>::kWarps * 32, 1) attn_mma_k
       }
     }
     const int p0 = at.tile * kAttnTile + (lane >> 2);  // this lane's tokens: p0, p0 + 8
-    const bool inner = at.tile * kAttnTile >= at.r.lo && (at.tile + 1) * kAttnTile <= at.r.n;
     const bool live0 = inner || (p0 >= at.r.lo && p0 < at.r.n), live1 = inner || (p0 + 8 >= at.r.lo && p0 + 8 < at.r.n);
     uint32_t hi[NT][2], lo[NT][2];
 #pragma unroll
@@ -794,11 +912,11 @@ __global__ void __launch_bounds__(AttnMmaCfg<DP, NT>::kWarps * 32, 1) attn_mma_k
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-        const float m2 = fmaxf(m[nt][j], mx), base = m2 == -INFINITY ? 0.f : m2;
-        keep[j] = exp2f(m[nt][j] - base);
+        const float m2 = fmaxf(m[nt][j], mx), top = m2 == -INFINITY ? 0.f : m2;
+        keep[j] = exp2_fast(m[nt][j] - top);
         m[nt][j] = m2;
-        x[j] = exp2f(x[j] - base);
-        x[j + 2] = exp2f(x[j + 2] - base);
+        x[j] = exp2_fast(x[j] - top);
+        x[j + 2] = exp2_fast(x[j + 2] - top);
         l[nt][j] = l[nt][j] * keep[j] + x[j] + x[j + 2];  // of this lane's tokens; added over lanes at the end
       }
       if (__any_sync(0xffffffffu, keep[0] != 1.f || keep[1] != 1.f)) {
@@ -817,21 +935,22 @@ __global__ void __launch_bounds__(AttnMmaCfg<DP, NT>::kWarps * 32, 1) attn_mma_k
     }
 #pragma unroll
     for (int mt = 0; mt < KS; ++mt) {
-      if (mt * 16 >= p.c.dim) break;
+      if (!TMA && mt * 16 >= p.c.dim) break;
       uint32_t a[4];
-      ldsm_x4_trans(vs0 + Tile::offset(vrow, 2 * mt + vchunk), a);
+      ldsm_x4_trans(base + voff[mt & 3] + (mt >> 2) * (kAttnTile * 128), a);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         mma_16816<BF16>(o[nt][mt], a, hi[nt][0], hi[nt][1]);
         mma_16816<BF16>(o[nt][mt], a, lo[nt][0], lo[nt][1]);
       }
     }
-    stage = stage + 1 == Cfg::kStages ? 0 : stage + 1;
+    if (++stage == STAGES) stage = 0, parity ^= 1;
 
     const bool done = at.tile + 1 == at.r.t1;
-    if (done || pos + 1 == s.end) {
-      const AttnPlace to = attn_place(p, s, at, pos, begun, done);
-      const int64_t head0 = (int64_t)at.row * p.c.kv_heads * p.group + kv * p.group + h0;
+    if (done || i + 1 == s.count) {
+      const AttnPlace to = attn_place(p, s, at, s.begin + i, begun, done);
+      const int h0 = at.blk * p.block_heads, nh = min(p.block_heads, p.group - h0);
+      const int64_t head0 = ((int64_t)at.row * p.c.kv_heads + at.kv) * p.group + h0;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -849,13 +968,13 @@ __global__ void __launch_bounds__(AttnMmaCfg<DP, NT>::kWarps * 32, 1) attn_mma_k
 #pragma unroll
           for (int mt = 0; mt < KS; ++mt)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const int d = mt * 16 + i * 8 + (lane >> 2);
+            for (int e = 0; e < 2; ++e) {
+              const int d = mt * 16 + e * 8 + (lane >> 2);
               if (d >= p.c.dim) continue;
               if (to.whole)
-                out[d] = Chunk<T>::put(o[nt][mt][2 * i + j] * f);
+                out[d] = Chunk<T>::put(o[nt][mt][2 * e + j] * f);
               else
-                part[d] = o[nt][mt][2 * i + j];
+                part[d] = o[nt][mt][2 * e + j];
             }
         }
       }
@@ -878,21 +997,20 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_join_kernel(const AttnPa
   griddep_launch();
   const int4 d = p.desc[blockIdx.x];
   const int h = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (d.z == 0) return;
-  const int kv = d.y / p.blocks, blk = d.y - kv * p.blocks;
-  const int h0 = blk * p.block_heads, dim = p.c.dim;
+  if (d.w == 0) return;
+  const int kv = d.y, h0 = d.z * p.block_heads, dim = p.c.dim;
   if (h0 + h >= p.group) return;
   float m = -INFINITY, l = 0.f, o[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) o[e] = 0.f;
-  for (int i = warp; i < d.z; i += kJoinWarps) {
+  for (int i = warp; i < d.w; i += kJoinWarps) {
     const int64_t part = ((blockIdx.x + i) * 2ll + (i == 0 ? 1 : 0)) * p.block_heads + h;
     const float2 ml = p.part_ml[part];
     float4 a = make_float4(0, 0, 0, 0), b = a;
     if (lane * 4 < dim) a = *reinterpret_cast<const float4*>(p.part_o + part * dim + lane * 4);
     if (128 + lane * 4 < dim) b = *reinterpret_cast<const float4*>(p.part_o + part * dim + 128 + lane * 4);
     const float m2 = fmaxf(m, ml.x), base = m2 == -INFINITY ? 0.f : m2;
-    const float keep = exp2f(m - base), f = exp2f(ml.x - base);
+    const float keep = exp2_fast(m - base), f = exp2_fast(ml.x - base);
     m = m2;
     l = l * keep + ml.y * f;
     o[0] = o[0] * keep + a.x * f, o[1] = o[1] * keep + a.y * f, o[2] = o[2] * keep + a.z * f, o[3] = o[3] * keep + a.w * f;
@@ -907,7 +1025,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_join_kernel(const AttnPa
   for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, s_m[w]);
   const float base = top == -INFINITY ? 0.f : top;
 #pragma unroll
-  for (int w = 0; w < kJoinWarps; ++w) f[w] = exp2f(s_m[w] - base), sum += s_l[w] * f[w];
+  for (int w = 0; w < kJoinWarps; ++w) f[w] = exp2_fast(s_m[w] - base), sum += s_l[w] * f[w];
   const float inv = sum > 0.f ? 1.f / sum : 0.f;
   T* out = (T*)p.out + ((int64_t)d.x * p.c.kv_heads * p.group + kv * p.group + h0 + h) * dim;
   for (int e = threadIdx.x; e < dim; e += kJoinWarps * 32) {

@@ -150,8 +150,10 @@ int device_info(DeviceInfo** out) {
     SET_GRID((sgmv_expand_stream_kernel<false>), kStreamSmemLimit)
     SET_GRID(seg_scan_place_kernel, (kSegScanPlaceMaxInts + kSegMaxSlots + 1) * 4)
 #define SET_ATTN(DP, NT)                                                       \
-  SET_GRID((attn_mma_kernel<true, DP, NT>), (AttnMmaCfg<DP, NT>::kSmemBytes))  \
-  SET_GRID((attn_mma_kernel<false, DP, NT>), (AttnMmaCfg<DP, NT>::kSmemBytes))
+  SET_GRID((attn_mma_kernel<true, DP, NT, true>), (AttnMmaCfg<DP, NT>::kSmemBytes))   \
+  SET_GRID((attn_mma_kernel<false, DP, NT, true>), (AttnMmaCfg<DP, NT>::kSmemBytes))  \
+  SET_GRID((attn_mma_kernel<true, DP, NT, false>), (AttnMmaCfg<DP, NT>::kSmemBytes))  \
+  SET_GRID((attn_mma_kernel<false, DP, NT, false>), (AttnMmaCfg<DP, NT>::kSmemBytes))
     SET_ATTN(64, 1)
     SET_ATTN(64, 2)
     SET_ATTN(64, 4)
@@ -732,17 +734,44 @@ cudaError_t launch_append(const AppendParams& p, bool vec, unsigned grid, cudaSt
              : launch_kernel(paged_append_kernel<T, false>, dim3(grid), dim3(kAppendThreads), 0, s, true, 0, p);
 }
 
-cudaError_t launch_attn(const AttnParams& p, const AttnPlan& a, int dtype, cudaStream_t s) {
+// A 16-bit cache viewed as (64 elements, slot, 64-element block, kv head, page);
+// a box is a tile: 16 slots of one head of one page, block by block.
+int make_map_cache(CUtensorMap* map, const void* base, int dtype, const PagedView& c, int64_t page_stride) {
+  auto enc = tensor_map_encoder();
+  if (!enc) return fail(PLORA_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  const cuuint64_t d = c.dim;
+  const cuuint64_t dims[5] = {64, (cuuint64_t)c.page_size, d / 64, (cuuint64_t)c.kv_heads, (cuuint64_t)c.num_pages};
+  const cuuint64_t strides[4] = {d * 2, 128, (cuuint64_t)c.page_size * d * 2, (cuuint64_t)page_stride * 2};
+  const cuuint32_t box[5] = {64, kAttnTile, (cuuint32_t)(d / 64), 1, 1};
+  const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  const CUtensorMapDataType dt = dtype == PLORA_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                           : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  CUresult r = enc(map, dt, 5, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(PLORA_ERR_CUDA, "cuTensorMapEncodeTiled (cache) failed (%d)", (int)r);
+  return PLORA_OK;
+}
+
+// TMA copies whole tiles of whole pages, 64 elements at a time.
+bool attn_by_tma(const PagedView& c, const AttnPlan& a) {
+  const int64_t most = (1ll << 39) - 1;  // elements: strides below 2^40 bytes
+  return a.eights > 0 && c.dim == a.dp && c.page_size % kAttnTile == 0 && c.k_page <= most && c.v_page <= most;
+}
+
+cudaError_t launch_attn(const AttnParams& p, const AttnPlan& a, int dtype, bool tma, const CUtensorMap& mk,
+                        const CUtensorMap& mv, cudaStream_t s) {
   cudaError_t e = cudaErrorInvalidValue;
 #define PLORA_SIMT(DP)                                                                                          \
   if (a.eights == 0 && a.dp == DP)                                                                              \
     e = launch_kernel(attn_simt_kernel<DP>, dim3(kAttnGrid), dim3(a.warps * 32), AttnSimtCfg<DP>::kSmemBytes, s, \
                       true, 0, p);
-#define PLORA_MMA(BF16, DP, NT)                                                                           \
-  if (a.eights == NT && a.dp == DP && BF16 == (dtype == PLORA_DTYPE_BF16))                                \
-    e = launch_kernel(attn_mma_kernel<BF16, DP, NT>, dim3(kAttnGrid), dim3(a.warps * 32),                 \
-                      AttnMmaCfg<DP, NT>::kSmemBytes, s, true, 0, p);
-#define PLORA_MMA_BOTH(DP, NT) PLORA_MMA(true, DP, NT) PLORA_MMA(false, DP, NT)
+#define PLORA_MMA(BF16, DP, NT, TMA)                                                                      \
+  if (a.eights == NT && a.dp == DP && BF16 == (dtype == PLORA_DTYPE_BF16) && TMA == tma)                  \
+    e = launch_kernel(attn_mma_kernel<BF16, DP, NT, TMA>, dim3(kAttnGrid), dim3(a.warps * 32),            \
+                      AttnMmaCfg<DP, NT>::kSmemBytes, s, true, 0, p, mk, mv);
+#define PLORA_MMA_BOTH(DP, NT) \
+  PLORA_MMA(true, DP, NT, true) PLORA_MMA(false, DP, NT, true) PLORA_MMA(true, DP, NT, false) PLORA_MMA(false, DP, NT, false)
   PLORA_SIMT(64) PLORA_SIMT(128) PLORA_SIMT(256)
   PLORA_MMA_BOTH(64, 1) PLORA_MMA_BOTH(64, 2) PLORA_MMA_BOTH(64, 4)
   PLORA_MMA_BOTH(128, 1) PLORA_MMA_BOTH(128, 2) PLORA_MMA_BOTH(128, 4)
@@ -1161,7 +1190,12 @@ int plora_paged_attention(const void* q, int64_t q_row_stride, int64_t q_head_st
   p.part_ml = reinterpret_cast<float2*>(ws + a.ml_offset);
   p.desc = reinterpret_cast<int4*>(ws + a.desc_offset);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  PLORA_CUDA(launch_attn(p, a, dtype, s), "launch paged attention");
+  CUtensorMap mk = {}, mv = {};
+  const bool tma = attn_by_tma(p.c, a);
+  if (tma && ((st = make_map_cache(&mk, k_cache, dtype, p.c, k_page_stride)) ||
+              (st = make_map_cache(&mv, v_cache, dtype, p.c, v_page_stride))))
+    return st;
+  PLORA_CUDA(launch_attn(p, a, dtype, tma, mk, mv, s), "launch paged attention");
   return PLORA_OK;
 }
 

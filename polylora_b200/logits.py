@@ -8,7 +8,7 @@ The reference has no counterpart (it ends at the base model's output).
 
 from __future__ import annotations
 
-from dataclasses import dataclass, fields
+from dataclasses import dataclass
 
 import torch
 
@@ -43,7 +43,9 @@ class LogitRules:
     allowed: torch.Tensor | None = None
 
     def tensors(self) -> list[torch.Tensor]:
-        return [t for t in (getattr(self, f.name) for f in fields(self)) if t is not None]
+        every = (self.tokens, self.token_lens, self.prompt_lens, self.repetition_penalty, self.presence_penalty,
+                 self.frequency_penalty, self.bias_tokens, self.bias_values, self.allowed)
+        return [t for t in every if t is not None]
 
 
 def _rows_of(t: torch.Tensor, rows: int, name: str) -> torch.Tensor:
@@ -55,7 +57,7 @@ def _rows_of(t: torch.Tensor, rows: int, name: str) -> torch.Tensor:
 def _per_row(t: torch.Tensor | None, rows: int, dtype: torch.dtype, name: str) -> torch.Tensor | None:
     if t is None:
         return None
-    if t.shape != (rows,):
+    if t.dim() != 1 or t.shape[0] != rows:
         raise ValueError(f"{name} must have shape ({rows},), got {tuple(t.shape)}")
     return _as(t, dtype)
 
@@ -79,7 +81,7 @@ def apply_logit_rules(logits: torch.Tensor, rules: LogitRules, out: torch.Tensor
     if logits.shape[1] > 1 and logits.stride(1) != 1:
         raise ValueError("logits rows must be contiguous")
     if out is None:
-        out = torch.empty((rows, vocab), dtype=logits.dtype, device=dev)
+        out = logits.new_empty((rows, vocab))
     elif out.shape != logits.shape or out.dtype != logits.dtype or out.device != dev or (vocab > 1 and out.stride(1) != 1):
         raise ValueError("out must have the logits' shape, dtype and device, with contiguous rows")
     tokens, bias_tokens, bias_values, allowed = rules.tokens, rules.bias_tokens, rules.bias_values, rules.allowed
@@ -90,8 +92,8 @@ def apply_logit_rules(logits: torch.Tensor, rules: LogitRules, out: torch.Tensor
     if tokens is not None:
         tokens = _rows_of(tokens, rows, "tokens")
         width = tokens.dtype
-    elif any(t is not None for t in (rules.token_lens, rules.prompt_lens, rules.repetition_penalty,
-                                     rules.presence_penalty, rules.frequency_penalty)):
+    elif not (rules.token_lens is rules.prompt_lens is rules.repetition_penalty is rules.presence_penalty
+              is rules.frequency_penalty is None):
         raise ValueError("penalties and lengths need tokens")
     if (bias_tokens is None) != (bias_values is None):
         raise ValueError("bias_tokens and bias_values go together")
@@ -102,7 +104,9 @@ def apply_logit_rules(logits: torch.Tensor, rules: LogitRules, out: torch.Tensor
         if width is not None and bias_tokens.dtype != width:  # both as the wider: narrowing could alias ids
             tokens, bias_tokens = tokens.to(torch.int64), bias_tokens.to(torch.int64)
         width = bias_tokens.dtype
-        bias_values = _rows_of(bias_values.to(torch.float32), rows, "bias_values")
+        if bias_values.dtype != torch.float32:
+            bias_values = bias_values.to(torch.float32)
+        bias_values = _rows_of(bias_values, rows, "bias_values")
     if allowed is not None:
         if allowed.dtype != torch.int32 or allowed.dim() != 2 or allowed.shape[1] < (vocab + 31) // 32:
             raise ValueError(f"allowed must be int32 ({rows}, at least {(vocab + 31) // 32})")

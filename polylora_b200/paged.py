@@ -19,7 +19,7 @@ import math
 import torch
 
 from . import _native
-from .sgmv import _as, _require_cuda, _stream, dtype_code
+from .sgmv import _as, _require_cuda, dtype_code
 
 
 def rotary_phases(inv_freq: torch.Tensor) -> torch.Tensor:
@@ -36,25 +36,31 @@ def rotary_phases(inv_freq: torch.Tensor) -> torch.Tensor:
 
 
 def _no_grad(*tensors: torch.Tensor | None) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError("the paged-cache and logit operators have no gradient: call them under torch.no_grad()")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError("the paged-cache and logit operators have no gradient: call them under torch.no_grad()")
 
 
-def _strides(t: torch.Tensor) -> list[int]:
-    return [st if n > 1 else 0 for n, st in zip(t.shape, t.stride())]
-
-
-def _heads(t: torch.Tensor) -> tuple[torch.Tensor, list[int]]:
+def _heads(t: torch.Tensor) -> tuple[torch.Tensor, tuple[int, ...]]:
     """``t`` with dense last dimension and 16-byte aligned rows (a copy where
     it has neither) and its strides, 0 for dimensions of one."""
     vec = 16 // t.element_size()
-    st = _strides(t)
-    if (t.shape[-1] > 1 and st[-1] != 1) or any(s % vec for s in st[:-1]) or t.data_ptr() % 16:
-        t = t.contiguous()
-        if t.data_ptr() % 16:
-            t = t.clone()
+    if t.is_contiguous() and t.shape[-1] % vec == 0:
+        st = t.stride() if 1 not in t.shape else _strides(t)
+    else:
+        st = _strides(t)
+        if (t.shape[-1] > 1 and st[-1] != 1) or any(s % vec for s in st[:-1]):
+            t = t.contiguous()
+            st = _strides(t)
+    if t.data_ptr() % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
         st = _strides(t)
     return t, st
+
+
+def _strides(t: torch.Tensor) -> tuple[int, ...]:
+    return tuple([st if n > 1 else 0 for n, st in zip(t.shape, t.stride())])
 
 
 def _check_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor, rows: int, dim: int,
@@ -67,10 +73,11 @@ def _check_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch
         raise ValueError(f"head_dim mismatch: tokens={dim}, cache={d}")
     if not (k_cache.dtype == v_cache.dtype == dtype):
         raise TypeError(f"dtype mismatch: tokens={dtype}, k_cache={k_cache.dtype}, v_cache={v_cache.dtype}")
-    inner = (size * d, d, 1)
-    for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
-        if c.stride()[1:] != inner and any(st != want for n, st, want in zip(c.shape[1:], c.stride()[1:], inner) if n > 1):
-            raise ValueError(f"{name} pages must be contiguous")
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+        inner = (size * d, d, 1)
+        for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
+            if any(st != want for n, st, want in zip(c.shape[1:], c.stride()[1:], inner) if n > 1):
+                raise ValueError(f"{name} pages must be contiguous")
     if page_table.dim() != 2 or page_table.shape[0] != rows or page_table.dtype != torch.int32:
         raise ValueError(f"page_table must be int32 ({rows}, max_pages)")
     if page_table.shape[1] > 1 and page_table.stride(1) != 1:
@@ -81,17 +88,21 @@ def _check_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch
 
 
 def _lens(t: torch.Tensor, rows: int, name: str) -> torch.Tensor:
-    if t.shape != (rows,):
+    if t.dim() != 1 or t.shape[0] != rows:
         raise ValueError(f"{name} must have shape ({rows},), got {tuple(t.shape)}")
     return _as(t, torch.int32)
 
 
 def _call(dev: torch.device, func: str, *args: object) -> None:
-    if dev.index == torch.cuda.current_device():
-        _native.call(func, *args, _stream(dev))
+    """The entry point on the device's current stream, with the device current."""
+    index = dev.index
+    # the raw handle: a Stream object costs 2 us of a call whose kernel takes less than 3
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if index == torch.cuda.current_device():
+        _native.call(func, *args, stream)
     else:
-        with torch.cuda.device(dev):
-            _native.call(func, *args, _stream(dev))
+        with torch.cuda.device(index):
+            _native.call(func, *args, stream)
 
 
 def paged_append(
@@ -121,7 +132,7 @@ def paged_append(
     tokens zero); None for what was not given or asked for.  Rows of one call
     must not write to the same page."""
     dev = _require_cuda(k, v, k_cache, v_cache, page_table, past_lens,
-                        *(t for t in (q, new_lens, phases) if t is not None))
+                        *[t for t in (q, new_lens, phases) if t is not None])
     _no_grad(q, k, v)
     if k.dim() != 4 or v.shape != k.shape or (q is not None and (q.dim() != 4 or q.shape[:2] != k.shape[:2]
                                                                  or q.shape[3] != k.shape[3])):
@@ -144,8 +155,8 @@ def paged_append(
     kc, ks = _heads(k)
     vc, vs = _heads(v)
     qc, qs = _heads(q) if q is not None else (None, (0, 0, 0))
-    q_out = torch.empty((rows, new, heads, dim), dtype=q.dtype, device=dev) if q is not None else None
-    k_out = torch.empty((rows, new, kv_heads, dim), dtype=k.dtype, device=dev) if return_keys else None
+    q_out = k.new_empty((rows, new, heads, dim)) if q is not None else None
+    k_out = k.new_empty((rows, new, kv_heads, dim)) if return_keys else None
     _call(
         dev, "plora_paged_append",
         qc.data_ptr() if qc is not None else 0, qs[0], qs[1], qs[2], kc.data_ptr(), ks[0], ks[1], ks[2],
@@ -183,18 +194,18 @@ def paged_attention(
         raise ValueError(f"{heads} heads over {kv_heads} kv heads")
     lens = _lens(seq_lens, rows, "seq_lens")
     if out is None:
-        out = torch.empty((rows, heads, dim), dtype=q.dtype, device=dev)
+        out = q.new_empty((rows, heads, dim))
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or not out.is_contiguous():
         raise ValueError("out must be a contiguous tensor of q's shape, dtype and device")
     qc, qs = _heads(q)
     code = dtype_code(q.dtype)
-    ws = torch.empty(max(_native.load().plora_paged_attention_workspace(heads, kv_heads, dim, code), 256),
-                     dtype=torch.uint8, device=dev)
+    ws_bytes = _native.load().plora_paged_attention_workspace(heads, kv_heads, dim, code)
+    ws = lens.new_empty(max(ws_bytes, 256) // 4)
     _call(
         dev, "plora_paged_attention",
         qc.data_ptr(), qs[0], qs[1], k_cache.data_ptr(), v_cache.data_ptr(), k_page, v_page, page_table.data_ptr(),
         page_table.stride(0) if rows > 1 else page_table.shape[1], lens.data_ptr(), out.data_ptr(),
         dim**-0.5 if scale is None else scale, window, rows, heads, kv_heads, dim, size, pages, page_table.shape[1],
-        code, ws.data_ptr(), ws.numel(),
+        code, ws.data_ptr(), ws_bytes,
     )
     return out

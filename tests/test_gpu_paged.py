@@ -375,3 +375,27 @@ def test_empty_calls(cuda_status_clean):
                         torch.zeros(2, 0, 2, 16, device=dev), kc, kc.clone(), torch.zeros(2, 1, dtype=torch.int32, device=dev),
                         torch.zeros(2, device=dev), return_keys=True)
     assert q.shape == (2, 0, 4, 16) and k.shape == (2, 0, 2, 16)
+
+
+@pytest.mark.parametrize("lens", [[900, 300], [120000, 100000]])
+def test_expired_wait_is_reported_and_clears(native, lens):
+    """With the wait limit at 0 the attention's waits for its copies may run
+    out: the call returns, the status says so, and the next call is whole.
+    Copies of a small cache may all be there at the first look; the large one
+    (225 MB, beyond the L2) has each warp wait some twenty times."""
+    g, dev = _gen(13), _dev()
+    table, pages = _table(lens, 16, g)
+    args = [torch.randn(2, 8, 128, generator=g).to(BF).to(dev),
+            *(torch.randn(pages, 2, 16, 128, generator=g).to(BF).to(dev) for _ in range(2)), table.to(dev),
+            torch.tensor(lens, dtype=torch.int32, device=dev)]
+    want = paged_attention(*args)
+    native.device_status(clear=True)
+    prev = native.set_wait_limit_ns(0)
+    try:
+        paged_attention(*args)
+        status = native.device_status(clear=True)
+    finally:
+        native.set_wait_limit_ns(prev)
+    assert status in ((0, _native.DEV_WAIT_TIMEOUT) if lens[0] < 1000 else (_native.DEV_WAIT_TIMEOUT,))
+    assert torch.equal(paged_attention(*args), want)
+    assert native.device_status(clear=True) == 0
