@@ -273,10 +273,11 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const Appe
 // there: an item is a row and a key-value head (or a block of its query
 // heads), a tile 16 of its tokens, and the tiles of all items in order are
 // dealt in equal contiguous shares to the grid's warps, each of which streams
-// its share through a ring of shared-memory stages of its own (cp.async, no
-// barrier between warps).  An item cut by a share's end leaves partial sums in
-// the workspace, which attn_join_kernel adds in the order of the shares; every
-// item has at least one (empty) tile, so rows without tokens are written too.
+// its share through a ring of shared-memory stages of its own (no barrier
+// between warps).  An item cut by the ends of shares is put together in two
+// steps: first the parts of a CTA's warps, then, by attn_join_kernel, what the
+// CTAs left in the workspace, always in the order of the shares.  Every item has
+// at least one (empty) tile, so rows without tokens are written too.
 constexpr int kAttnTile = 16;
 
 // 2^x to 2 ulp; results below 2^-126 are zero, next to a largest term of 1.
@@ -294,10 +295,12 @@ struct AttnParams {
   int64_t q_row, q_head;
   int32_t rows, group, blocks, block_heads, window;  // blocks of block_heads query heads cover a group
   float scale_log2;                                  // scale * log2(e)
-  // workspace: two partials a worker (slot 0: its first item, begun by another; 1: its last, that goes on)
-  float* part_o;    // (workers, 2, block_heads, dim)
-  float2* part_ml;  // (workers, 2, block_heads): maximum (in units of scale_log2), sum
-  int4* desc;       // (workers): row, kv head, head block, parts of the item that begins and is cut here (0: none)
+  // workspace.  A part of an item: its sums of block_heads heads, and for each
+  // head its maximum (in units of scale_log2) and sum of probabilities
+  float* warp_o;   // (warps, block_heads, dim): a warp's part of the item that another began
+  float* cta_o;    // (CTAs, 2, block_heads, dim): a CTA's parts of the items that it shares (0: begun by
+  float2* cta_ml;  // (CTAs, 2, block_heads)       another, 1: begun here)
+  int4* desc;      // (CTAs): row, kv head, head block, CTAs of the item begun here and shared (0: none)
 };
 
 struct AttnRow {
@@ -334,11 +337,16 @@ struct AttnCursor {
 };
 
 struct AttnShare {
-  int64_t begin;        // first tile of this warp in the list
-  int count;            // its tiles
-  int64_t total;        // tiles of all items
-  int workers, worker;  // warps with a share
-  AttnCursor at;        // at `begin`
+  int64_t begin;  // first tile of this warp in the list
+  int count;      // its tiles
+  int warps;      // warps with a share, of all CTAs; warp w of CTA c is number c * WARPS + w
+  int base, rem;  // the first rem of them have base + 1 tiles, the others base
+  AttnCursor at;  // at `begin`
+  // The warp whose share holds tile x of the list.
+  __device__ __forceinline__ int holder(int64_t x) const {
+    const int64_t split = (int64_t)rem * (base + 1);
+    return x < split ? (int)(x / (base + 1)) : rem + (int)((x - split) / base);
+  }
 };
 
 // Sum over the CTA's threads before this one (exclusive) and over all of them.
@@ -373,56 +381,61 @@ __device__ __forceinline__ AttnShare attn_share(const AttnParams& p) {
   __shared__ int64_t s_before[WARPS], s_begin[WARPS];
   const int tid = threadIdx.x, warp = tid >> 5;
   const int per_row = p.c.kv_heads * p.blocks;
-  int64_t tiles = 0;
-  for (int base = 0; base < p.rows; base += THREADS) {
-    int n = 0, sum;
-    if (base + tid < p.rows) {
-      const AttnRow r = attn_row(p, base + tid);
-      n = r.t1 - r.t0;
-    }
-    block_scan<WARPS>(n, s_warp, &sum);
+  auto tiles_of = [&](int row) {
+    if (row >= p.rows) return 0;
+    const AttnRow r = attn_row(p, row);
+    return r.t1 - r.t0;
+  };
+  // tiles of the rows before this thread's (of the last round), and of all
+  int n = tiles_of(tid), sum;
+  int64_t mine = block_scan<WARPS>(n, s_warp, &sum), tiles = sum;
+  for (int first = THREADS; first < p.rows; first += THREADS) {
+    block_scan<WARPS>(tiles_of(first + tid), s_warp, &sum);
     tiles += sum;
   }
+  const int64_t total = tiles * per_row;
   AttnShare s;
-  s.total = tiles * per_row;
-  // worker w of the grid is warp w / gridDim.x of CTA w % gridDim.x: few shares spread over the SMs
-  const int all = gridDim.x * WARPS;
-  s.workers = s.total < all ? (int)s.total : all;
-  s.worker = warp * gridDim.x + blockIdx.x;
-  s.begin = 0, s.count = 0;
-  if (s.worker < s.workers) {
-    s.begin = s.total * s.worker / s.workers;
-    s.count = (int)(s.total * (s.worker + 1) / s.workers - s.begin);
+  const int all = gridDim.x * WARPS, id = blockIdx.x * WARPS + warp;
+  s.warps = total < all ? (int)total : all;
+  if (total <= INT32_MAX) {  // a 64-bit division takes a microsecond's tenth
+    s.base = (int)((uint32_t)total / (uint32_t)s.warps);
+    s.rem = (int)((uint32_t)total - (uint32_t)s.base * s.warps);
+  } else {
+    s.base = (int)(total / s.warps);
+    s.rem = (int)(total - (int64_t)s.base * s.warps);
   }
-  if ((tid & 31) == 0) s_begin[warp] = s.count ? s.begin : -1;  // the scan's barriers publish it
-  int64_t before = 0;
-  for (int base = 0; base < p.rows; base += THREADS) {
-    int n = 0, sum;
-    if (base + tid < p.rows) {
-      const AttnRow r = attn_row(p, base + tid);
-      n = r.t1 - r.t0;
-    }
-    const int64_t mine = before + block_scan<WARPS>(n, s_warp, &sum);
+  s.begin = (int64_t)id * s.base + min(id, s.rem);
+  s.count = id < s.warps ? s.base + (id < s.rem ? 1 : 0) : 0;
+  if ((tid & 31) == 0) s_begin[warp] = s.count ? s.begin : -1;
+  __syncthreads();
+  int64_t before = 0;  // tiles of the rounds before
+  for (int first = 0;;) {
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) {
       const int64_t x = s_begin[w];
       if (x >= mine * per_row && x < (mine + n) * per_row) {
-        s_row[w] = base + tid;
+        s_row[w] = first + tid;
         s_before[w] = mine;
       }
     }
+    if (p.rows <= THREADS) break;
+    block_scan<WARPS>(n, s_warp, &sum);
     before += sum;
+    first += THREADS;
+    if (first >= p.rows) break;
+    n = tiles_of(first + tid);
+    mine = before + block_scan<WARPS>(n, s_warp, &sum);
   }
   __syncthreads();
   if (s.count) {
     s.at.row = s_row[warp];
     s.at.r = attn_row(p, s.at.row);
-    const int n = s.at.r.t1 - s.at.r.t0;
+    const int nt = s.at.r.t1 - s.at.r.t0;
     const int rest = (int)(s.begin - s_before[warp] * per_row);
-    const int item = rest / n;
+    const int item = rest / nt;
     s.at.kv = item / p.blocks;
     s.at.blk = item - s.at.kv * p.blocks;
-    s.at.tile = s.at.r.t0 + rest - item * n;
+    s.at.tile = s.at.r.t0 + rest - item * nt;
   }
   return s;
 }
@@ -549,23 +562,117 @@ struct AttnTmaLoader {
   }
 };
 
-// Where a warp leaves the sums of the item it has finished its part of:
-// `begun` / `done`: the part holds the item's first / last tile.
-struct AttnPlace {
-  bool whole;
-  int64_t part;  // row of part_ml: ((worker * 2 + slot) * block_heads)
+// What the warps of a CTA leave to one another: parts of items cut by the ends
+// of shares, slot 0 of the item that another warp began, slot 1 of the one that
+// goes on in the next warp.  The sums of a warp's last part lie in its ring (rows of
+// DP + 4 floats: fragment rows then fall into different banks), those of an
+// earlier one, while the ring is still in use, in the workspace.
+template <int WARPS, int HEADS>
+struct AttnBoard {
+  float2 ml[WARPS][2][HEADS];  // maximum, sum
+  int4 item[WARPS][2];         // row, kv head, head block; w: 0 none, 1 in the workspace, 2 in the ring
+  int done[WARPS];             // the item of slot 0 ends in this warp
+  int ctas[WARPS];             // CTAs of the item of slot 1
 };
-__device__ __forceinline__ AttnPlace attn_place(const AttnParams& p, const AttnShare& s, const AttnCursor& at,
-                                                int64_t pos, bool begun, bool done) {  // pos: of tile `at`
+
+// Where a warp puts the sums of an item that it has done its part of.
+struct AttnPlace {
+  bool whole;   // to the output
+  int slot;
+  float* sums;  // else here, rows of `pitch`
+  int pitch;
+};
+template <int WARPS, int HEADS, int DP>
+__device__ __forceinline__ AttnPlace attn_place(const AttnParams& p, const AttnShare& s, AttnBoard<WARPS, HEADS>& board,
+                                                float* ring, const AttnCursor& at, int i, bool begun, bool done) {
+  const int warp = threadIdx.x >> 5;
   AttnPlace o;
   o.whole = begun && done;
-  o.part = (s.worker * 2ll + (begun ? 1 : 0)) * p.block_heads;
-  if (begun && !done && (threadIdx.x & 31) == 0) {  // the item goes on in later shares
-    const int64_t last = pos + (at.r.t1 - 1 - at.tile);  // its last tile
-    const int w = (int)(((last + 1) * s.workers - 1) / s.total);  // the worker whose share holds it
-    p.desc[s.worker] = make_int4(at.row, at.kv, at.blk, w - s.worker + 1);
+  o.slot = begun ? 1 : 0;
+  const bool last = i + 1 == s.count;
+  o.sums = last ? ring : p.warp_o + (int64_t)(blockIdx.x * WARPS + warp) * p.block_heads * p.c.dim;
+  o.pitch = last ? DP + 4 : p.c.dim;
+  if (!o.whole && (threadIdx.x & 31) == 0) {
+    board.item[warp][o.slot] = make_int4(at.row, at.kv, at.blk, last ? 2 : 1);
+    if (begun)  // its last tile is this many on
+      board.ctas[warp] = s.holder(s.begin + i + (at.r.t1 - 1 - at.tile)) / WARPS - blockIdx.x + 1;
+    else
+      board.done[warp] = done;
   }
   return o;
+}
+
+// Four elements of a head from its parts' maxima, sums and elements.
+struct AttnSum {
+  float m, l, o[4];
+  __device__ __forceinline__ void clear() { m = -INFINITY, l = o[0] = o[1] = o[2] = o[3] = 0.f; }
+  __device__ __forceinline__ void add(float pm, float pl, const float4& v) {
+    const float m2 = fmaxf(m, pm), top = m2 == -INFINITY ? 0.f : m2;
+    const float keep = exp2_fast(m - top), f = exp2_fast(pm - top);
+    m = m2;
+    l = l * keep + pl * f;
+    o[0] = o[0] * keep + v.x * f, o[1] = o[1] * keep + v.y * f, o[2] = o[2] * keep + v.z * f, o[3] = o[3] * keep + v.w * f;
+  }
+  template <typename T>
+  __device__ __forceinline__ void put(T* out) const {
+    const float f = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // NaN stays
+#pragma unroll
+    for (int e = 0; e < 4; ++e) out[e] = Chunk<T>::put(o[e] * f);
+  }
+};
+
+// Puts the warps' parts together: a chain is the parts of one item in
+// neighbouring warps; a whole item goes to the output, else its sums go to the
+// workspace for attn_join_kernel.  Block-collective; a warp takes a chain's head,
+// a lane four (of 128) elements of it.
+template <typename T, int WARPS, int HEADS, int DP>
+__device__ __forceinline__ void attn_merge(const AttnParams& p, const AttnBoard<WARPS, HEADS>& board,
+                                           const unsigned char* ring0, int ring_pitch) {
+  __syncthreads();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, dim = p.c.dim;
+  int task = 0;
+  bool shared = false;  // an item begun here goes on in the next CTA
+  for (int w0 = -1; w0 < WARPS; ++w0) {  // chains: slot 0 of warp 0 (w0 = -1), slot 1 of warp w0
+    const int w = max(w0, 0), slot = w0 < 0 ? 0 : 1;
+    const int4 item = board.item[w][slot];
+    if (item.w == 0) continue;
+    int end = w + 1;  // past the chain's last warp
+    bool closed = slot == 0 && board.done[0];
+    while (!closed && end < WARPS && board.item[end][0].w) closed = board.done[end++];
+    const bool whole = closed && slot == 1;
+    const int h0 = item.z * p.block_heads, nh = min(p.block_heads, p.group - h0);
+    if (slot == 1 && !closed) {
+      shared = true;
+      if (threadIdx.x == 0) p.desc[blockIdx.x] = make_int4(item.x, item.y, item.z, board.ctas[w]);
+    }
+    for (int h = 0; h < nh; ++h, ++task) {
+      if (task % WARPS != warp) continue;
+#pragma unroll
+      for (int d0 = 0; d0 < DP; d0 += 128) {
+        const int d = d0 + lane * 4;
+        if (d >= dim) continue;
+        AttnSum sum;
+        sum.clear();
+#pragma unroll 4
+        for (int u = w; u < end; ++u) {
+          const int sl = u == w ? slot : 0;
+          const bool in_ring = board.item[u][sl].w == 2;
+          const float* from = in_ring ? reinterpret_cast<const float*>(ring0 + u * ring_pitch) + h * (DP + 4)
+                                      : p.warp_o + ((int64_t)(blockIdx.x * WARPS + u) * p.block_heads + h) * dim;
+          const float2 ml = board.ml[u][sl][h];
+          sum.add(ml.x, ml.y, *reinterpret_cast<const float4*>(from + d));
+        }
+        if (whole) {
+          sum.put((T*)p.out + (((int64_t)item.x * p.c.kv_heads + item.y) * p.group + h0 + h) * dim + d);
+        } else {
+          const int64_t part = (blockIdx.x * 2ll + slot) * p.block_heads + h;
+          *reinterpret_cast<float4*>(p.cta_o + part * dim + d) = make_float4(sum.o[0], sum.o[1], sum.o[2], sum.o[3]);
+          if (d == 0) p.cta_ml[part] = make_float2(sum.m, sum.l);
+        }
+      }
+    }
+  }
+  if (!shared && threadIdx.x == 0) p.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
 }
 
 template <int DP>
@@ -589,22 +696,22 @@ __global__ void __launch_bounds__(AttnSimtCfg<DP>::kWarps * 32, 1) attn_simt_ker
   using Tile = AttnTileCfg<4, DP>;
   constexpr int H = Cfg::kHeads, N = Chunk<T>::N, E = DP / 32;
   extern __shared__ __align__(128) unsigned char attn_smem[];
+  __shared__ AttnBoard<Cfg::kWarps, H> board;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   unsigned char* mine = attn_smem + warp * Cfg::kWarpBytes;
   float* sq = reinterpret_cast<float*>(mine + Cfg::kStages * Tile::kStageBytes);  // [H][DP]
   float* sp = sq + H * DP;                                                        // [16][H]
   for (int i = lane; i < Cfg::kWarpBytes / 16; i += 32) reinterpret_cast<uint4*>(mine)[i] = make_uint4(0, 0, 0, 0);
+  if (lane < 2) board.item[warp][lane].w = 0;
   griddep_wait();
   griddep_launch();
   const AttnShare s = attn_share<Cfg::kWarps>(p);
-  if (lane == 0) p.desc[s.worker] = make_int4(0, 0, 0, 0);
   __syncwarp();
-  if (s.count == 0) return;
 
   AttnCopyLoader<4, DP> load;
   load.at = s.at;
   load.left = s.count;
-  load.look_up(p);
+  if (s.count) load.look_up(p);
   const uint32_t ring = smem_u32(mine);
 #pragma unroll
   for (int i = 0; i < Cfg::kStages - 1; ++i) load.issue(p, ring + i * Tile::kStageBytes);
@@ -690,25 +797,22 @@ __global__ void __launch_bounds__(AttnSimtCfg<DP>::kWarps * 32, 1) attn_simt_ker
 
     const bool done = at.tile + 1 == at.r.t1;
     if (done || i + 1 == s.count) {
-      const AttnPlace to = attn_place(p, s, at, s.begin + i, begun, done);
+      __syncwarp();  // the ring may take the sums
+      const AttnPlace to = attn_place<Cfg::kWarps, H, DP>(p, s, board, reinterpret_cast<float*>(mine), at, i, begun, done);
 #pragma unroll
       for (int h = 0; h < H; ++h) {
 #pragma unroll
         for (int d = 16; d; d >>= 1) l[h] += __shfl_xor_sync(0xffffffffu, l[h], d);
         if (h >= nh) continue;
-        const float f = to.whole ? (l[h] > 0.f ? 1.f / l[h] : 0.f) : 1.f;
-        if (!to.whole && lane == 0) p.part_ml[to.part + h] = make_float2(m[h], l[h]);
+        const float f = l[h] > 0.f ? 1.f / l[h] : (l[h] == 0.f ? 0.f : l[h]);  // NaN stays
+        if (!to.whole && lane == 0) board.ml[warp][to.slot][h] = make_float2(m[h], l[h]);
+        float* out = to.whole ? (float*)p.out + (((int64_t)at.row * p.c.kv_heads + kv) * p.group + h0 + h) * p.c.dim
+                              : to.sums + h * to.pitch;
 #pragma unroll
         for (int e = 0; e < E; e += 2) {
           const int d = e * 32 + 2 * lane;
-          if (d >= p.c.dim) continue;
-          if (to.whole) {
-            T* out = (T*)p.out + ((int64_t)at.row * p.c.kv_heads * p.group + kv * p.group + h0 + h) * p.c.dim + d;
-            out[0] = Chunk<T>::put(o[h][e] * f), out[1] = Chunk<T>::put(o[h][e + 1] * f);
-          } else {
-            float* out = p.part_o + (to.part + h) * p.c.dim + d;
-            out[0] = o[h][e], out[1] = o[h][e + 1];
-          }
+          if (d < p.c.dim) *reinterpret_cast<float2*>(out + d) = to.whole ? make_float2(o[h][e] * f, o[h][e + 1] * f)
+                                                                          : make_float2(o[h][e], o[h][e + 1]);
         }
       }
       begun = true, fresh = true;
@@ -716,6 +820,7 @@ __global__ void __launch_bounds__(AttnSimtCfg<DP>::kWarps * 32, 1) attn_simt_ker
     at.next(p);
     __syncwarp();
   }
+  attn_merge<float, Cfg::kWarps, H, DP>(p, board, attn_smem, Cfg::kWarpBytes);
 }
 
 template <int DP, int NT>
@@ -726,7 +831,7 @@ struct AttnMmaCfg {
   static constexpr int kQBytes = kQShared ? kHeads * DP * 2 : 0;
   static constexpr int kStages = DP == 256 ? 2 : (DP == 128 ? 3 : 6);
   static constexpr int kWarpBytes = kStages * Tile::kStageBytes + kQBytes;
-  static constexpr int kFit = 224 * 1024 / kWarpBytes;
+  static constexpr int kFit = 220 * 1024 / kWarpBytes;
   static constexpr int kWarps = kFit < 8 ? kFit : 8;
   static constexpr int kSmemBytes = 1024 + kWarps * kWarpBytes;  // aligned to 1024 bytes
 };
@@ -751,8 +856,10 @@ __global__ void __launch_bounds__(AttnMmaCfg<DP, NT>::kWarps * 32, 1)
   extern __shared__ __align__(128) unsigned char attn_smem[];
   __shared__ uint64_t bars[TMA ? Cfg::kWarps * STAGES : 1];
   __shared__ int abort_flag;
+  __shared__ AttnBoard<Cfg::kWarps, Cfg::kHeads> board;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  unsigned char* mine = attn_smem + ((1024 - (smem_u32(attn_smem) & 1023)) & 1023) + warp * Cfg::kWarpBytes;
+  unsigned char* rings = attn_smem + ((1024 - (smem_u32(attn_smem) & 1023)) & 1023);
+  unsigned char* mine = rings + warp * Cfg::kWarpBytes;
   const uint32_t ring = smem_u32(mine), sq = ring + STAGES * Tile::kStageBytes;
   uint64_t* bar = bars + (TMA ? warp * STAGES : 0);
   if constexpr (TMA) {
@@ -766,25 +873,24 @@ __global__ void __launch_bounds__(AttnMmaCfg<DP, NT>::kWarps * 32, 1)
   } else if (p.c.dim < DP) {  // columns that no copy fills
     for (int i = lane; i < STAGES * Tile::kStageBytes / 16; i += 32) reinterpret_cast<uint4*>(mine)[i] = make_uint4(0, 0, 0, 0);
   }
+  if (lane < 2) board.item[warp][lane].w = 0;
   griddep_wait();
   griddep_launch();
   const AttnShare s = attn_share<Cfg::kWarps>(p);
-  if (lane == 0) p.desc[s.worker] = make_int4(0, 0, 0, 0);
   __syncwarp();
-  if (s.count == 0) return;
 
   AttnCopyLoader<2, DP> copy;
   AttnTmaLoader<DP> tma;
   if constexpr (TMA) {
     tma.at = s.at, tma.left = s.count;
-    if (lane == 0) {
+    if (lane == 0 && s.count) {
       tma.look_up(p);
 #pragma unroll
       for (int i = 0; i < STAGES - 1; ++i) tma.issue(p, &mk, &mv, ring + i * Tile::kStageBytes, bar + i);
     }
   } else {
     copy.at = s.at, copy.left = s.count;
-    copy.look_up(p);
+    if (s.count) copy.look_up(p);
 #pragma unroll
     for (int i = 0; i < STAGES - 1; ++i) copy.issue(p, ring + i * Tile::kStageBytes);
   }
@@ -849,7 +955,7 @@ __global__ void __launch_bounds__(AttnMmaCfg<DP, NT>::kWarps * 32, 1)
           mbar_drain(bar + stage, parity);
           if (++stage == STAGES) stage = 0, parity ^= 1;
         }
-        return;
+        break;  // to the CTA's barrier, with the status raised
       }
     } else {
       cp_async_wait<STAGES - 2>();
@@ -948,7 +1054,9 @@ __global__ void __launch_bounds__(AttnMmaCfg<DP, NT>::kWarps * 32, 1)
 
     const bool done = at.tile + 1 == at.r.t1;
     if (done || i + 1 == s.count) {
-      const AttnPlace to = attn_place(p, s, at, s.begin + i, begun, done);
+      __syncwarp();  // the ring may take the sums
+      const AttnPlace to = attn_place<Cfg::kWarps, Cfg::kHeads, DP>(p, s, board, reinterpret_cast<float*>(mine), at, i,
+                                                                    begun, done);
       const int h0 = at.blk * p.block_heads, nh = min(p.block_heads, p.group - h0);
       const int64_t head0 = ((int64_t)at.row * p.c.kv_heads + at.kv) * p.group + h0;
 #pragma unroll
@@ -961,10 +1069,10 @@ __global__ void __launch_bounds__(AttnMmaCfg<DP, NT>::kWarps * 32, 1)
           sum += __shfl_xor_sync(0xffffffffu, sum, 16);
           const int h = nt * 8 + (lane & 3) * 2 + j;
           if (h >= nh) continue;
-          const float f = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
-          if (!to.whole && lane < 4) p.part_ml[to.part + h] = make_float2(m[nt][j], sum);
+          const float f = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);  // NaN stays
+          if (!to.whole && lane < 4) board.ml[warp][to.slot][h] = make_float2(m[nt][j], sum);
           T* out = (T*)p.out + (head0 + h) * p.c.dim;
-          float* part = p.part_o + (to.part + h) * p.c.dim;
+          float* part = to.sums + h * to.pitch;
 #pragma unroll
           for (int mt = 0; mt < KS; ++mt)
 #pragma unroll
@@ -983,56 +1091,48 @@ __global__ void __launch_bounds__(AttnMmaCfg<DP, NT>::kWarps * 32, 1)
     at.next(p);
     __syncwarp();
   }
+  attn_merge<T, Cfg::kWarps, Cfg::kHeads, DP>(p, board, rings, Cfg::kWarpBytes);
 }
 
-// Joins the parts of the items that share ends cut.  CTA (w, h): head h of the
-// item that begins in worker w's share and goes on in the next ones, if there
-// is one; its warps take the parts in turn, a lane four elements.
+// Joins the parts of the items that several CTAs share.  CTA (c, y): heads y,
+// y + gridDim.y, ... of the item that begins in CTA c of the attention grid and
+// goes on in the next ones, if there is one; its warps take the parts in turn.
 constexpr int kJoinWarps = 8;
 template <typename T>
 __global__ void __launch_bounds__(kJoinWarps * 32) attn_join_kernel(const AttnParams p) {
-  __shared__ float s_o[kJoinWarps][256];
-  __shared__ float s_l[kJoinWarps], s_m[kJoinWarps];
+  __shared__ float4 s_o[kJoinWarps][64];
+  __shared__ float2 s_ml[kJoinWarps];
   griddep_wait();
   griddep_launch();
-  const int4 d = p.desc[blockIdx.x];
-  const int h = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (d.w == 0) return;
-  const int kv = d.y, h0 = d.z * p.block_heads, dim = p.c.dim;
-  if (h0 + h >= p.group) return;
-  float m = -INFINITY, l = 0.f, o[8];
+  const int4 item = p.desc[blockIdx.x];
+  if (item.w == 0) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, dim = p.c.dim;
+  const int h0 = item.z * p.block_heads, nh = min(p.block_heads, p.group - h0);
+  for (int h = blockIdx.y; h < nh; h += gridDim.y) {
+    AttnSum a, b;  // elements 4 lane .. and 128 + 4 lane ..
+    a.clear(), b.clear();
+#pragma unroll 2
+    for (int i = warp; i < item.w; i += kJoinWarps) {
+      const int64_t part = ((blockIdx.x + i) * 2ll + (i == 0 ? 1 : 0)) * p.block_heads + h;
+      const float2 ml = p.cta_ml[part];
+      const float* o = p.cta_o + part * dim;
+      a.add(ml.x, ml.y, lane * 4 < dim ? *reinterpret_cast<const float4*>(o + lane * 4) : make_float4(0, 0, 0, 0));
+      if (dim > 128)
+        b.add(ml.x, ml.y, 128 + lane * 4 < dim ? *reinterpret_cast<const float4*>(o + 128 + lane * 4) : make_float4(0, 0, 0, 0));
+    }
+    __syncthreads();  // the head before has been read
+    s_o[warp][lane] = make_float4(a.o[0], a.o[1], a.o[2], a.o[3]);
+    if (dim > 128) s_o[warp][32 + lane] = make_float4(b.o[0], b.o[1], b.o[2], b.o[3]);
+    if (lane == 0) s_ml[warp] = make_float2(a.m, a.l);
+    __syncthreads();
+    const int e = threadIdx.x;  // four elements
+    if (e * 4 < dim) {
+      AttnSum sum;
+      sum.clear();
 #pragma unroll
-  for (int e = 0; e < 8; ++e) o[e] = 0.f;
-  for (int i = warp; i < d.w; i += kJoinWarps) {
-    const int64_t part = ((blockIdx.x + i) * 2ll + (i == 0 ? 1 : 0)) * p.block_heads + h;
-    const float2 ml = p.part_ml[part];
-    float4 a = make_float4(0, 0, 0, 0), b = a;
-    if (lane * 4 < dim) a = *reinterpret_cast<const float4*>(p.part_o + part * dim + lane * 4);
-    if (128 + lane * 4 < dim) b = *reinterpret_cast<const float4*>(p.part_o + part * dim + 128 + lane * 4);
-    const float m2 = fmaxf(m, ml.x), base = m2 == -INFINITY ? 0.f : m2;
-    const float keep = exp2_fast(m - base), f = exp2_fast(ml.x - base);
-    m = m2;
-    l = l * keep + ml.y * f;
-    o[0] = o[0] * keep + a.x * f, o[1] = o[1] * keep + a.y * f, o[2] = o[2] * keep + a.z * f, o[3] = o[3] * keep + a.w * f;
-    o[4] = o[4] * keep + b.x * f, o[5] = o[5] * keep + b.y * f, o[6] = o[6] * keep + b.z * f, o[7] = o[7] * keep + b.w * f;
-  }
-#pragma unroll
-  for (int e = 0; e < 4; ++e) s_o[warp][lane * 4 + e] = o[e], s_o[warp][128 + lane * 4 + e] = o[4 + e];
-  if (lane == 0) s_m[warp] = m, s_l[warp] = l;
-  __syncthreads();
-  float top = -INFINITY, sum = 0.f, f[kJoinWarps];
-#pragma unroll
-  for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, s_m[w]);
-  const float base = top == -INFINITY ? 0.f : top;
-#pragma unroll
-  for (int w = 0; w < kJoinWarps; ++w) f[w] = exp2_fast(s_m[w] - base), sum += s_l[w] * f[w];
-  const float inv = sum > 0.f ? 1.f / sum : 0.f;
-  T* out = (T*)p.out + ((int64_t)d.x * p.c.kv_heads * p.group + kv * p.group + h0 + h) * dim;
-  for (int e = threadIdx.x; e < dim; e += kJoinWarps * 32) {
-    float x = 0.f;
-#pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w) x += s_o[w][e] * f[w];
-    out[e] = Chunk<T>::put(x * inv);
+      for (int w = 0; w < kJoinWarps; ++w) sum.add(s_ml[w].x, s_ml[w].y, s_o[w][e]);
+      sum.put((T*)p.out + (((int64_t)item.x * p.c.kv_heads + item.y) * p.group + h0 + h) * dim + e * 4);
+    }
   }
 }
 

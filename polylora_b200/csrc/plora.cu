@@ -660,7 +660,7 @@ constexpr int64_t kPagedMaxRows = 1 << 20;
 // large as registers allow, for a second block reads the cache again.
 struct AttnPlan {
   int dp, eights, blocks, block_heads, warps;
-  size_t ml_offset, desc_offset, bytes;
+  size_t cta_offset, ml_offset, desc_offset, bytes;
 };
 AttnPlan attn_plan(int32_t heads, int32_t kv_heads, int32_t dim, int dtype) {
   AttnPlan a;
@@ -682,10 +682,11 @@ AttnPlan attn_plan(int32_t heads, int32_t kv_heads, int32_t dim, int dtype) {
     PLORA_WARPS(256, 1) PLORA_WARPS(256, 2)
 #undef PLORA_WARPS
   }
-  const size_t workers = (size_t)kAttnGrid * a.warps, parts = workers * 2 * a.block_heads;
-  a.ml_offset = align256(parts * dim * 4);
+  const size_t parts = (size_t)kAttnGrid * 2 * a.block_heads;
+  a.cta_offset = align256((size_t)kAttnGrid * a.warps * a.block_heads * dim * 4);
+  a.ml_offset = a.cta_offset + align256(parts * dim * 4);
   a.desc_offset = a.ml_offset + align256(parts * 8);
-  a.bytes = a.desc_offset + align256(workers * 16);
+  a.bytes = a.desc_offset + align256((size_t)kAttnGrid * 16);
   return a;
 }
 
@@ -780,7 +781,7 @@ cudaError_t launch_attn(const AttnParams& p, const AttnPlan& a, int dtype, bool 
 #undef PLORA_MMA
 #undef PLORA_SIMT
   if (e != cudaSuccess) return e;
-  const dim3 grid((unsigned)(kAttnGrid * a.warps), (unsigned)a.block_heads), block(kJoinWarps * 32);
+  const dim3 grid(kAttnGrid, (unsigned)std::min(a.block_heads, 4)), block(kJoinWarps * 32);
   return dtype == PLORA_DTYPE_F32   ? launch_kernel(attn_join_kernel<float>, grid, block, 0, s, true, 0, p)
          : dtype == PLORA_DTYPE_F16 ? launch_kernel(attn_join_kernel<__half>, grid, block, 0, s, true, 0, p)
                                     : launch_kernel(attn_join_kernel<__nv_bfloat16>, grid, block, 0, s, true, 0, p);
@@ -1186,8 +1187,9 @@ int plora_paged_attention(const void* q, int64_t q_row_stride, int64_t q_head_st
   p.window = (int32_t)std::min<int64_t>(window, INT32_MAX);
   p.scale_log2 = scale * 1.4426950408889634f;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  p.part_o = reinterpret_cast<float*>(ws);
-  p.part_ml = reinterpret_cast<float2*>(ws + a.ml_offset);
+  p.warp_o = reinterpret_cast<float*>(ws);
+  p.cta_o = reinterpret_cast<float*>(ws + a.cta_offset);
+  p.cta_ml = reinterpret_cast<float2*>(ws + a.ml_offset);
   p.desc = reinterpret_cast<int4*>(ws + a.desc_offset);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   CUtensorMap mk = {}, mv = {};
