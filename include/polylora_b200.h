@@ -355,7 +355,7 @@ int plora_paged_append(const void* q, int64_t q_row_stride, int64_t q_token_stri
                        int32_t kv_heads, int32_t head_dim, int32_t page_size, int64_t num_pages, int64_t max_pages,
                        int32_t dtype, void* stream);
 
-size_t plora_paged_attention_workspace(int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t dtype);
+size_t plora_paged_attention_workspace(int64_t rows, int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t dtype);
 
 int plora_paged_attention(const void* q, int64_t q_row_stride, int64_t q_head_stride, const void* k_cache,
                           const void* v_cache, int64_t k_page_stride, int64_t v_page_stride,

@@ -7,6 +7,8 @@
 // table[p / page_size].
 #pragma once
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "sgmv_grid.cuh"
 #include "sgmv_stream.cuh"
@@ -270,14 +272,19 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const Appe
 //
 // Bound by HBM: the cache is read once, 4 * group flops for each 2 * elem
 // bytes.  The rows' lengths are known on the device only, so the work is cut
-// there: an item is a row and a key-value head (or a block of its query
-// heads), a tile 16 of its tokens, and the tiles of all items in order are
-// dealt in equal contiguous shares to the grid's warps, each of which streams
-// its share through a ring of shared-memory stages of its own (no barrier
-// between warps).  An item cut by the ends of shares is put together in two
-// steps: first the parts of a CTA's warps, then, by attn_join_kernel, what the
-// CTAs left in the workspace, always in the order of the shares.  Every item has
-// at least one (empty) tile, so rows without tokens are written too.
+// there.  An item is a row and a key-value head (or a block of its query
+// heads), a tile 16 of its tokens; every item has at least one (empty) tile, so
+// rows without tokens are written too.  The list of all items' tiles is cut into
+// segments, which warps stream through a ring of shared-memory stages of their
+// own, with no barrier between them.
+//
+// Where there is much to do, the first three quarters of the list are dealt in
+// equal segments to the grid's warps and the rest in small ones to whoever asks
+// next: SMs of a GPC share its way to memory, and with equal shares alone the
+// slowest warp of a 2 GB call ended 17 % after the mean (325 and 277 us).  The
+// segments' bounds depend on the lengths only, not on who takes them, and an item
+// cut by them is put together in the order of the list (attn_join_kernel), so
+// results do not depend on timing.
 constexpr int kAttnTile = 16;
 
 // 2^x to 2 ulp; results below 2^-126 are zero, next to a largest term of 1.
@@ -295,12 +302,25 @@ struct AttnParams {
   int64_t q_row, q_head;
   int32_t rows, group, blocks, block_heads, window;  // blocks of block_heads query heads cover a group
   float scale_log2;                                  // scale * log2(e)
-  // workspace.  A part of an item: its sums of block_heads heads, and for each
-  // head its maximum (in units of scale_log2) and sum of probabilities
-  float* warp_o;   // (warps, block_heads, dim): a warp's part of the item that another began
-  float* cta_o;    // (CTAs, 2, block_heads, dim): a CTA's parts of the items that it shares (0: begun by
-  float2* cta_ml;  // (CTAs, 2, block_heads)       another, 1: begun here)
-  int4* desc;      // (CTAs): row, kv head, head block, CTAs of the item begun here and shared (0: none)
+  // workspace
+  struct AttnWork* work;
+  int64_t* before;  // (rows): tiles of the rows before, per item
+  int4* cut;        // items cut by segments: row, item of the row, segment it begins in, segments; those of
+  int cut_room;     // more than kJoinAlone segments from the end of the list (of cut_room entries) backwards
+  // a segment's parts of cut items (0: begun in an earlier one, 1: begun here): the
+  // sums of block_heads heads, and for each its maximum (in units of scale_log2)
+  // and sum of probabilities
+  float* part_o;    // (segments, 2, block_heads, dim)
+  float2* part_ml;  // (segments, 2, block_heads)
+};
+
+// The list of tiles and its segments: `dealt` of base or (the first rem) base + 1
+// tiles, then `asked` of `chunk` tiles (the last one of what is left).
+struct AttnWork {
+  int64_t total;
+  int dealt, base, rem, asked, chunk;
+  int next;  // the next segment to be asked for
+  int cuts[2];  // entries of the list of cut items, from its begin and from its end
 };
 
 struct AttnRow {
@@ -336,19 +356,6 @@ struct AttnCursor {
   }
 };
 
-struct AttnShare {
-  int64_t begin;  // first tile of this warp in the list
-  int count;      // its tiles
-  int warps;      // warps with a share, of all CTAs; warp w of CTA c is number c * WARPS + w
-  int base, rem;  // the first rem of them have base + 1 tiles, the others base
-  AttnCursor at;  // at `begin`
-  // The warp whose share holds tile x of the list.
-  __device__ __forceinline__ int holder(int64_t x) const {
-    const int64_t split = (int64_t)rem * (base + 1);
-    return x < split ? (int)(x / (base + 1)) : rem + (int)((x - split) / base);
-  }
-};
-
 // Sum over the CTA's threads before this one (exclusive) and over all of them.
 template <int WARPS>
 __device__ __forceinline__ int block_scan(int v, int* s_warp, int* total) {
@@ -372,73 +379,156 @@ __device__ __forceinline__ int block_scan(int v, int* s_warp, int* total) {
   return before + incl - v;
 }
 
-// The calling warp's share.  Block-collective; warps without one get count 0.
-template <int WARPS>
-__device__ __forceinline__ AttnShare attn_share(const AttnParams& p) {
-  constexpr int THREADS = WARPS * 32;
-  __shared__ int s_warp[WARPS];
-  __shared__ int s_row[WARPS];
-  __shared__ int64_t s_before[WARPS], s_begin[WARPS];
-  const int tid = threadIdx.x, warp = tid >> 5;
-  const int per_row = p.c.kv_heads * p.blocks;
-  auto tiles_of = [&](int row) {
-    if (row >= p.rows) return 0;
-    const AttnRow r = attn_row(p, row);
-    return r.t1 - r.t0;
-  };
-  // tiles of the rows before this thread's (of the last round), and of all
-  int n = tiles_of(tid), sum;
-  int64_t mine = block_scan<WARPS>(n, s_warp, &sum), tiles = sum;
-  for (int first = THREADS; first < p.rows; first += THREADS) {
-    block_scan<WARPS>(tiles_of(first + tid), s_warp, &sum);
+// Segments that a call may have, for `warps` of the grid and block_heads heads: a
+// part costs 4 * block_heads * dim bytes and a tile 64 * dim, so small segments are
+// as many as keep the parts below a sixteenth of the cache's bytes.
+__host__ __device__ constexpr int attn_asked_max(int warps, int block_heads) {
+  return warps * (block_heads <= 4 ? 4 : (block_heads <= 8 ? 2 : 1));
+}
+constexpr int kAttnPlanThreads = 1024;
+constexpr int kAttnDealOnly = 32;   // tiles a warp up to which all are dealt
+constexpr int kAttnChunk = 8;       // smallest chunk: a loader's lead of up to 5 tiles then spans two segments
+constexpr int kAttnAsk = 4;         // tiles ahead of which the next segment is asked for
+
+// Counts the tiles of the rows and cuts their list.  One CTA.
+__global__ void __launch_bounds__(kAttnPlanThreads) attn_plan_kernel(const AttnParams p, int warps) {
+  __shared__ int s_warp[kAttnPlanThreads / 32];
+  griddep_wait();
+  griddep_launch();
+  int64_t tiles = 0;
+  for (int first = 0; first < p.rows; first += kAttnPlanThreads) {
+    const int row = first + threadIdx.x;
+    int n = 0, sum;
+    if (row < p.rows) {
+      const AttnRow r = attn_row(p, row);
+      n = r.t1 - r.t0;
+    }
+    const int before = block_scan<kAttnPlanThreads / 32>(n, s_warp, &sum);
+    if (row < p.rows) p.before[row] = tiles + before;
     tiles += sum;
   }
-  const int64_t total = tiles * per_row;
-  AttnShare s;
-  const int all = gridDim.x * WARPS, id = blockIdx.x * WARPS + warp;
-  s.warps = total < all ? (int)total : all;
-  if (total <= INT32_MAX) {  // a 64-bit division takes a microsecond's tenth
-    s.base = (int)((uint32_t)total / (uint32_t)s.warps);
-    s.rem = (int)((uint32_t)total - (uint32_t)s.base * s.warps);
-  } else {
-    s.base = (int)(total / s.warps);
-    s.rem = (int)(total - (int64_t)s.base * s.warps);
-  }
-  s.begin = (int64_t)id * s.base + min(id, s.rem);
-  s.count = id < s.warps ? s.base + (id < s.rem ? 1 : 0) : 0;
-  if ((tid & 31) == 0) s_begin[warp] = s.count ? s.begin : -1;
-  __syncthreads();
-  int64_t before = 0;  // tiles of the rounds before
-  for (int first = 0;;) {
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
-      const int64_t x = s_begin[w];
-      if (x >= mine * per_row && x < (mine + n) * per_row) {
-        s_row[w] = first + tid;
-        s_before[w] = mine;
-      }
+  if (threadIdx.x == 0) {
+    AttnWork w;
+    w.total = tiles * p.c.kv_heads * p.blocks;
+    w.next = w.cuts[0] = w.cuts[1] = 0;
+    if (w.total < (int64_t)warps * kAttnDealOnly) {
+      w.dealt = (int)(w.total < warps ? w.total : warps);
+      w.base = (int)w.total / w.dealt;  // total < 32 warps here
+      w.rem = (int)w.total - w.base * w.dealt;
+      w.asked = 0, w.chunk = 1;
+    } else {
+      w.dealt = warps;
+      w.base = (int)(w.total / 4 * 3 / warps);
+      w.rem = 0;
+      const int64_t rest = w.total - (int64_t)w.base * warps;
+      const int most = attn_asked_max(warps, p.block_heads);
+      const int64_t chunk = (rest + most - 1) / most;
+      w.chunk = (int)max(chunk, (int64_t)max(kAttnChunk, p.block_heads));
+      w.asked = (int)((rest + w.chunk - 1) / w.chunk);
     }
-    if (p.rows <= THREADS) break;
-    block_scan<WARPS>(n, s_warp, &sum);
-    before += sum;
-    first += THREADS;
-    if (first >= p.rows) break;
-    n = tiles_of(first + tid);
-    mine = before + block_scan<WARPS>(n, s_warp, &sum);
+    *p.work = w;
   }
-  __syncthreads();
-  if (s.count) {
-    s.at.row = s_row[warp];
-    s.at.r = attn_row(p, s.at.row);
-    const int nt = s.at.r.t1 - s.at.r.t0;
-    const int rest = (int)(s.begin - s_before[warp] * per_row);
-    const int item = rest / nt;
+}
+
+// A segment of the list: tiles [begin, begin + count) from `at` on.
+struct AttnSegment {
+  AttnCursor at;
+  int id, count;
+  int64_t begin;
+};
+
+// What a warp knows of the list.
+struct AttnList {
+  AttnWork w;
+  __device__ __forceinline__ void read(const AttnParams& p) {
+    w.total = ld_cg_i64(&p.work->total);
+    w.dealt = ld_cg_i32(&p.work->dealt), w.base = ld_cg_i32(&p.work->base), w.rem = ld_cg_i32(&p.work->rem);
+    w.asked = ld_cg_i32(&p.work->asked), w.chunk = ld_cg_i32(&p.work->chunk);
+  }
+  __device__ __forceinline__ int64_t dealt_tiles() const { return (int64_t)w.dealt * w.base + w.rem; }
+  // The segment that holds tile x.
+  __device__ __forceinline__ int holder(int64_t x) const {
+    if (x >= dealt_tiles()) return w.dealt + (int)((x - dealt_tiles()) / w.chunk);
+    const int64_t split = (int64_t)w.rem * (w.base + 1);
+    return x < split ? (int)(x / (w.base + 1)) : w.rem + (int)((x - split) / w.base);
+  }
+  // Segment id < dealt + asked.  Warp-collective.
+  __device__ __forceinline__ AttnSegment segment(const AttnParams& p, int id) const {
+    AttnSegment s;
+    s.id = id;
+    if (id < w.dealt) {
+      s.begin = (int64_t)id * w.base + min(id, w.rem);
+      s.count = w.base + (id < w.rem ? 1 : 0);
+    } else {
+      s.begin = dealt_tiles() + (int64_t)(id - w.dealt) * w.chunk;
+      s.count = (int)min((int64_t)w.chunk, w.total - s.begin);
+    }
+    // the last row that begins at or before s.begin: 32 probes a round
+    const int lane = threadIdx.x & 31, per_row = p.c.kv_heads * p.blocks;
+    int lo = 0, hi = p.rows;
+    int64_t first = 0;  // tiles before row lo
+    while (hi - lo > 1) {
+      const int step = (hi - lo + 31) / 32, at = lo + (lane + 1) * step;
+      int64_t v = 0;
+      bool le = false;
+      if (at < hi) {
+        v = ld_cg_i64(p.before + at) * per_row;
+        le = v <= s.begin;
+      }
+      const int k = __popc(__ballot_sync(0xffffffffu, le));
+      if (k) first = __shfl_sync(0xffffffffu, v, k - 1);
+      lo += k * step;
+      hi = min(hi, lo + step);
+    }
+    s.at.row = lo;
+    s.at.r = attn_row(p, lo);
+    const int n = s.at.r.t1 - s.at.r.t0;
+    const int rest = (int)(s.begin - first), item = rest / n;
     s.at.kv = item / p.blocks;
     s.at.blk = item - s.at.kv * p.blocks;
-    s.at.tile = s.at.r.t0 + rest - item * nt;
+    s.at.tile = s.at.r.t0 + rest - item * n;
+    return s;
   }
-  return s;
-}
+};
+
+// A warp's walk through its segments: the one that it computes, and the next,
+// into which its loader may have run ahead.
+struct AttnWalk {
+  AttnList list;
+  AttnSegment cur, nxt;
+  int asked;      // lane 0: the segment asked for last
+  bool more;      // there may be another one
+  bool have_nxt;
+  // False when this warp has nothing to do.
+  __device__ __forceinline__ bool start(const AttnParams& p) {
+    list.read(p);
+    // few segments spread over the SMs
+    const int id = (threadIdx.x >> 5) * gridDim.x + blockIdx.x;
+    if (id >= list.w.dealt) return false;
+    more = list.w.asked > 0, have_nxt = false;
+    cur = list.segment(p, id);
+    return true;
+  }
+  // Called before each copy of a loader with `left` tiles to start: asks for the
+  // next segment a few tiles ahead (every one but the last is longer), and with
+  // nothing left moves the loader to it.
+  __device__ __forceinline__ bool look_ahead(const AttnParams& p, int left) {
+    if (!more) return false;
+    if (left == kAttnAsk && (threadIdx.x & 31) == 0) asked = list.w.dealt + atomicAdd(&p.work->next, 1);
+    if (left > 0) return false;
+    const int id = __shfl_sync(0xffffffffu, asked, 0), ids = list.w.dealt + list.w.asked;
+    more = id + 1 < ids;
+    if (id >= ids) return false;
+    nxt = list.segment(p, id);
+    have_nxt = true;
+    return true;
+  }
+  __device__ __forceinline__ bool step() {
+    if (!have_nxt) return false;
+    cur = nxt, have_nxt = false;
+    return true;
+  }
+};
 
 // cp_async16 that writes zeros instead where `ok` is false.
 __device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool ok) {
@@ -472,6 +562,10 @@ struct AttnCopyLoader {
   int left;
   int page, inner;  // of this lane's token of tile `at`; page -1: reads as zeros
 
+  __device__ __forceinline__ void start(const AttnParams& p, const AttnSegment& s) {
+    at = s.at, left = s.count;
+    look_up(p);
+  }
   __device__ __forceinline__ void look_up(const AttnParams& p) {
     page = -1, inner = 0;
     if (left <= 0) return;
@@ -527,6 +621,10 @@ struct AttnTmaLoader {
   int left;
   int page, slot;  // of tile `at`
 
+  __device__ __forceinline__ void start(const AttnParams& p, const AttnSegment& s) {
+    at = s.at, left = s.count;
+    look_up(p);
+  }
   __device__ __forceinline__ void look_up(const AttnParams& p) {
     if (left <= 0) return;
     page = p.c.num_pages, slot = 0;
@@ -541,13 +639,15 @@ struct AttnTmaLoader {
       }
     }
   }
-  // One lane's: starts the copies of tile `at`, completing on `bar`, and steps on.
+  // Lane 0 starts the copies of tile `at`, completing on `bar`; all step on.
   __device__ __forceinline__ void issue(const AttnParams& p, const CUtensorMap* mk, const CUtensorMap* mv,
                                         uint32_t stage, uint64_t* bar) {
     if (left <= 0) return;
-    mbar_arrive_expect_tx(bar, Tile::kStageBytes);
-    tma_load_tile(stage, mk, bar, slot, at.kv, page);
-    tma_load_tile(stage + Tile::kTileBytes, mv, bar, slot, at.kv, page);
+    if ((threadIdx.x & 31) == 0) {
+      mbar_arrive_expect_tx(bar, Tile::kStageBytes);
+      tma_load_tile(stage, mk, bar, slot, at.kv, page);
+      tma_load_tile(stage + Tile::kTileBytes, mv, bar, slot, at.kv, page);
+    }
     at.next(p);
     --left;
     look_up(p);
@@ -562,117 +662,25 @@ struct AttnTmaLoader {
   }
 };
 
-// What the warps of a CTA leave to one another: parts of items cut by the ends
-// of shares, slot 0 of the item that another warp began, slot 1 of the one that
-// goes on in the next warp.  The sums of a warp's last part lie in its ring (rows of
-// DP + 4 floats: fragment rows then fall into different banks), those of an
-// earlier one, while the ring is still in use, in the workspace.
-template <int WARPS, int HEADS>
-struct AttnBoard {
-  float2 ml[WARPS][2][HEADS];  // maximum, sum
-  int4 item[WARPS][2];         // row, kv head, head block; w: 0 none, 1 in the workspace, 2 in the ring
-  int done[WARPS];             // the item of slot 0 ends in this warp
-  int ctas[WARPS];             // CTAs of the item of slot 1
-};
+constexpr int kJoinAlone = 32;  // parts that one warp joins
 
-// Where a warp puts the sums of an item that it has done its part of.
+// Where the sums of an item go whose part of segment `s` ends with its i-th tile:
+// the output, or row `part` of the parts.
 struct AttnPlace {
-  bool whole;   // to the output
-  int slot;
-  float* sums;  // else here, rows of `pitch`
-  int pitch;
+  bool whole;
+  int64_t part;
 };
-template <int WARPS, int HEADS, int DP>
-__device__ __forceinline__ AttnPlace attn_place(const AttnParams& p, const AttnShare& s, AttnBoard<WARPS, HEADS>& board,
-                                                float* ring, const AttnCursor& at, int i, bool begun, bool done) {
-  const int warp = threadIdx.x >> 5;
+__device__ __forceinline__ AttnPlace attn_place(const AttnParams& p, const AttnList& list, const AttnSegment& s,
+                                                const AttnCursor& at, int i, bool begun, bool done) {
   AttnPlace o;
   o.whole = begun && done;
-  o.slot = begun ? 1 : 0;
-  const bool last = i + 1 == s.count;
-  o.sums = last ? ring : p.warp_o + (int64_t)(blockIdx.x * WARPS + warp) * p.block_heads * p.c.dim;
-  o.pitch = last ? DP + 4 : p.c.dim;
-  if (!o.whole && (threadIdx.x & 31) == 0) {
-    board.item[warp][o.slot] = make_int4(at.row, at.kv, at.blk, last ? 2 : 1);
-    if (begun)  // its last tile is this many on
-      board.ctas[warp] = s.holder(s.begin + i + (at.r.t1 - 1 - at.tile)) / WARPS - blockIdx.x + 1;
-    else
-      board.done[warp] = done;
+  o.part = (s.id * 2ll + (begun ? 1 : 0)) * p.block_heads;
+  if (begun && !done && (threadIdx.x & 31) == 0) {  // it goes on in the next segments, to the one of its last tile
+    const int segments = list.holder(s.begin + i + (at.r.t1 - 1 - at.tile)) - s.id + 1;
+    const int far = segments > kJoinAlone, n = atomicAdd(&p.work->cuts[far], 1);
+    p.cut[far ? p.cut_room - 1 - n : n] = make_int4(at.row, at.kv * p.blocks + at.blk, s.id, segments);
   }
   return o;
-}
-
-// Four elements of a head from its parts' maxima, sums and elements.
-struct AttnSum {
-  float m, l, o[4];
-  __device__ __forceinline__ void clear() { m = -INFINITY, l = o[0] = o[1] = o[2] = o[3] = 0.f; }
-  __device__ __forceinline__ void add(float pm, float pl, const float4& v) {
-    const float m2 = fmaxf(m, pm), top = m2 == -INFINITY ? 0.f : m2;
-    const float keep = exp2_fast(m - top), f = exp2_fast(pm - top);
-    m = m2;
-    l = l * keep + pl * f;
-    o[0] = o[0] * keep + v.x * f, o[1] = o[1] * keep + v.y * f, o[2] = o[2] * keep + v.z * f, o[3] = o[3] * keep + v.w * f;
-  }
-  template <typename T>
-  __device__ __forceinline__ void put(T* out) const {
-    const float f = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // NaN stays
-#pragma unroll
-    for (int e = 0; e < 4; ++e) out[e] = Chunk<T>::put(o[e] * f);
-  }
-};
-
-// Puts the warps' parts together: a chain is the parts of one item in
-// neighbouring warps; a whole item goes to the output, else its sums go to the
-// workspace for attn_join_kernel.  Block-collective; a warp takes a chain's head,
-// a lane four (of 128) elements of it.
-template <typename T, int WARPS, int HEADS, int DP>
-__device__ __forceinline__ void attn_merge(const AttnParams& p, const AttnBoard<WARPS, HEADS>& board,
-                                           const unsigned char* ring0, int ring_pitch) {
-  __syncthreads();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, dim = p.c.dim;
-  int task = 0;
-  bool shared = false;  // an item begun here goes on in the next CTA
-  for (int w0 = -1; w0 < WARPS; ++w0) {  // chains: slot 0 of warp 0 (w0 = -1), slot 1 of warp w0
-    const int w = max(w0, 0), slot = w0 < 0 ? 0 : 1;
-    const int4 item = board.item[w][slot];
-    if (item.w == 0) continue;
-    int end = w + 1;  // past the chain's last warp
-    bool closed = slot == 0 && board.done[0];
-    while (!closed && end < WARPS && board.item[end][0].w) closed = board.done[end++];
-    const bool whole = closed && slot == 1;
-    const int h0 = item.z * p.block_heads, nh = min(p.block_heads, p.group - h0);
-    if (slot == 1 && !closed) {
-      shared = true;
-      if (threadIdx.x == 0) p.desc[blockIdx.x] = make_int4(item.x, item.y, item.z, board.ctas[w]);
-    }
-    for (int h = 0; h < nh; ++h, ++task) {
-      if (task % WARPS != warp) continue;
-#pragma unroll
-      for (int d0 = 0; d0 < DP; d0 += 128) {
-        const int d = d0 + lane * 4;
-        if (d >= dim) continue;
-        AttnSum sum;
-        sum.clear();
-#pragma unroll 4
-        for (int u = w; u < end; ++u) {
-          const int sl = u == w ? slot : 0;
-          const bool in_ring = board.item[u][sl].w == 2;
-          const float* from = in_ring ? reinterpret_cast<const float*>(ring0 + u * ring_pitch) + h * (DP + 4)
-                                      : p.warp_o + ((int64_t)(blockIdx.x * WARPS + u) * p.block_heads + h) * dim;
-          const float2 ml = board.ml[u][sl][h];
-          sum.add(ml.x, ml.y, *reinterpret_cast<const float4*>(from + d));
-        }
-        if (whole) {
-          sum.put((T*)p.out + (((int64_t)item.x * p.c.kv_heads + item.y) * p.group + h0 + h) * dim + d);
-        } else {
-          const int64_t part = (blockIdx.x * 2ll + slot) * p.block_heads + h;
-          *reinterpret_cast<float4*>(p.cta_o + part * dim + d) = make_float4(sum.o[0], sum.o[1], sum.o[2], sum.o[3]);
-          if (d == 0) p.cta_ml[part] = make_float2(sum.m, sum.l);
-        }
-      }
-    }
-  }
-  if (!shared && threadIdx.x == 0) p.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
 }
 
 template <int DP>
@@ -696,31 +704,32 @@ __global__ void __launch_bounds__(AttnSimtCfg<DP>::kWarps * 32, 1) attn_simt_ker
   using Tile = AttnTileCfg<4, DP>;
   constexpr int H = Cfg::kHeads, N = Chunk<T>::N, E = DP / 32;
   extern __shared__ __align__(128) unsigned char attn_smem[];
-  __shared__ AttnBoard<Cfg::kWarps, H> board;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   unsigned char* mine = attn_smem + warp * Cfg::kWarpBytes;
   float* sq = reinterpret_cast<float*>(mine + Cfg::kStages * Tile::kStageBytes);  // [H][DP]
   float* sp = sq + H * DP;                                                        // [16][H]
-  for (int i = lane; i < Cfg::kWarpBytes / 16; i += 32) reinterpret_cast<uint4*>(mine)[i] = make_uint4(0, 0, 0, 0);
-  if (lane < 2) board.item[warp][lane].w = 0;
+  if (p.c.dim < DP)  // columns that no copy fills
+    for (int i = lane; i < Cfg::kWarpBytes / 16; i += 32) reinterpret_cast<uint4*>(mine)[i] = make_uint4(0, 0, 0, 0);
+  __syncwarp();
   griddep_wait();
   griddep_launch();
-  const AttnShare s = attn_share<Cfg::kWarps>(p);
-  __syncwarp();
-
+  AttnWalk walk;
+  if (!walk.start(p)) return;
   AttnCopyLoader<4, DP> load;
-  load.at = s.at;
-  load.left = s.count;
-  if (s.count) load.look_up(p);
+  load.start(p, walk.cur);
   const uint32_t ring = smem_u32(mine);
-#pragma unroll
-  for (int i = 0; i < Cfg::kStages - 1; ++i) load.issue(p, ring + i * Tile::kStageBytes);
+  auto refill = [&](int to) {
+    if (walk.look_ahead(p, load.left)) load.start(p, walk.nxt);
+    load.issue(p, ring + to * Tile::kStageBytes);
+  };
+#pragma unroll 1
+  for (int i = 0; i < Cfg::kStages - 1; ++i) refill(i);
 
-  AttnCursor at = s.at;
+  AttnCursor at = walk.cur.at;
   bool begun = at.tile == at.r.t0, fresh = true;
   float m[H], l[H], o[H][E];
   int stage = 0;
-  for (int i = 0; i < s.count; ++i) {
+  for (int i = 0;;) {
     const int kv = at.kv, h0 = at.blk * p.block_heads, nh = min(p.block_heads, p.group - h0);
     if (fresh) {
       const T* q = (const T*)p.q + at.row * p.q_row + (kv * p.group + h0) * p.q_head;
@@ -737,8 +746,7 @@ __global__ void __launch_bounds__(AttnSimtCfg<DP>::kWarps * 32, 1) attn_simt_ker
     cp_async_wait<Cfg::kStages - 2>();
     __syncwarp();
     // the stage read in the last round is free again
-    const int ahead = stage == 0 ? Cfg::kStages - 1 : stage - 1;
-    load.issue(p, ring + ahead * Tile::kStageBytes);
+    refill(stage == 0 ? Cfg::kStages - 1 : stage - 1);
 
     const unsigned char* ks = mine + stage * Tile::kStageBytes;
     const int tok = lane & 15, half = lane >> 4;
@@ -795,32 +803,35 @@ __global__ void __launch_bounds__(AttnSimtCfg<DP>::kWarps * 32, 1) attn_simt_ker
     }
     stage = stage + 1 == Cfg::kStages ? 0 : stage + 1;
 
-    const bool done = at.tile + 1 == at.r.t1;
-    if (done || i + 1 == s.count) {
-      __syncwarp();  // the ring may take the sums
-      const AttnPlace to = attn_place<Cfg::kWarps, H, DP>(p, s, board, reinterpret_cast<float*>(mine), at, i, begun, done);
+    const bool done = at.tile + 1 == at.r.t1, end = i + 1 == walk.cur.count;
+    if (done || end) {
+      const AttnPlace to = attn_place(p, walk.list, walk.cur, at, i, begun, done);
 #pragma unroll
       for (int h = 0; h < H; ++h) {
 #pragma unroll
         for (int d = 16; d; d >>= 1) l[h] += __shfl_xor_sync(0xffffffffu, l[h], d);
         if (h >= nh) continue;
-        const float f = l[h] > 0.f ? 1.f / l[h] : (l[h] == 0.f ? 0.f : l[h]);  // NaN stays
-        if (!to.whole && lane == 0) board.ml[warp][to.slot][h] = make_float2(m[h], l[h]);
+        const float f = to.whole ? (l[h] > 0.f ? 1.f / l[h] : (l[h] == 0.f ? 0.f : l[h])) : 1.f;  // NaN stays
+        if (!to.whole && lane == 0) p.part_ml[to.part + h] = make_float2(m[h], l[h]);
         float* out = to.whole ? (float*)p.out + (((int64_t)at.row * p.c.kv_heads + kv) * p.group + h0 + h) * p.c.dim
-                              : to.sums + h * to.pitch;
+                              : p.part_o + (to.part + h) * p.c.dim;
 #pragma unroll
         for (int e = 0; e < E; e += 2) {
           const int d = e * 32 + 2 * lane;
-          if (d < p.c.dim) *reinterpret_cast<float2*>(out + d) = to.whole ? make_float2(o[h][e] * f, o[h][e + 1] * f)
-                                                                          : make_float2(o[h][e], o[h][e + 1]);
+          if (d < p.c.dim) *reinterpret_cast<float2*>(out + d) = make_float2(o[h][e] * f, o[h][e + 1] * f);
         }
       }
       begun = true, fresh = true;
     }
-    at.next(p);
     __syncwarp();
+    if (end) {
+      if (!walk.step()) return;
+      at = walk.cur.at, i = 0;
+      begun = at.tile == at.r.t0;
+    } else {
+      at.next(p), ++i;
+    }
   }
-  attn_merge<float, Cfg::kWarps, H, DP>(p, board, attn_smem, Cfg::kWarpBytes);
 }
 
 template <int DP, int NT>
@@ -856,10 +867,8 @@ __global__ void __launch_bounds__(AttnMmaCfg<DP, NT>::kWarps * 32, 1)
   extern __shared__ __align__(128) unsigned char attn_smem[];
   __shared__ uint64_t bars[TMA ? Cfg::kWarps * STAGES : 1];
   __shared__ int abort_flag;
-  __shared__ AttnBoard<Cfg::kWarps, Cfg::kHeads> board;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  unsigned char* rings = attn_smem + ((1024 - (smem_u32(attn_smem) & 1023)) & 1023);
-  unsigned char* mine = rings + warp * Cfg::kWarpBytes;
+  unsigned char* mine = attn_smem + ((1024 - (smem_u32(attn_smem) & 1023)) & 1023) + warp * Cfg::kWarpBytes;
   const uint32_t ring = smem_u32(mine), sq = ring + STAGES * Tile::kStageBytes;
   uint64_t* bar = bars + (TMA ? warp * STAGES : 0);
   if constexpr (TMA) {
@@ -873,27 +882,27 @@ __global__ void __launch_bounds__(AttnMmaCfg<DP, NT>::kWarps * 32, 1)
   } else if (p.c.dim < DP) {  // columns that no copy fills
     for (int i = lane; i < STAGES * Tile::kStageBytes / 16; i += 32) reinterpret_cast<uint4*>(mine)[i] = make_uint4(0, 0, 0, 0);
   }
-  if (lane < 2) board.item[warp][lane].w = 0;
+  if constexpr (TMA) __syncthreads();  // abort_flag
+  __syncwarp();
   griddep_wait();
   griddep_launch();
-  const AttnShare s = attn_share<Cfg::kWarps>(p);
-  __syncwarp();
+  AttnWalk walk;
+  if (!walk.start(p)) return;
 
-  AttnCopyLoader<2, DP> copy;
-  AttnTmaLoader<DP> tma;
-  if constexpr (TMA) {
-    tma.at = s.at, tma.left = s.count;
-    if (lane == 0 && s.count) {
-      tma.look_up(p);
-#pragma unroll
-      for (int i = 0; i < STAGES - 1; ++i) tma.issue(p, &mk, &mv, ring + i * Tile::kStageBytes, bar + i);
+  std::conditional_t<TMA, AttnTmaLoader<DP>, AttnCopyLoader<2, DP>> load;
+  load.start(p, walk.cur);
+  int flying = 0;  // TMA: tiles whose copies have not been waited for
+  auto refill = [&](int to) {
+    if (walk.look_ahead(p, load.left)) load.start(p, walk.nxt);
+    if constexpr (TMA) {
+      flying += load.left > 0;
+      load.issue(p, &mk, &mv, ring + to * Tile::kStageBytes, bar + to);
+    } else {
+      load.issue(p, ring + to * Tile::kStageBytes);
     }
-  } else {
-    copy.at = s.at, copy.left = s.count;
-    if (s.count) copy.look_up(p);
-#pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i) copy.issue(p, ring + i * Tile::kStageBytes);
-  }
+  };
+#pragma unroll 1
+  for (int i = 0; i < STAGES - 1; ++i) refill(i);
 
   // ldmatrix rows of this lane: keys (token l & 15, chunk 2 ks + l / 16), values
   // transposed (token (l & 7) + 8 (l / 16), chunk 2 mt + (l / 8) % 2); four chunk
@@ -905,13 +914,13 @@ __global__ void __launch_bounds__(AttnMmaCfg<DP, NT>::kWarps * 32, 1)
     koff[j] = Tile::offset(krow, 2 * j + (lane >> 4));
     voff[j] = Tile::kTileBytes + Tile::offset(vrow, 2 * j + ((lane >> 3) & 1));
   }
-  AttnCursor at = s.at;
+  AttnCursor at = walk.cur.at;
   bool begun = at.tile == at.r.t0, fresh = true;
   uint32_t qf[Cfg::kQShared ? 1 : NT][Cfg::kQShared ? 1 : KS][2];
   float m[NT][2], l[NT][2], o[NT][KS][4];
   int stage = 0;
   uint32_t parity = 0;
-  for (int i = 0; i < s.count; ++i) {
+  for (int i = 0;;) {
     if (fresh) {
       const int h0 = at.blk * p.block_heads, nh = min(p.block_heads, p.group - h0);
       const T* q = (const T*)p.q + at.row * p.q_row + (at.kv * p.group + h0) * p.q_head;
@@ -945,22 +954,21 @@ __global__ void __launch_bounds__(AttnMmaCfg<DP, NT>::kWarps * 32, 1)
       }
       fresh = false;
     }
-    const int ahead = stage == 0 ? STAGES - 1 : stage - 1;  // read in the last round: free again
     if constexpr (TMA) {
-      if (lane == 0) tma.issue(p, &mk, &mv, ring + ahead * Tile::kStageBytes, bar + ahead);
+      refill(stage == 0 ? STAGES - 1 : stage - 1);  // read in the last round: free again
       if (!mbar_wait_warp(bar + stage, parity, &abort_flag)) {
-        // let this warp's copies land before the CTA's memory goes
-        const int flying = min(STAGES, s.count - i);
-        for (int j = 0; j < flying; ++j) {
+        // the status is raised; let this warp's copies land before the CTA's memory goes
+        for (; flying > 0; --flying) {
           mbar_drain(bar + stage, parity);
           if (++stage == STAGES) stage = 0, parity ^= 1;
         }
-        break;  // to the CTA's barrier, with the status raised
+        return;
       }
+      --flying;
     } else {
       cp_async_wait<STAGES - 2>();
       __syncwarp();
-      copy.issue(p, ring + ahead * Tile::kStageBytes);
+      refill(stage == 0 ? STAGES - 1 : stage - 1);
     }
     const uint32_t base = ring + stage * Tile::kStageBytes;
     const bool inner = at.tile * kAttnTile >= at.r.lo && (at.tile + 1) * kAttnTile <= at.r.n;
@@ -1052,11 +1060,9 @@ __global__ void __launch_bounds__(AttnMmaCfg<DP, NT>::kWarps * 32, 1)
     }
     if (++stage == STAGES) stage = 0, parity ^= 1;
 
-    const bool done = at.tile + 1 == at.r.t1;
-    if (done || i + 1 == s.count) {
-      __syncwarp();  // the ring may take the sums
-      const AttnPlace to = attn_place<Cfg::kWarps, Cfg::kHeads, DP>(p, s, board, reinterpret_cast<float*>(mine), at, i,
-                                                                    begun, done);
+    const bool done = at.tile + 1 == at.r.t1, end = i + 1 == walk.cur.count;
+    if (done || end) {
+      const AttnPlace to = attn_place(p, walk.list, walk.cur, at, i, begun, done);
       const int h0 = at.blk * p.block_heads, nh = min(p.block_heads, p.group - h0);
       const int64_t head0 = ((int64_t)at.row * p.c.kv_heads + at.kv) * p.group + h0;
 #pragma unroll
@@ -1070,9 +1076,9 @@ __global__ void __launch_bounds__(AttnMmaCfg<DP, NT>::kWarps * 32, 1)
           const int h = nt * 8 + (lane & 3) * 2 + j;
           if (h >= nh) continue;
           const float f = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);  // NaN stays
-          if (!to.whole && lane < 4) board.ml[warp][to.slot][h] = make_float2(m[nt][j], sum);
+          if (!to.whole && lane < 4) p.part_ml[to.part + h] = make_float2(m[nt][j], sum);
           T* out = (T*)p.out + (head0 + h) * p.c.dim;
-          float* part = to.sums + h * to.pitch;
+          float* part = p.part_o + (to.part + h) * p.c.dim;
 #pragma unroll
           for (int mt = 0; mt < KS; ++mt)
 #pragma unroll
@@ -1088,51 +1094,127 @@ __global__ void __launch_bounds__(AttnMmaCfg<DP, NT>::kWarps * 32, 1)
       }
       begun = true, fresh = true;
     }
-    at.next(p);
     __syncwarp();
+    if (end) {
+      if (!walk.step()) return;
+      at = walk.cur.at, i = 0;
+      begun = at.tile == at.r.t0;
+    } else {
+      at.next(p), ++i;
+    }
   }
-  attn_merge<T, Cfg::kWarps, Cfg::kHeads, DP>(p, board, rings, Cfg::kWarpBytes);
 }
 
-// Joins the parts of the items that several CTAs share.  CTA (c, y): heads y,
-// y + gridDim.y, ... of the item that begins in CTA c of the attention grid and
-// goes on in the next ones, if there is one; its warps take the parts in turn.
-constexpr int kJoinWarps = 8;
+// Joins the parts of the items that segments cut.  A warp takes a head of an item
+// of up to 32 parts, a CTA one of more, its warps a run of them each; a lane
+// holds a part's maximum and sum, then four (of 128) elements of the head.
+constexpr int kJoinWarps = 8, kJoinGrid = 4 * 148;
+
+struct AttnSum {
+  float m, l, o[8];
+  __device__ __forceinline__ void clear() {
+    m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = 0.f;
+  }
+  // Parts [i0, i1) of item `c`, head h; UPPER: of more than 128 elements.  Warp-collective.
+  template <bool UPPER>
+  __device__ __forceinline__ void add(const AttnParams& p, const int4& c, int h, int i0, int i1) {
+    const int lane = threadIdx.x & 31, dim = p.c.dim;
+    const int lo = min(lane * 4, dim - 4), hi = min(128 + lane * 4, dim - 4);  // lanes past dim repeat its last four
+    for (int first = i0; first < i1; first += 32) {
+      const int n = min(32, i1 - first), i = first + lane;
+      float2 ml = make_float2(-INFINITY, 0.f);
+      if (lane < n) ml = p.part_ml[((c.z + i) * 2ll + (i == 0 ? 1 : 0)) * p.block_heads + h];
+      float top = ml.x;
+#pragma unroll
+      for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+      top = fmaxf(top, m);
+      const float base = top == -INFINITY ? 0.f : top;
+      const float keep = exp2_fast(m - base), f = exp2_fast(ml.x - base);
+      float sum = ml.y * f;
+#pragma unroll
+      for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      m = top, l = l * keep + sum;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] *= keep;
+      // eight parts' loads at a time, none behind a branch: a load from the L2 takes
+      // longer than all the arithmetic
+      for (int j0 = 0; j0 < n; j0 += 8) {
+        float4 lower[8], upper[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int at = first + min(j0 + j, n - 1);
+          const float* from = p.part_o + (((c.z + at) * 2ll + (at == 0 ? 1 : 0)) * p.block_heads + h) * dim;
+          lower[j] = *reinterpret_cast<const float4*>(from + lo);
+          if (UPPER) upper[j] = *reinterpret_cast<const float4*>(from + hi);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float g = __shfl_sync(0xffffffffu, f, j0 + j);
+          if (j0 + j >= n) continue;
+          o[0] += lower[j].x * g, o[1] += lower[j].y * g, o[2] += lower[j].z * g, o[3] += lower[j].w * g;
+          if (UPPER) o[4] += upper[j].x * g, o[5] += upper[j].y * g, o[6] += upper[j].z * g, o[7] += upper[j].w * g;
+        }
+      }
+    }
+  }
+};
+
 template <typename T>
+__device__ __forceinline__ void join_put(const AttnParams& p, const int4& c, int h, int e, float l, const float* o) {
+  const float f = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // NaN stays
+  const int kv = c.y / p.blocks, h0 = (c.y - kv * p.blocks) * p.block_heads;
+  T* out = (T*)p.out + (((int64_t)c.x * p.c.kv_heads + kv) * p.group + h0 + h) * p.c.dim + e;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) out[j] = Chunk<T>::put(o[j] * f);
+}
+
+template <typename T, bool UPPER>
 __global__ void __launch_bounds__(kJoinWarps * 32) attn_join_kernel(const AttnParams p) {
-  __shared__ float4 s_o[kJoinWarps][64];
+  __shared__ float s_o[kJoinWarps][256];
   __shared__ float2 s_ml[kJoinWarps];
   griddep_wait();
   griddep_launch();
-  const int4 item = p.desc[blockIdx.x];
-  if (item.w == 0) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, dim = p.c.dim;
-  const int h0 = item.z * p.block_heads, nh = min(p.block_heads, p.group - h0);
-  for (int h = blockIdx.y; h < nh; h += gridDim.y) {
-    AttnSum a, b;  // elements 4 lane .. and 128 + 4 lane ..
-    a.clear(), b.clear();
-#pragma unroll 2
-    for (int i = warp; i < item.w; i += kJoinWarps) {
-      const int64_t part = ((blockIdx.x + i) * 2ll + (i == 0 ? 1 : 0)) * p.block_heads + h;
-      const float2 ml = p.cta_ml[part];
-      const float* o = p.cta_o + part * dim;
-      a.add(ml.x, ml.y, lane * 4 < dim ? *reinterpret_cast<const float4*>(o + lane * 4) : make_float4(0, 0, 0, 0));
-      if (dim > 128)
-        b.add(ml.x, ml.y, 128 + lane * 4 < dim ? *reinterpret_cast<const float4*>(o + 128 + lane * 4) : make_float4(0, 0, 0, 0));
-    }
+  const int near = p.work->cuts[0], far = p.work->cuts[1];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, dim = p.c.dim, bh = p.block_heads;
+  auto heads_of = [&](const int4& c) { return min(bh, p.group - c.y % p.blocks * bh); };
+  AttnSum a;
+  for (int t = blockIdx.x; t < far * bh; t += gridDim.x) {
+    const int4 c = p.cut[p.cut_room - 1 - t / bh];
+    const int h = t % bh;
+    if (h >= heads_of(c)) continue;
+    a.clear();
+    a.add<UPPER>(p, c, h, c.w * warp / kJoinWarps, c.w * (warp + 1) / kJoinWarps);
     __syncthreads();  // the head before has been read
-    s_o[warp][lane] = make_float4(a.o[0], a.o[1], a.o[2], a.o[3]);
-    if (dim > 128) s_o[warp][32 + lane] = make_float4(b.o[0], b.o[1], b.o[2], b.o[3]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s_o[warp][lane * 4 + e] = a.o[e], s_o[warp][128 + lane * 4 + e] = a.o[4 + e];
     if (lane == 0) s_ml[warp] = make_float2(a.m, a.l);
     __syncthreads();
-    const int e = threadIdx.x;  // four elements
-    if (e * 4 < dim) {
-      AttnSum sum;
-      sum.clear();
+    const int e = threadIdx.x * 4;
+    if (e < dim) {
+      float top = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int w = 0; w < kJoinWarps; ++w) sum.add(s_ml[w].x, s_ml[w].y, s_o[w][e]);
-      sum.put((T*)p.out + (((int64_t)item.x * p.c.kv_heads + item.y) * p.group + h0 + h) * dim + e * 4);
+      for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, s_ml[w].x);
+      const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+      for (int w = 0; w < kJoinWarps; ++w) {
+        const float f = exp2_fast(s_ml[w].x - base);
+        l += s_ml[w].y * f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] += s_o[w][e + j] * f;
+      }
+      join_put<T>(p, c, h, e, l, o);
     }
+  }
+  for (int t = warp * gridDim.x + blockIdx.x; t < near * bh; t += gridDim.x * kJoinWarps) {
+    const int4 c = p.cut[t / bh];
+    const int h = t % bh;
+    if (h >= heads_of(c)) continue;
+    a.clear();
+    a.add<UPPER>(p, c, h, 0, c.w);
+    if (lane * 4 < dim) join_put<T>(p, c, h, lane * 4, a.l, a.o);
+    if (128 + lane * 4 < dim) join_put<T>(p, c, h, 128 + lane * 4, a.l, a.o + 4);
   }
 }
 

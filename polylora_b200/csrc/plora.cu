@@ -166,7 +166,7 @@ int device_info(DeviceInfo** out) {
     SET_GRID(attn_simt_kernel<64>, AttnSimtCfg<64>::kSmemBytes)
     SET_GRID(attn_simt_kernel<128>, AttnSimtCfg<128>::kSmemBytes)
     SET_GRID(attn_simt_kernel<256>, AttnSimtCfg<256>::kSmemBytes)
-    constexpr int kRulesSmem = kRulesChunk * 6 + kRulesMaxBiases * 5;
+    constexpr int kRulesSmem = rules_smem_bytes(kRulesStep, kRulesStep, kRulesMaxBiases);
 #define SET_RULES(T)                                     \
   SET_GRID((logit_rules_kernel<T, int32_t>), kRulesSmem) \
   SET_GRID((logit_rules_kernel<T, int64_t>), kRulesSmem)
@@ -659,10 +659,10 @@ constexpr int64_t kPagedMaxRows = 1 << 20;
 // eights for the tensor cores, 0: CUDA cores) and warps of a CTA.  Blocks are as
 // large as registers allow, for a second block reads the cache again.
 struct AttnPlan {
-  int dp, eights, blocks, block_heads, warps;
-  size_t cta_offset, ml_offset, desc_offset, bytes;
+  int dp, eights, blocks, block_heads, warps, segments;
+  size_t before_offset, cut_offset, ml_offset, part_offset, bytes;
 };
-AttnPlan attn_plan(int32_t heads, int32_t kv_heads, int32_t dim, int dtype) {
+AttnPlan attn_plan(int64_t rows, int32_t heads, int32_t kv_heads, int32_t dim, int dtype) {
   AttnPlan a;
   const int group = heads / kv_heads;
   a.dp = dim <= 64 ? 64 : (dim <= 128 ? 128 : 256);
@@ -682,11 +682,14 @@ AttnPlan attn_plan(int32_t heads, int32_t kv_heads, int32_t dim, int dtype) {
     PLORA_WARPS(256, 1) PLORA_WARPS(256, 2)
 #undef PLORA_WARPS
   }
-  const size_t parts = (size_t)kAttnGrid * 2 * a.block_heads;
-  a.cta_offset = align256((size_t)kAttnGrid * a.warps * a.block_heads * dim * 4);
-  a.ml_offset = a.cta_offset + align256(parts * dim * 4);
-  a.desc_offset = a.ml_offset + align256(parts * 8);
-  a.bytes = a.desc_offset + align256((size_t)kAttnGrid * 16);
+  const size_t segments = (size_t)kAttnGrid * a.warps + attn_asked_max(kAttnGrid * a.warps, a.block_heads);
+  const size_t parts = segments * 2 * a.block_heads;
+  a.before_offset = 256;
+  a.segments = (int)segments;
+  a.cut_offset = a.before_offset + align256((size_t)rows * 8);
+  a.ml_offset = a.cut_offset + align256(segments * 16);
+  a.part_offset = a.ml_offset + align256(parts * 8);
+  a.bytes = a.part_offset + align256(parts * dim * 4);
   return a;
 }
 
@@ -762,7 +765,9 @@ bool attn_by_tma(const PagedView& c, const AttnPlan& a) {
 
 cudaError_t launch_attn(const AttnParams& p, const AttnPlan& a, int dtype, bool tma, const CUtensorMap& mk,
                         const CUtensorMap& mv, cudaStream_t s) {
-  cudaError_t e = cudaErrorInvalidValue;
+  cudaError_t e = launch_kernel(attn_plan_kernel, dim3(1), dim3(kAttnPlanThreads), 0, s, true, 0, p, kAttnGrid * a.warps);
+  if (e != cudaSuccess) return e;
+  e = cudaErrorInvalidValue;
 #define PLORA_SIMT(DP)                                                                                          \
   if (a.eights == 0 && a.dp == DP)                                                                              \
     e = launch_kernel(attn_simt_kernel<DP>, dim3(kAttnGrid), dim3(a.warps * 32), AttnSimtCfg<DP>::kSmemBytes, s, \
@@ -781,15 +786,19 @@ cudaError_t launch_attn(const AttnParams& p, const AttnPlan& a, int dtype, bool 
 #undef PLORA_MMA
 #undef PLORA_SIMT
   if (e != cudaSuccess) return e;
-  const dim3 grid(kAttnGrid, (unsigned)std::min(a.block_heads, 4)), block(kJoinWarps * 32);
-  return dtype == PLORA_DTYPE_F32   ? launch_kernel(attn_join_kernel<float>, grid, block, 0, s, true, 0, p)
-         : dtype == PLORA_DTYPE_F16 ? launch_kernel(attn_join_kernel<__half>, grid, block, 0, s, true, 0, p)
-                                    : launch_kernel(attn_join_kernel<__nv_bfloat16>, grid, block, 0, s, true, 0, p);
+  const dim3 grid(kJoinGrid), block(kJoinWarps * 32);
+#define PLORA_JOIN(T)                                                                             \
+  (a.dp == 256 ? launch_kernel(attn_join_kernel<T, true>, grid, block, 0, s, true, 0, p)          \
+               : launch_kernel(attn_join_kernel<T, false>, grid, block, 0, s, true, 0, p))
+  return dtype == PLORA_DTYPE_F32   ? PLORA_JOIN(float)
+         : dtype == PLORA_DTYPE_F16 ? PLORA_JOIN(__half)
+                                    : PLORA_JOIN(__nv_bfloat16);
+#undef PLORA_JOIN
 }
 
 template <typename T>
 cudaError_t launch_rules(const RulesParams& p, bool wide, int64_t rows, size_t smem, cudaStream_t s) {
-  const dim3 grid((unsigned)((p.vocab + kRulesChunk - 1) / kRulesChunk), (unsigned)rows);
+  const dim3 grid((unsigned)((p.vocab + p.chunk - 1) / p.chunk), (unsigned)rows);
   return wide ? launch_kernel(logit_rules_kernel<T, int64_t>, grid, dim3(kRulesThreads), smem, s, true, 0, p)
               : launch_kernel(logit_rules_kernel<T, int32_t>, grid, dim3(kRulesThreads), smem, s, true, 0, p);
 }
@@ -1148,11 +1157,11 @@ int plora_paged_append(const void* q, int64_t q_row_stride, int64_t q_token_stri
   return PLORA_OK;
 }
 
-size_t plora_paged_attention_workspace(int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t dtype) {
-  if (!valid_dtype(dtype) || kv_heads < 1 || heads < 1 || heads % kv_heads || heads > 65535 || head_dim < 1 ||
+size_t plora_paged_attention_workspace(int64_t rows, int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t dtype) {
+  if (!valid_dtype(dtype) || rows < 0 || rows > kPagedMaxRows || kv_heads < 1 || heads < 1 || heads % kv_heads || heads > 65535 || head_dim < 1 ||
       head_dim > 256 || head_dim % 8)
     return 0;
-  return attn_plan(heads, kv_heads, head_dim, dtype).bytes;
+  return attn_plan(rows, heads, kv_heads, head_dim, dtype).bytes;
 }
 
 int plora_paged_attention(const void* q, int64_t q_row_stride, int64_t q_head_stride, const void* k_cache,
@@ -1174,7 +1183,7 @@ int plora_paged_attention(const void* q, int64_t q_row_stride, int64_t q_head_st
   if (q_row_stride < 0 || q_head_stride < 0 || q_row_stride * elem % 16 || q_head_stride * elem % 16 ||
       !aligned16(q) || !aligned16(out))
     return fail(PLORA_ERR_INVALID_ARGUMENT, "q and out must be 16-byte aligned, with q's strides multiples of 16 bytes");
-  const AttnPlan a = attn_plan(heads, kv_heads, head_dim, dtype);
+  const AttnPlan a = attn_plan(rows, heads, kv_heads, head_dim, dtype);
   if (!workspace || workspace_size < a.bytes)
     return fail(PLORA_ERR_WORKSPACE, "attention workspace %zu < %zu bytes", workspace_size, a.bytes);
   if (reinterpret_cast<uintptr_t>(workspace) % 256)
@@ -1187,10 +1196,12 @@ int plora_paged_attention(const void* q, int64_t q_row_stride, int64_t q_head_st
   p.window = (int32_t)std::min<int64_t>(window, INT32_MAX);
   p.scale_log2 = scale * 1.4426950408889634f;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  p.warp_o = reinterpret_cast<float*>(ws);
-  p.cta_o = reinterpret_cast<float*>(ws + a.cta_offset);
-  p.cta_ml = reinterpret_cast<float2*>(ws + a.ml_offset);
-  p.desc = reinterpret_cast<int4*>(ws + a.desc_offset);
+  p.work = reinterpret_cast<AttnWork*>(ws);
+  p.before = reinterpret_cast<int64_t*>(ws + a.before_offset);
+  p.cut = reinterpret_cast<int4*>(ws + a.cut_offset);
+  p.cut_room = a.segments;
+  p.part_ml = reinterpret_cast<float2*>(ws + a.ml_offset);
+  p.part_o = reinterpret_cast<float*>(ws + a.part_offset);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   CUtensorMap mk = {}, mv = {};
   const bool tma = attn_by_tma(p.c, a);
@@ -1237,7 +1248,15 @@ int plora_logit_rules(const void* logits, int64_t logits_stride, void* out, int6
   p.bias_tokens = bias_tokens, p.bias_row = bias_tokens_stride;
   p.bias_values = bias_values, p.value_row = bias_values_stride, p.biases = (int32_t)biases;
   p.allowed = reinterpret_cast<const uint32_t*>(allowed), p.mask_row = allowed_stride;
-  const size_t smem = history || biases ? (size_t)kRulesChunk * 6 + (size_t)biases * 5 : 0;
+  // the largest chunk that still makes eight CTAs for each SM, four of which its
+  // tables leave room for: a row's history is read once per chunk
+  p.chunk = kRulesStep;
+  const int64_t entries = history + biases;
+  for (int chunk = 2 * kRulesStep; chunk <= kRulesMaxChunk; chunk += kRulesStep)
+    if (rows * ((vocab + chunk - 1) / chunk) >= 8 * di->sm_count &&
+        rules_smem_bytes(chunk, entries, (int)biases) <= 48 * 1024)
+      p.chunk = chunk;
+  const size_t smem = entries ? (size_t)rules_smem_bytes(p.chunk, entries, (int)biases) : 0;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool wide = token_bytes == 8;
   cudaError_t e = dtype == PLORA_DTYPE_F32   ? launch_rules<float>(p, wide, rows, smem, s)

@@ -199,7 +199,7 @@ def paged_attention(
         raise ValueError("out must be a contiguous tensor of q's shape, dtype and device")
     qc, qs = _heads(q)
     code = dtype_code(q.dtype)
-    ws_bytes = _native.load().plora_paged_attention_workspace(heads, kv_heads, dim, code)
+    ws_bytes = _native.load().plora_paged_attention_workspace(rows, heads, kv_heads, dim, code)
     ws = lens.new_empty(max(ws_bytes, 256) // 4)
     _call(
         dev, "plora_paged_attention",

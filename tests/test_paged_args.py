@@ -67,12 +67,12 @@ def test_attention_arguments_rejected_before_cuda(native):
     for kw in (dict(heads=0), dict(window=-1), dict(q=None), dict(lens=None), dict(out=None), dict(out=D + 8),
                dict(qs=(1024, 4)), dict(ws=D + 16)):
         assert _attend(lib, native, **kw) == native.ERR_INVALID_ARGUMENT, kw
-    need = lib.plora_paged_attention_workspace(16, 4, 64, native.DTYPE_BF16)
+    need = lib.plora_paged_attention_workspace(2, 16, 4, 64, native.DTYPE_BF16)
     assert need > 0
     assert _attend(lib, native, wb=need - 1) == native.ERR_WORKSPACE
     assert _attend(lib, native, ws=None) == native.ERR_WORKSPACE
     assert _attend(lib, native, rows=0) == native.OK
-    for bad in ((16, 5, 64, 2), (0, 4, 64, 2), (16, 4, 65, 2), (16, 4, 512, 2), (16, 4, 64, 7)):
+    for bad in ((2, 16, 5, 64, 2), (2, 0, 4, 64, 2), (2, 16, 4, 65, 2), (2, 16, 4, 512, 2), (2, 16, 4, 64, 7), (-1, 16, 4, 64, 2)):
         assert lib.plora_paged_attention_workspace(*bad) == 0
 
 
