@@ -377,14 +377,21 @@ int plora_paged_attention(const void* q, int64_t q_row_stride, int64_t q_head_st
  *   -infinity                                      where bit t % 32 of
  *       allowed[b, t / 32] is 0 (null: all are allowed).
  * Null repetition / presence / frequency mean 1 / 0 / 0.  Token ids are
- * int32 or int64 (token_bytes 4 or 8); ids outside [0, vocab) are skipped. */
+ * int32 or int64 (token_bytes 4 or 8); ids outside [0, vocab) are skipped.  At
+ * most 65535 rows and 4096 biases a row.  The workspace
+ * (plora_logit_rules_workspace bytes, 256-byte aligned; 0 for few rows and for
+ * arguments the call rejects; not used in place without a mask) needs no
+ * initialisation; calls that may overlap
+ * need one each. */
+size_t plora_logit_rules_workspace(int64_t rows, int64_t vocab, int64_t history, int64_t biases);
+
 int plora_logit_rules(const void* logits, int64_t logits_stride, void* out, int64_t out_stride, int64_t rows,
                       int64_t vocab, int32_t dtype, const void* tokens, int64_t tokens_stride, int64_t history,
                       const int32_t* token_lens, const int32_t* prompt_lens, const float* repetition,
                       const float* presence, const float* frequency, const void* bias_tokens,
                       int64_t bias_tokens_stride, const float* bias_values, int64_t bias_values_stride,
                       int64_t biases, const int32_t* allowed, int64_t allowed_stride, int32_t token_bytes,
-                      void* stream);
+                      void* workspace, size_t workspace_size, void* stream);
 
 #ifdef __cplusplus
 }

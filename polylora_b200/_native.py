@@ -171,11 +171,13 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
             ctypes.c_float, _i64, _i64, _i32, _i32, _i32, _i32, _i64, _i64, _i32, _c_void_p, _size, _c_void_p,
         ],
     ),
+    "plora_logit_rules_workspace": (_size, [_i64, _i64, _i64, _i64]),
     "plora_logit_rules": (
         ctypes.c_int,
         [
             _c_void_p, _i64, _c_void_p, _i64, _i64, _i64, _i32, _c_void_p, _i64, _i64, _c_void_p, _c_void_p,
             _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p, _i64, _i64, _c_void_p, _i64, _i32, _c_void_p,
+            _size, _c_void_p,
         ],
     ),
     "plora_slot_fill": (
@@ -231,7 +233,9 @@ def check(func: str, status: int) -> None:
 
 def call(func: str, *args: object) -> None:
     """Calls a status-returning entry point and raises on failure."""
-    check(func, getattr(load(), func)(*args))
+    status = getattr(_lib or load(), func)(*args)
+    if status != OK:
+        check(func, status)
 
 
 def device_status(clear: bool = True) -> int:

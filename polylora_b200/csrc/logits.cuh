@@ -8,18 +8,22 @@
 //   x -> -infinity                     for tokens the mask does not allow
 //
 // in 32 bits, rounded once.  Bound by HBM (the logits read and written once).
+//
 // A token without a rule keeps its bits, or becomes -infinity, and few tokens have
-// one.  So half of a CTA's warps copy a chunk of a row's logits, 16 bytes a lane,
-// putting -infinity where the mask says so, while the other half works out the
-// chunk's rules; then all of them go over the tokens with rules.
+// one.  So logit_copy_kernel copies the logits, 16 bytes a lane, with -infinity
+// where the mask says so; logit_find_kernel finds the tokens with rules, which
+// leaves the memory idle; and the rules are applied to those tokens once the copy
+// is done.  The first two run side by side.  Rows few enough for all of their
+// finding CTAs to wait out the copy: the copy first, and a finding CTA applies its
+// own rules.  More rows: the finding first, which leaves lists, and
+// logit_apply_kernel after both.  (256 x 128256 bf16 logits: 47 us in one kernel
+// whose CTAs do all three.)
 //
 // The rules are found in two readings of the row's history.  The first sets a bit
-// for each of the chunk's tokens; the bits, counted, give the list of those tokens
-// and each one's place in it.  The second adds up a word of marks and a count at
-// that place, with integer atomics, so the order of threads does not matter.  A
-// bias belongs to the first entry of the list that names its token, which adds up
-// the others in their order.  With a bit per token and eight bytes per token that
-// has a rule a chunk can be large, and a row's history is read by few CTAs.
+// for each of its tokens; the bits, counted, give each token's place in the list of
+// those with a rule.  The second adds up a word of marks and a count at that place,
+// with integer atomics, so the order of threads does not matter.  Biases of one
+// token are added in the order of the list.
 #pragma once
 
 #include "paged.cuh"
@@ -27,25 +31,28 @@
 namespace plora {
 
 constexpr int kRulesThreads = 256;
-constexpr int kRulesHalf = kRulesThreads / 2;  // threads that copy, threads that find the rules
-constexpr int kRulesStep = 8192;               // vocabulary entries of a CTA: this many times 1, 2, 3 or 4
-constexpr int kRulesMaxChunk = 4 * kRulesStep;
-constexpr int kRulesMaxBiases = 4096;          // entries of a row's bias list
-constexpr int kRulesHeld = 16;                 // history entries that a thread keeps between its two readings
+constexpr int kRulesStrip = 128;        // 16-byte chunks that a copying warp takes at a time
+constexpr int kRulesBesideCtas = 148;  // finding CTAs that run beside the copy
+constexpr int kRulesMostPart = 1 << 18; // vocabulary entries of a CTA that finds rules
+constexpr int kRulesMostSmem = 100 * 1024;
+constexpr int kRulesMaxBiases = 4096;   // entries of a row's bias list
+constexpr int kRulesHeld = 8;           // history entries that a thread reads at once, and of the first keeps
 
-// Shared memory of a call with a history or biases: bits and the rank of each word
-// of them; for each token with a rule its marks, its place in the chunk and its
-// entry of the bias list; the bias list and its sums.
-__host__ __device__ constexpr int rules_ruled(int chunk, int64_t entries) {
-  return ((entries < chunk ? (int)entries : chunk) + 3) & ~3;
+// Shared memory of a CTA that finds rules: bits of its part's tokens and the rank
+// of each word of them; for each token with a rule its marks, itself and the first
+// entry of the bias list that names it; the bias list and whether others name an
+// entry's token.
+__host__ __device__ constexpr int rules_words(int part) { return (part + 127) / 128 * 4; }
+__host__ __device__ constexpr int rules_ruled(int part, int64_t entries) {
+  return ((entries < part ? (int)entries : part) + 3) & ~3;
 }
-__host__ __device__ constexpr int rules_smem_bytes(int chunk, int64_t entries, int biases) {
-  return (chunk / 32 + 4) * 6 + rules_ruled(chunk, entries) * 8 + biases * 12;
+__host__ __device__ constexpr int rules_smem_bytes(int part, int64_t entries, int biases) {
+  return rules_words(part) * 8 + rules_ruled(part, entries) * 12 + ((biases + 3) & ~3) * 9;
 }
 
-constexpr uint32_t kRulesSeen = 0x80000000u;    // the token is in the history
-constexpr uint32_t kRulesBiased = 0x40000000u;  // the token has a bias
-constexpr uint32_t kRulesCount = 0x3fffffffu;   // times in the answer
+constexpr uint32_t kRulesSeen = 0x80000000u;   // the token is in the history
+constexpr uint32_t kRulesCount = 0x7fffffffu;  // times in the answer
+constexpr uint32_t kRulesNone = 0xffffffffu;   // no entry of the bias list
 
 struct RulesParams {
   const void* x;
@@ -57,7 +64,18 @@ struct RulesParams {
   const int32_t *token_lens, *prompt_lens;  // null: the whole list; 0
   const float *repetition, *presence, *frequency, *bias_values;
   const uint32_t* allowed;
-  int32_t history, biases, chunk;
+  int32_t history, biases;
+  int32_t part;        // vocabulary entries of a CTA that finds rules
+  bool beside;         // the finding is launched after the copy, and beside it
+  // lists (null: a finding CTA applies its rules): entries of each (row, part) and how many
+  struct RulesEntry* list;
+  int32_t* listed;
+};
+
+struct RulesEntry {
+  int32_t token;  // offset in the part
+  uint32_t mark;
+  float bias;
 };
 
 // Bits i .. of a mask as the low bits of a word (a lane's chunk has at most 8).
@@ -85,164 +103,266 @@ __device__ __forceinline__ uint4 rules_masked(const uint4& u, uint32_t keep) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-template <typename T, typename I>
-__global__ void __launch_bounds__(kRulesThreads) logit_rules_kernel(const RulesParams p) {
-  constexpr int N = Chunk<T>::N, VECS = 8;  // 16-byte chunks that a copying thread has on their way
-  extern __shared__ __align__(16) unsigned char rules_smem[];
-  const int words = p.chunk / 32, ruled = rules_ruled(p.chunk, (int64_t)p.history + p.biases);
-  uint32_t* touched = reinterpret_cast<uint32_t*>(rules_smem);        // [words, four more]
-  uint32_t* mark = touched + words + 4;                               // [ruled]
-  int32_t* bias_at = reinterpret_cast<int32_t*>(mark + ruled);        // [biases]: place in the chunk, or -1
-  float* bias_v = reinterpret_cast<float*>(bias_at + p.biases);       // [biases]
-  float* bias_sum = bias_v + p.biases;                                // [biases]
-  uint16_t* rank = reinterpret_cast<uint16_t*>(bias_sum + p.biases);  // [words, four more]: bits set before the word
-  uint16_t* place_of = rank + words + 4;                              // [ruled]
-  uint16_t* bias_of = place_of + ruled;                               // [ruled]: a biased token's entry
-  __shared__ int s_warp[kRulesHalf / 32];
-  const int tid = threadIdx.x;
-  const int64_t row = blockIdx.y, c0 = (int64_t)blockIdx.x * p.chunk;
-  const int nc = (int)min((int64_t)p.chunk, p.vocab - c0);
-  const bool marks = p.history > 0 || p.biases > 0;
-  if (marks)
-    for (int i = tid; i < words + 4; i += kRulesThreads) touched[i] = 0;
-  __syncthreads();
-  griddep_wait();
-  griddep_launch();
-  const uint32_t* mask = p.allowed ? p.allowed + row * p.mask_row : nullptr;
-  const T* x = (const T*)p.x + row * p.x_row + c0;
-  T* y = (T*)p.y + row * p.y_row + c0;
-  float rep = 1.f, pres = 0.f, freq = 0.f;
-  if (p.repetition) rep = p.repetition[row];
-  if (p.presence) pres = p.presence[row];
-  if (p.frequency) freq = p.frequency[row];
+// One token's rules.
+struct RulesRow {
+  float rep, pres, freq;
+  __device__ __forceinline__ void read(const RulesParams& p, int64_t row) {
+    rep = p.repetition ? p.repetition[row] : 1.f;
+    pres = p.presence ? p.presence[row] : 0.f;
+    freq = p.frequency ? p.frequency[row] : 0.f;
+  }
+  __device__ __forceinline__ float apply(float v, uint32_t mark) const {
+    if (mark & kRulesSeen) v = v > 0.f ? v / rep : v * rep;
+    const uint32_t n = mark & kRulesCount;
+    return n ? v - freq * (float)n - pres : v;
+  }
+};
 
-  if (tid >= kRulesHalf) {
-    if (x != y || mask) {
-      const int th = tid - kRulesHalf;
-      // 16-byte chunks where x and y lie alike on them, single elements before and after
-      const int off = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
-      const bool alike = (reinterpret_cast<uintptr_t>(x) & 15) == (reinterpret_cast<uintptr_t>(y) & 15);
-      const int head = alike ? min(nc, off ? N - off : 0) : nc;
-      const int vecs = (nc - head) / N;
-      const bool even = head % N == 0;  // the mask bits of a 16-byte chunk lie in one word (c0 is a multiple of 32)
-      for (int j0 = th; j0 < vecs; j0 += VECS * kRulesHalf) {
-        uint4 u[VECS];
-        uint32_t w0[VECS], w1[VECS];
+// y = x with -infinity where the mask does not allow.  A warp takes a strip of a
+// row, from the row's first 16-byte boundary on, and a lane 16-byte chunks lane,
+// lane + 32, ... of it, all four of them on their way.
+template <typename T>
+__global__ void __launch_bounds__(kRulesThreads) logit_copy_kernel(const RulesParams p) {
+  constexpr int N = Chunk<T>::N, ROUNDS = kRulesStrip / 32;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, vocab = (int)p.vocab;
+  const int64_t row = blockIdx.y;
+  const int strip = blockIdx.x * (kRulesThreads / 32) + warp;
+  // After the finding kernel nothing need be waited for at first: it lets this one
+  // start when all of its CTAs have waited for what came before.
+  if (p.beside) griddep_wait();
+  griddep_launch();
+  const T* x = (const T*)p.x + row * p.x_row;
+  T* y = (T*)p.y + row * p.y_row;
+  const uint32_t* mask = p.allowed ? p.allowed + row * p.mask_row : nullptr;
+  const int off = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
+  const int head = min(vocab, off ? N - off : 0), first = head + strip * kRulesStrip * N;
+  auto one = [&](int i) { y[i] = mask && !(mask_bits(mask, i, 1) & 1) ? Chunk<T>::put(-INFINITY) : x[i]; };
+  if (first < vocab || strip == 0) {
+    if ((reinterpret_cast<uintptr_t>(x) & 15) == (reinterpret_cast<uintptr_t>(y) & 15)) {
+      const int chunks = (vocab - first) / N;  // of the row from here on
+      const uint4* from = reinterpret_cast<const uint4*>(x + first);
+      uint4* to = reinterpret_cast<uint4*>(y + first);
+      uint4 u[ROUNDS];
 #pragma unroll
-        for (int v = 0; v < VECS; ++v) {
-          const int i = head + min(j0 + v * kRulesHalf, vecs - 1) * N;
-          u[v] = *reinterpret_cast<const uint4*>(x + i);
-          w0[v] = w1[v] = ~0u;
-          if (mask) {
-            w0[v] = mask[(c0 + i) >> 5];
-            if (!even) w1[v] = mask[(c0 + i + N - 1) >> 5];
-          }
-        }
+      for (int v = 0; v < ROUNDS; ++v)
+        if (lane + v * 32 < chunks) u[v] = from[lane + v * 32];
+      if (mask) {
+        const int i0 = first + lane * N, shift = i0 & 31;  // of the chunk's mask bits in their word, in every round
+        const uint32_t* m = mask + (i0 >> 5);
+        uint32_t w[ROUNDS];
 #pragma unroll
-        for (int v = 0; v < VECS; ++v) {
-          const int j = j0 + v * kRulesHalf, i = head + j * N;
-          if (j < vecs) *reinterpret_cast<uint4*>(y + i) = rules_masked<T>(u[v], __funnelshift_r(w0[v], w1[v], i & 31));
-        }
-      }
-      auto one = [&](int i) { y[i] = mask && !(mask_bits(mask, c0 + i, 1) & 1) ? Chunk<T>::put(-INFINITY) : x[i]; };
-#pragma unroll 4
-      for (int i = th; i < head; i += kRulesHalf) one(i);
-      for (int i = head + vecs * N + th; i < nc; i += kRulesHalf) one(i);
-    }
-  } else if (marks) {
-    const I* tok = (const I*)p.tokens + row * p.token_row;
-    const I* bt = (const I*)p.bias_tokens + row * p.bias_row;
-    const float* bv = p.bias_values + row * p.value_row;
-    const int len = p.history > 0 ? min(p.token_lens ? p.token_lens[row] : p.history, p.history) : 0;
-    const int prompt = p.history > 0 && p.prompt_lens ? p.prompt_lens[row] : 0;
-    auto place = [&](int64_t id) {  // -1: not of this chunk
-      const int64_t t = id - c0;
-      return t >= 0 && t < nc ? (int)t : -1;
-    };
-    auto touch = [&](int t) {
-      if (t >= 0) atomicOr(touched + (t >> 5), 1u << (t & 31));
-    };
-    auto slot = [&](int t) { return rank[t >> 5] + __popc(touched[t >> 5] & ((1u << (t & 31)) - 1)); };
-    for (int j = tid; j < p.biases; j += kRulesHalf) {
-      const int t = place(bt[j]);
-      bias_at[j] = t;
-      bias_v[j] = bv[j];
-      touch(t);
-    }
-    int held[kRulesHeld];
+        for (int v = 0; v < ROUNDS; ++v) w[v] = lane + v * 32 < chunks ? m[v * N] : 0u;
 #pragma unroll
-    for (int k = 0; k < kRulesHeld; ++k) {
-      const int i = tid + k * kRulesHalf;
-      held[k] = i < len ? place(tok[i]) : -1;
-    }
-#pragma unroll
-    for (int k = 0; k < kRulesHeld; ++k) touch(held[k]);
-#pragma unroll 4
-    for (int i = tid + kRulesHeld * kRulesHalf; i < len; i += kRulesHalf) touch(place(tok[i]));
-    named_barrier(1, kRulesHalf);
-    {  // ranks: a thread takes neighbouring words
-      const int per = (words + kRulesHalf - 1) / kRulesHalf, first = min(tid * per, words), last = min(first + per, words);
-      int mine = 0;
-      for (int w = first; w < last; ++w) mine += __popc(touched[w]);
-      int before = mine;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, before, d);
-        if ((tid & 31) >= d) before += v;
-      }
-      if ((tid & 31) == 31) s_warp[tid >> 5] = before;
-      before -= mine;
-      named_barrier(1, kRulesHalf);
-      for (int w = 0; w < (tid >> 5); ++w) before += s_warp[w];
-      for (int w = first; w < last; ++w) {
-        rank[w] = (uint16_t)before;
-        for (uint32_t bits = touched[w]; bits; bits &= bits - 1, ++before) {
-          place_of[before] = (uint16_t)(w * 32 + __ffs(bits) - 1);
-          mark[before] = 0;
+        for (int v = 0; v < ROUNDS; ++v) {
+          uint32_t keep = w[v] >> shift;
+          if (shift + N > 32 && lane + v * 32 < chunks) keep |= m[v * N + 1] << (32 - shift);  // the rest is in the next word
+          u[v] = rules_masked<T>(u[v], keep);
         }
       }
-    }
-    named_barrier(1, kRulesHalf);
-    auto count = [&](int t, int i) {
-      if (t < 0) return;
-      uint32_t* w = mark + slot(t);
-      if (i >= prompt) atomicAdd(w, 1u);
-      atomicOr(w, kRulesSeen);
-    };
 #pragma unroll
-    for (int k = 0; k < kRulesHeld; ++k) count(held[k], tid + k * kRulesHalf);
-#pragma unroll 4
-    for (int i = tid + kRulesHeld * kRulesHalf; i < len; i += kRulesHalf) count(place(tok[i]), i);
-    for (int j = tid; j < p.biases; j += kRulesHalf) {
-      const int t = bias_at[j];
-      if (t < 0) continue;
-      bool owner = true;
-      for (int k = 0; k < j && owner; ++k) owner = bias_at[k] != t;
-      if (!owner) continue;
-      float v = bias_v[j];
-      for (int k = j + 1; k < p.biases; ++k)
-        if (bias_at[k] == t) v += bias_v[k];
-      bias_sum[j] = v;
-      const int r = slot(t);
-      bias_of[r] = (uint16_t)j;
-      atomicOr(mark + r, kRulesBiased);
+      for (int v = 0; v < ROUNDS; ++v)
+        if (lane + v * 32 < chunks) to[lane + v * 32] = u[v];
+      // single elements before the first chunk and after the last
+      if (strip == 0 && lane < head) one(lane);
+      const int tail = first + chunks * N;
+      if (chunks <= kRulesStrip && tail + lane < vocab) one(tail + lane);
+    } else {
+      const int last = min(first + kRulesStrip * N, vocab);
+#pragma unroll 8
+      for (int i = (strip == 0 ? 0 : first) + lane; i < last; i += 32) one(i);
     }
   }
-  if (!marks) return;
-  __syncthreads();
+  // this grid's end has to mean the finding kernel's end too, for the kernel that applies its lists
+  if (!p.beside && blockIdx.x + 1 == gridDim.x && blockIdx.y + 1 == gridDim.y) griddep_wait();
+}
 
-  const int total = s_warp[0] + s_warp[1] + s_warp[2] + s_warp[3];
-  static_assert(kRulesHalf == 128, "four warps' counts");
-#pragma unroll 4
-  for (int r = tid; r < total; r += kRulesThreads) {
-    const int i = place_of[r];
-    float v = Chunk<T>::get(x[i]);  // in place: still the logit, or -infinity behind the mask
-    const uint32_t w = mark[r];
-    if (w & kRulesSeen) v = v > 0.f ? v / rep : v * rep;
-    const uint32_t n = w & kRulesCount;
-    if (n) v = v - freq * (float)n - pres;
-    if (w & kRulesBiased) v += bias_sum[bias_of[r]];
-    if (!mask || (mask_bits(mask, c0 + i, 1) & 1)) y[i] = Chunk<T>::put(v);
+template <typename T, typename I>
+__global__ void __launch_bounds__(kRulesThreads) logit_find_kernel(const RulesParams p) {
+  extern __shared__ __align__(16) unsigned char rules_smem[];
+  const int words = rules_words(p.part), ruled = rules_ruled(p.part, (int64_t)p.history + p.biases);
+  const int entries = (p.biases + 3) & ~3;
+  uint32_t* touched = reinterpret_cast<uint32_t*>(rules_smem);    // [words]
+  uint32_t* rank = touched + words;                               // [words]: bits set before the word
+  uint32_t* mark = rank + words;                                  // [ruled]
+  int32_t* token_of = reinterpret_cast<int32_t*>(mark + ruled);   // [ruled]: offset in the part
+  uint32_t* bias_of = reinterpret_cast<uint32_t*>(token_of + ruled);  // [ruled]: first entry of the token
+  int32_t* bias_at = reinterpret_cast<int32_t*>(bias_of + ruled);     // [biases]: offset in the part, or -1
+  float* bias_v = reinterpret_cast<float*>(bias_at + entries);        // [biases]
+  uint8_t* twice = reinterpret_cast<uint8_t*>(bias_v + entries);      // [biases]: others name its token
+  __shared__ int s_warp[kRulesThreads / 32];
+  const int tid = threadIdx.x;
+  const int64_t row = blockIdx.y, c0 = (int64_t)blockIdx.x * p.part;
+  const int nc = (int)min((int64_t)p.part, p.vocab - c0);
+  for (int i = tid; i < words; i += kRulesThreads) touched[i] = 0;
+  for (int j = tid; j < entries; j += kRulesThreads) twice[j] = 0;
+  // Beside the copy everything but the logits may be read at once: it lets this
+  // kernel start when all of its CTAs have waited for what came before.
+  if (!p.beside) {
+    griddep_wait();
+    griddep_launch();
+  }
+  const I* tok = (const I*)p.tokens + row * p.token_row;
+  const I* bt = (const I*)p.bias_tokens + row * p.bias_row;
+  const float* bv = p.bias_values + row * p.value_row;
+  int len = 0, prompt = 0;
+  if (p.history > 0) {
+    len = min(p.token_lens ? p.token_lens[row] : p.history, p.history);
+    if (p.prompt_lens) prompt = p.prompt_lens[row];
+  }
+  I bias_id = -1;
+  float bias_value = 0.f;
+  if (tid < p.biases) bias_id = bt[tid], bias_value = bv[tid];
+
+  auto offset = [&](int64_t id) {  // in the part, -1: not of it
+    const int64_t t = id - c0;
+    return t >= 0 && t < nc ? (int)t : -1;
+  };
+  auto touch = [&](int at) {
+    if (at >= 0) atomicOr(touched + (at >> 5), 1u << (at & 31));
+  };
+  auto slot = [&](int at) { return rank[at >> 5] + __popc(touched[at >> 5] & ((1u << (at & 31)) - 1)); };
+  // kRulesHeld entries of a thread at a time, loaded before any is looked at
+  auto read = [&](int i0, int (&at)[kRulesHeld]) {
+    I id[kRulesHeld];
+#pragma unroll
+    for (int k = 0; k < kRulesHeld; ++k) id[k] = tok[min(i0 + k * kRulesThreads, len - 1)];
+#pragma unroll
+    for (int k = 0; k < kRulesHeld; ++k) at[k] = i0 + k * kRulesThreads < len ? offset(id[k]) : -1;
+  };
+  constexpr int kRound = kRulesHeld * kRulesThreads;
+  int held[kRulesHeld];  // the first round's, kept for the second reading
+#pragma unroll
+  for (int k = 0; k < kRulesHeld; ++k) held[k] = -1;
+  if (len > 0) read(tid, held);
+  __syncthreads();  // the bits are zero
+#pragma unroll
+  for (int k = 0; k < kRulesHeld; ++k) touch(held[k]);
+  for (int i0 = tid + kRound; i0 < len; i0 += kRound) {
+    int at[kRulesHeld];
+    read(i0, at);
+#pragma unroll
+    for (int k = 0; k < kRulesHeld; ++k) touch(at[k]);
+  }
+  for (int j = tid; j < entries; j += kRulesThreads) {
+    if (j != tid) bias_id = j < p.biases ? bt[j] : -1, bias_value = j < p.biases ? bv[j] : 0.f;
+    const int at = offset(bias_id);
+    bias_at[j] = at;
+    bias_v[j] = bias_value;
+    touch(at);
+  }
+  __syncthreads();
+  int total;
+  {  // ranks: a thread takes every 256th four words of neighbouring ones
+    int before = 0;  // of the rounds before
+    for (int w0 = 0; w0 < words; w0 += 4 * kRulesThreads) {
+      const int w = w0 + 4 * tid;
+      uint4 b = make_uint4(0, 0, 0, 0);
+      if (w < words) b = *reinterpret_cast<const uint4*>(touched + w);
+      const int n0 = __popc(b.x), n1 = n0 + __popc(b.y), n2 = n1 + __popc(b.z), n3 = n2 + __popc(b.w);
+      const int at = before + block_scan<kRulesThreads / 32>(n3, s_warp, &total);
+      if (w < words) *reinterpret_cast<uint4*>(rank + w) = make_uint4(at, at + n0, at + n1, at + n2);
+      before += total;
+    }
+    total = before;
+    for (int r = tid; r < total; r += kRulesThreads) mark[r] = 0, bias_of[r] = kRulesNone;
+  }
+  __syncthreads();
+  auto count = [&](int at, int i) {
+    if (at < 0) return;
+    const int r = slot(at);
+    token_of[r] = at;  // the same from each of the token's entries
+    if (i >= prompt) atomicAdd(mark + r, 1u);
+    atomicOr(mark + r, kRulesSeen);
+  };
+#pragma unroll
+  for (int k = 0; k < kRulesHeld; ++k) count(held[k], tid + k * kRulesThreads);
+  for (int i0 = tid + kRound; i0 < len; i0 += kRound) {
+    int at[kRulesHeld];
+    read(i0, at);
+#pragma unroll
+    for (int k = 0; k < kRulesHeld; ++k) count(at[k], i0 + k * kRulesThreads);
+  }
+  for (int j = tid; j < p.biases; j += kRulesThreads) {
+    const int at = bias_at[j];
+    if (at < 0) continue;
+    const int r = slot(at);
+    token_of[r] = at;
+    atomicMin(bias_of + r, (uint32_t)j);
+  }
+  RulesRow rules;
+  if (!p.list) rules.read(p, row);
+  __syncthreads();
+  if (p.biases > 0) {
+    for (int j = tid; j < p.biases; j += kRulesThreads) {
+      if (bias_at[j] < 0) continue;
+      const uint32_t first = bias_of[slot(bias_at[j])];
+      if (first != j) twice[first] = 1;
+    }
+    __syncthreads();
+  }
+  auto bias = [&](int r) {
+    const uint32_t j = bias_of[r];
+    if (j == kRulesNone) return 0.f;
+    float sum = bias_v[j];
+    if (twice[j])
+      for (int o = j + 1; o < p.biases; ++o)
+        if (bias_at[o] == token_of[r]) sum += bias_v[o];
+    return sum;
+  };
+
+  if (p.list) {
+    const int64_t at = row * gridDim.x + blockIdx.x;
+    RulesEntry* list = p.list + at * ruled;
+    for (int r = tid; r < total; r += kRulesThreads) list[r] = RulesEntry{token_of[r], mark[r], bias(r)};
+    if (tid == 0) p.listed[at] = total;
+    return;
+  }
+  if (p.beside) {
+    griddep_wait();
+    griddep_launch();
+  }
+  const uint32_t* mask = p.allowed ? p.allowed + row * p.mask_row : nullptr;
+  const T* x = (const T*)p.x + row * p.x_row;
+  T* y = (T*)p.y + row * p.y_row;
+  for (int r0 = tid; r0 < total; r0 += 4 * kRulesThreads) {
+    int64_t i[4];
+    T v[4];
+    uint32_t allowed[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {  // loads first, past the end of the last one
+      i[k] = c0 + token_of[min(r0 + k * kRulesThreads, total - 1)];
+      v[k] = x[i[k]];  // in place: still the logit, or -infinity behind the mask
+      allowed[k] = mask ? mask[i[k] >> 5] >> (i[k] & 31) : 1u;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int r = r0 + k * kRulesThreads;
+      if (r < total && (allowed[k] & 1)) y[i[k]] = Chunk<T>::put(rules.apply(Chunk<T>::get(v[k]), mark[r]) + bias(r));
+    }
+  }
+}
+
+// Applies the lists: CTA (x, row) every gridDim.x-th 256 entries of the row's.
+template <typename T>
+__global__ void __launch_bounds__(kRulesThreads) logit_apply_kernel(const RulesParams p) {
+  const int64_t row = blockIdx.y;
+  const int parts = (int)((p.vocab + p.part - 1) / p.part), ruled = rules_ruled(p.part, (int64_t)p.history + p.biases);
+  const uint32_t* mask = p.allowed ? p.allowed + row * p.mask_row : nullptr;
+  const T* x = (const T*)p.x + row * p.x_row;
+  T* y = (T*)p.y + row * p.y_row;
+  griddep_wait();
+  griddep_launch();
+  RulesRow rules;
+  rules.read(p, row);
+  for (int part = 0; part < parts; ++part) {
+    const int64_t at = row * parts + part;
+    const int total = p.listed[at];
+    for (int r = blockIdx.x * kRulesThreads + threadIdx.x; r < total; r += gridDim.x * kRulesThreads) {
+      const RulesEntry e = p.list[at * ruled + r];
+      const int64_t i = (int64_t)part * p.part + e.token;
+      const T v = x[i];  // in place: still the logit, or -infinity behind the mask
+      if (!mask || (mask[i >> 5] >> (i & 31) & 1)) y[i] = Chunk<T>::put(rules.apply(Chunk<T>::get(v), e.mark) + e.bias);
+    }
   }
 }
 

@@ -683,13 +683,13 @@ __device__ __forceinline__ AttnPlace attn_place(const AttnParams& p, const AttnL
   return o;
 }
 
-template <int DP>
+template <int DP, int H>
 struct AttnSimtCfg {
   using Tile = AttnTileCfg<4, DP>;
-  static constexpr int kHeads = 8;  // query heads of a block
+  static constexpr int kHeads = H;  // query heads of a block
   static constexpr int kStages = DP == 256 ? 2 : 3;
   static constexpr int kWarps = DP == 256 ? 3 : (DP == 128 ? 4 : 8);
-  static constexpr int kQBytes = kHeads * DP * 4, kPBytes = kAttnTile * kHeads * 4;
+  static constexpr int kQBytes = kHeads * DP * 4, kPBytes = (kAttnTile * kHeads * 4 + 127) & ~127;
   static constexpr int kWarpBytes = kStages * Tile::kStageBytes + kQBytes + kPBytes;
   static constexpr int kSmemBytes = kWarps * kWarpBytes;
 };
@@ -697,12 +697,12 @@ struct AttnSimtCfg {
 // CUDA-core attention for fp32 (TF32 products would lose 13 bits of it).
 // Scores: lanes l and l + 16 take token l & 15, each half of the head's
 // elements.  Sums: a lane owns DP / 32 elements of all heads.
-template <int DP>
-__global__ void __launch_bounds__(AttnSimtCfg<DP>::kWarps * 32, 1) attn_simt_kernel(const AttnParams p) {
+template <int DP, int H>
+__global__ void __launch_bounds__(AttnSimtCfg<DP, H>::kWarps * 32, 1) attn_simt_kernel(const AttnParams p) {
   using T = float;
-  using Cfg = AttnSimtCfg<DP>;
+  using Cfg = AttnSimtCfg<DP, H>;
   using Tile = AttnTileCfg<4, DP>;
-  constexpr int H = Cfg::kHeads, N = Chunk<T>::N, E = DP / 32;
+  constexpr int N = Chunk<T>::N, E = DP / 32;
   extern __shared__ __align__(128) unsigned char attn_smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   unsigned char* mine = attn_smem + warp * Cfg::kWarpBytes;
@@ -1105,27 +1105,38 @@ __global__ void __launch_bounds__(AttnMmaCfg<DP, NT>::kWarps * 32, 1)
   }
 }
 
-// Joins the parts of the items that segments cut.  A warp takes a head of an item
-// of up to 32 parts, a CTA one of more, its warps a run of them each; a lane
-// holds a part's maximum and sum, then four (of 128) elements of the head.
-constexpr int kJoinWarps = 8, kJoinGrid = 4 * 148;
+// Joins the parts of the items that segments cut.  Of an item of up to 32 parts a
+// warp takes a head, one part after the other; of more parts, a CTA takes 32
+// elements of a head, each warp a run of parts, four of them at a time.
+constexpr int kJoinWarps = 8, kJoinGrid = 4 * 148, kJoinSlice = 32;
 
+// Sums of one head of an item from its parts; a lane holds four elements.
 struct AttnSum {
-  float m, l, o[8];
-  __device__ __forceinline__ void clear() {
-    m = -INFINITY, l = 0.f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) o[e] = 0.f;
-  }
-  // Parts [i0, i1) of item `c`, head h; UPPER: of more than 128 elements.  Warp-collective.
-  template <bool UPPER>
-  __device__ __forceinline__ void add(const AttnParams& p, const int4& c, int h, int i0, int i1) {
+  float m, l, o[4];
+  __device__ __forceinline__ void clear() { m = -INFINITY, l = o[0] = o[1] = o[2] = o[3] = 0.f; }
+  // Parts [i0, i1) of item `c`, head h, elements e0 + 4 (lane % LANES): 32 / LANES
+  // parts at a time, whose sums the lanes of one element keep apart.  Warp-collective.
+  template <int LANES>
+  __device__ __forceinline__ void add(const AttnParams& p, const int4& c, int h, int i0, int i1, int e0) {
+    constexpr int PER = 32 / LANES;
     const int lane = threadIdx.x & 31, dim = p.c.dim;
-    const int lo = min(lane * 4, dim - 4), hi = min(128 + lane * 4, dim - 4);  // lanes past dim repeat its last four
+    const int e = min(e0 + lane % LANES * 4, dim - 4);  // lanes past dim repeat its last four
     for (int first = i0; first < i1; first += 32) {
       const int n = min(32, i1 - first), i = first + lane;
       float2 ml = make_float2(-INFINITY, 0.f);
       if (lane < n) ml = p.part_ml[((c.z + i) * 2ll + (i == 0 ? 1 : 0)) * p.block_heads + h];
+      // eight loads at a time, none behind a branch: one from the L2 takes longer
+      // than all the arithmetic
+      float4 v[8];
+      auto load = [&](int j0) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int at = first + min(j0 + j * PER + lane / LANES, n - 1);
+          v[j] = *reinterpret_cast<const float4*>(
+              p.part_o + (((c.z + at) * 2ll + (at == 0 ? 1 : 0)) * p.block_heads + h) * dim + e);
+        }
+      };
+      load(0);
       float top = ml.x;
 #pragma unroll
       for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
@@ -1137,27 +1148,23 @@ struct AttnSum {
       for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
       m = top, l = l * keep + sum;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) o[e] *= keep;
-      // eight parts' loads at a time, none behind a branch: a load from the L2 takes
-      // longer than all the arithmetic
-      for (int j0 = 0; j0 < n; j0 += 8) {
-        float4 lower[8], upper[8];
+      for (int k = 0; k < 4; ++k) o[k] *= keep;
+      for (int j0 = 0;;) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const int at = first + min(j0 + j, n - 1);
-          const float* from = p.part_o + (((c.z + at) * 2ll + (at == 0 ? 1 : 0)) * p.block_heads + h) * dim;
-          lower[j] = *reinterpret_cast<const float4*>(from + lo);
-          if (UPPER) upper[j] = *reinterpret_cast<const float4*>(from + hi);
+          const int at = j0 + j * PER + lane / LANES;
+          const float g = __shfl_sync(0xffffffffu, f, at & 31);
+          if (at < n) o[0] += v[j].x * g, o[1] += v[j].y * g, o[2] += v[j].z * g, o[3] += v[j].w * g;
         }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float g = __shfl_sync(0xffffffffu, f, j0 + j);
-          if (j0 + j >= n) continue;
-          o[0] += lower[j].x * g, o[1] += lower[j].y * g, o[2] += lower[j].z * g, o[3] += lower[j].w * g;
-          if (UPPER) o[4] += upper[j].x * g, o[5] += upper[j].y * g, o[6] += upper[j].z * g, o[7] += upper[j].w * g;
-        }
+        j0 += 8 * PER;
+        if (j0 >= n) break;
+        load(j0);
       }
     }
+#pragma unroll
+    for (int d = LANES; d < 32; d <<= 1)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) o[k] += __shfl_xor_sync(0xffffffffu, o[k], d);
   }
 };
 
@@ -1170,9 +1177,9 @@ __device__ __forceinline__ void join_put(const AttnParams& p, const int4& c, int
   for (int j = 0; j < 4; ++j) out[j] = Chunk<T>::put(o[j] * f);
 }
 
-template <typename T, bool UPPER>
+template <typename T>
 __global__ void __launch_bounds__(kJoinWarps * 32) attn_join_kernel(const AttnParams p) {
-  __shared__ float s_o[kJoinWarps][256];
+  __shared__ float s_o[kJoinWarps][kJoinSlice];
   __shared__ float2 s_ml[kJoinWarps];
   griddep_wait();
   griddep_launch();
@@ -1180,19 +1187,19 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_join_kernel(const AttnPa
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, dim = p.c.dim, bh = p.block_heads;
   auto heads_of = [&](const int4& c) { return min(bh, p.group - c.y % p.blocks * bh); };
   AttnSum a;
-  for (int t = blockIdx.x; t < far * bh; t += gridDim.x) {
-    const int4 c = p.cut[p.cut_room - 1 - t / bh];
-    const int h = t % bh;
+  const int slices = (dim + kJoinSlice - 1) / kJoinSlice;
+  for (int t = blockIdx.x; t < far * bh * slices; t += gridDim.x) {
+    const int4 c = p.cut[p.cut_room - 1 - t / (bh * slices)];
+    const int h = t / slices % bh, e0 = t % slices * kJoinSlice;
     if (h >= heads_of(c)) continue;
     a.clear();
-    a.add<UPPER>(p, c, h, c.w * warp / kJoinWarps, c.w * (warp + 1) / kJoinWarps);
-    __syncthreads();  // the head before has been read
-#pragma unroll
-    for (int e = 0; e < 4; ++e) s_o[warp][lane * 4 + e] = a.o[e], s_o[warp][128 + lane * 4 + e] = a.o[4 + e];
+    a.add<kJoinSlice / 4>(p, c, h, c.w * warp / kJoinWarps, c.w * (warp + 1) / kJoinWarps, e0);
+    __syncthreads();  // the slice before has been read
+    if (lane < kJoinSlice / 4) *reinterpret_cast<float4*>(&s_o[warp][lane * 4]) = make_float4(a.o[0], a.o[1], a.o[2], a.o[3]);
     if (lane == 0) s_ml[warp] = make_float2(a.m, a.l);
     __syncthreads();
     const int e = threadIdx.x * 4;
-    if (e < dim) {
+    if (e < kJoinSlice && e0 + e < dim) {
       float top = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, s_ml[w].x);
@@ -1204,17 +1211,17 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_join_kernel(const AttnPa
 #pragma unroll
         for (int j = 0; j < 4; ++j) o[j] += s_o[w][e + j] * f;
       }
-      join_put<T>(p, c, h, e, l, o);
+      join_put<T>(p, c, h, e0 + e, l, o);
     }
   }
-  for (int t = warp * gridDim.x + blockIdx.x; t < near * bh; t += gridDim.x * kJoinWarps) {
-    const int4 c = p.cut[t / bh];
-    const int h = t % bh;
+  const int halves = (dim + 127) / 128;
+  for (int t = warp * gridDim.x + blockIdx.x; t < near * bh * halves; t += gridDim.x * kJoinWarps) {
+    const int4 c = p.cut[t / (bh * halves)];
+    const int h = t / halves % bh, e0 = t % halves * 128;
     if (h >= heads_of(c)) continue;
     a.clear();
-    a.add<UPPER>(p, c, h, 0, c.w);
-    if (lane * 4 < dim) join_put<T>(p, c, h, lane * 4, a.l, a.o);
-    if (128 + lane * 4 < dim) join_put<T>(p, c, h, 128 + lane * 4, a.l, a.o + 4);
+    a.add<32>(p, c, h, 0, c.w, e0);
+    if (e0 + lane * 4 < dim) join_put<T>(p, c, h, e0 + lane * 4, a.l, a.o);
   }
 }
 

@@ -163,16 +163,27 @@ int device_info(DeviceInfo** out) {
     SET_ATTN(256, 1)
     SET_ATTN(256, 2)
 #undef SET_ATTN
-    SET_GRID(attn_simt_kernel<64>, AttnSimtCfg<64>::kSmemBytes)
-    SET_GRID(attn_simt_kernel<128>, AttnSimtCfg<128>::kSmemBytes)
-    SET_GRID(attn_simt_kernel<256>, AttnSimtCfg<256>::kSmemBytes)
-    constexpr int kRulesSmem = rules_smem_bytes(kRulesStep, kRulesStep, kRulesMaxBiases);
+#define SET_SIMT(DP, H) SET_GRID((attn_simt_kernel<DP, H>), (AttnSimtCfg<DP, H>::kSmemBytes))
+#define SET_SIMT_ALL(DP) SET_SIMT(DP, 1) SET_SIMT(DP, 2) SET_SIMT(DP, 4) SET_SIMT(DP, 8)
+    SET_SIMT_ALL(64)
+    SET_SIMT_ALL(128)
+    SET_SIMT_ALL(256)
+#undef SET_SIMT_ALL
+#undef SET_SIMT
+    constexpr int kRulesSmem = kRulesMostSmem + kRulesMaxBiases * 12;
 #define SET_RULES(T)                                     \
-  SET_GRID((logit_rules_kernel<T, int32_t>), kRulesSmem) \
-  SET_GRID((logit_rules_kernel<T, int64_t>), kRulesSmem)
+  SET_GRID((logit_find_kernel<T, int32_t>), kRulesSmem) \
+  SET_GRID((logit_find_kernel<T, int64_t>), kRulesSmem) \
+  SET_MOST_SMEM(logit_copy_kernel<T>)
+    // the copy uses no shared memory, the rules beside it do
+#define SET_MOST_SMEM(kern)                                                                         \
+  PLORA_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout,             \
+                                  (int)cudaSharedmemCarveoutMaxShared),                             \
+             "cudaFuncSetAttribute(carveout)");
     SET_RULES(float)
     SET_RULES(__half)
     SET_RULES(__nv_bfloat16)
+#undef SET_MOST_SMEM
 #undef SET_RULES
 #undef SET_GRID
     // the row copies use no shared memory; an SM running them keeps its largest
@@ -655,11 +666,11 @@ int token_rows_impl(const void* host_rows, void* device_rows, bool to_host, int6
 constexpr int kAttnGrid = 148;
 constexpr int64_t kPagedMaxRows = 1 << 20;
 
-// The attention kernel of a call: padded head size, query heads of a block (in
-// eights for the tensor cores, 0: CUDA cores) and warps of a CTA.  Blocks are as
-// large as registers allow, for a second block reads the cache again.
+// The attention kernel of a call: padded head size, query heads of its block (in
+// eights for the tensor cores, 0: CUDA cores, `simt` heads) and warps of a CTA.
+// Blocks are as large as registers allow, for a second block reads the cache again.
 struct AttnPlan {
-  int dp, eights, blocks, block_heads, warps, segments;
+  int dp, eights, simt, blocks, block_heads, warps, segments;
   size_t before_offset, cut_offset, ml_offset, part_offset, bytes;
 };
 AttnPlan attn_plan(int64_t rows, int32_t heads, int32_t kv_heads, int32_t dim, int dtype) {
@@ -670,9 +681,10 @@ AttnPlan attn_plan(int64_t rows, int32_t heads, int32_t kv_heads, int32_t dim, i
   a.blocks = (group + most - 1) / most;
   a.block_heads = (group + a.blocks - 1) / a.blocks;
   a.blocks = (group + a.block_heads - 1) / a.block_heads;
+  a.eights = a.simt = 0;
   if (dtype == PLORA_DTYPE_F32) {
-    a.eights = 0;
-    a.warps = a.dp == 64 ? AttnSimtCfg<64>::kWarps : (a.dp == 128 ? AttnSimtCfg<128>::kWarps : AttnSimtCfg<256>::kWarps);
+    a.simt = a.block_heads <= 2 ? a.block_heads : (a.block_heads <= 4 ? 4 : 8);
+    a.warps = a.dp == 64 ? AttnSimtCfg<64, 8>::kWarps : (a.dp == 128 ? AttnSimtCfg<128, 8>::kWarps : AttnSimtCfg<256, 8>::kWarps);
   } else {
     a.eights = a.block_heads <= 8 ? 1 : (a.block_heads <= 16 ? 2 : 4);
 #define PLORA_WARPS(DP, NT) \
@@ -768,39 +780,80 @@ cudaError_t launch_attn(const AttnParams& p, const AttnPlan& a, int dtype, bool 
   cudaError_t e = launch_kernel(attn_plan_kernel, dim3(1), dim3(kAttnPlanThreads), 0, s, true, 0, p, kAttnGrid * a.warps);
   if (e != cudaSuccess) return e;
   e = cudaErrorInvalidValue;
-#define PLORA_SIMT(DP)                                                                                          \
-  if (a.eights == 0 && a.dp == DP)                                                                              \
-    e = launch_kernel(attn_simt_kernel<DP>, dim3(kAttnGrid), dim3(a.warps * 32), AttnSimtCfg<DP>::kSmemBytes, s, \
-                      true, 0, p);
+#define PLORA_SIMT(DP, H)                                                                                  \
+  if (a.simt == H && a.dp == DP)                                                                           \
+    e = launch_kernel(attn_simt_kernel<DP, H>, dim3(kAttnGrid), dim3(a.warps * 32),                        \
+                      AttnSimtCfg<DP, H>::kSmemBytes, s, true, 0, p);
+#define PLORA_SIMT_ALL(DP) PLORA_SIMT(DP, 1) PLORA_SIMT(DP, 2) PLORA_SIMT(DP, 4) PLORA_SIMT(DP, 8)
 #define PLORA_MMA(BF16, DP, NT, TMA)                                                                      \
   if (a.eights == NT && a.dp == DP && BF16 == (dtype == PLORA_DTYPE_BF16) && TMA == tma)                  \
     e = launch_kernel(attn_mma_kernel<BF16, DP, NT, TMA>, dim3(kAttnGrid), dim3(a.warps * 32),            \
                       AttnMmaCfg<DP, NT>::kSmemBytes, s, true, 0, p, mk, mv);
 #define PLORA_MMA_BOTH(DP, NT) \
   PLORA_MMA(true, DP, NT, true) PLORA_MMA(false, DP, NT, true) PLORA_MMA(true, DP, NT, false) PLORA_MMA(false, DP, NT, false)
-  PLORA_SIMT(64) PLORA_SIMT(128) PLORA_SIMT(256)
+  PLORA_SIMT_ALL(64) PLORA_SIMT_ALL(128) PLORA_SIMT_ALL(256)
   PLORA_MMA_BOTH(64, 1) PLORA_MMA_BOTH(64, 2) PLORA_MMA_BOTH(64, 4)
   PLORA_MMA_BOTH(128, 1) PLORA_MMA_BOTH(128, 2) PLORA_MMA_BOTH(128, 4)
   PLORA_MMA_BOTH(256, 1) PLORA_MMA_BOTH(256, 2)
 #undef PLORA_MMA_BOTH
 #undef PLORA_MMA
+#undef PLORA_SIMT_ALL
 #undef PLORA_SIMT
   if (e != cudaSuccess) return e;
   const dim3 grid(kJoinGrid), block(kJoinWarps * 32);
-#define PLORA_JOIN(T)                                                                             \
-  (a.dp == 256 ? launch_kernel(attn_join_kernel<T, true>, grid, block, 0, s, true, 0, p)          \
-               : launch_kernel(attn_join_kernel<T, false>, grid, block, 0, s, true, 0, p))
-  return dtype == PLORA_DTYPE_F32   ? PLORA_JOIN(float)
-         : dtype == PLORA_DTYPE_F16 ? PLORA_JOIN(__half)
-                                    : PLORA_JOIN(__nv_bfloat16);
-#undef PLORA_JOIN
+  return dtype == PLORA_DTYPE_F32   ? launch_kernel(attn_join_kernel<float>, grid, block, 0, s, true, 0, p)
+         : dtype == PLORA_DTYPE_F16 ? launch_kernel(attn_join_kernel<__half>, grid, block, 0, s, true, 0, p)
+                                    : launch_kernel(attn_join_kernel<__nv_bfloat16>, grid, block, 0, s, true, 0, p);
+}
+
+// The call's kernels: which run, how the finding cuts a row's vocabulary, and the
+// workspace that lists of rules need.
+struct RulesPlan {
+  bool copy, find, lists;
+  int part, parts;
+  size_t smem, listed_offset, bytes;
+};
+RulesPlan rules_plan(int64_t rows, int64_t vocab, int64_t history, int64_t biases, bool copy) {
+  RulesPlan a = {};
+  const int64_t entries = history + biases;
+  a.copy = copy;
+  a.find = entries > 0;
+  // the largest part whose tables leave room for a second CTA
+  a.part = (int)std::min<int64_t>(std::max<int64_t>(vocab, 1), kRulesMostPart);
+  while (a.part > 1024 && rules_smem_bytes(a.part, entries, 0) > kRulesMostSmem) a.part = (a.part / 2 + 31) & ~31;
+  a.parts = (int)((vocab + a.part - 1) / a.part);
+  a.smem = (size_t)rules_smem_bytes(a.part, entries, (int)biases);
+  // one finding CTA fits on an SM beside the copy
+  a.lists = a.find && copy && rows * a.parts > kRulesBesideCtas;
+  if (a.lists) {
+    a.listed_offset = align256((size_t)(rows * a.parts) * rules_ruled(a.part, entries) * sizeof(RulesEntry));
+    a.bytes = a.listed_offset + align256((size_t)(rows * a.parts) * 4);
+  }
+  return a;
 }
 
 template <typename T>
-cudaError_t launch_rules(const RulesParams& p, bool wide, int64_t rows, size_t smem, cudaStream_t s) {
-  const dim3 grid((unsigned)((p.vocab + p.chunk - 1) / p.chunk), (unsigned)rows);
-  return wide ? launch_kernel(logit_rules_kernel<T, int64_t>, grid, dim3(kRulesThreads), smem, s, true, 0, p)
-              : launch_kernel(logit_rules_kernel<T, int32_t>, grid, dim3(kRulesThreads), smem, s, true, 0, p);
+cudaError_t launch_rules(RulesParams& p, const RulesPlan& a, bool wide, int64_t rows, cudaStream_t s) {
+  const dim3 block(kRulesThreads);
+  cudaError_t e = cudaSuccess;
+  auto copy = [&] {
+    const int64_t strips = (p.vocab * sizeof(T) + kRulesStrip * 16 - 1) / (kRulesStrip * 16);
+    const dim3 grid((unsigned)((strips * 32 + kRulesThreads - 1) / kRulesThreads), (unsigned)rows);
+    e = launch_kernel(logit_copy_kernel<T>, grid, block, 0, s, true, 0, p);
+  };
+  p.beside = a.copy && !a.lists;
+  if (p.beside) {
+    copy();
+    if (e != cudaSuccess) return e;
+  }
+  if (!a.find) return e;
+  const dim3 grid((unsigned)a.parts, (unsigned)rows);
+  e = wide ? launch_kernel(logit_find_kernel<T, int64_t>, grid, block, a.smem, s, true, 0, p)
+           : launch_kernel(logit_find_kernel<T, int32_t>, grid, block, a.smem, s, true, 0, p);
+  if (e != cudaSuccess || !a.lists) return e;
+  copy();
+  if (e != cudaSuccess) return e;
+  return launch_kernel(logit_apply_kernel<T>, dim3(4, (unsigned)rows), block, 0, s, true, 0, p);
 }
 
 }  // namespace
@@ -1212,19 +1265,26 @@ int plora_paged_attention(const void* q, int64_t q_row_stride, int64_t q_head_st
   return PLORA_OK;
 }
 
+size_t plora_logit_rules_workspace(int64_t rows, int64_t vocab, int64_t history, int64_t biases) {
+  if (rows < 0 || rows > 65535 || vocab < 0 || vocab > (1 << 30) || history < 0 || history > (1 << 30) - 1 ||
+      biases < 0 || biases > kRulesMaxBiases)
+    return 0;
+  return rules_plan(rows, vocab, history, biases, true).bytes;
+}
+
 int plora_logit_rules(const void* logits, int64_t logits_stride, void* out, int64_t out_stride, int64_t rows,
                       int64_t vocab, int32_t dtype, const void* tokens, int64_t tokens_stride, int64_t history,
                       const int32_t* token_lens, const int32_t* prompt_lens, const float* repetition,
                       const float* presence, const float* frequency, const void* bias_tokens,
                       int64_t bias_tokens_stride, const float* bias_values, int64_t bias_values_stride,
                       int64_t biases, const int32_t* allowed, int64_t allowed_stride, int32_t token_bytes,
-                      void* stream) {
+                      void* workspace, size_t workspace_size, void* stream) {
   g_last_error.clear();
   if (!valid_dtype(dtype)) return fail(PLORA_ERR_INVALID_ARGUMENT, "unknown dtype %d", dtype);
   if (rows < 0 || vocab < 0 || history < 0 || biases < 0)
     return fail(PLORA_ERR_INVALID_ARGUMENT, "negative rows, vocab, history or biases");
   if (token_bytes != 4 && token_bytes != 8) return fail(PLORA_ERR_INVALID_ARGUMENT, "token ids of %d bytes", token_bytes);
-  if (rows > 65535 || vocab > INT32_MAX || history > (1 << 30) - 1 || biases > kRulesMaxBiases)
+  if (rows > 65535 || vocab > (1 << 30) || history > (1 << 30) - 1 || biases > kRulesMaxBiases)
     return fail(PLORA_ERR_UNSUPPORTED, "rows > 65535, vocab or history beyond 2^30, or more than %d biases a row",
                 kRulesMaxBiases);
   if (rows == 0 || vocab == 0) return PLORA_OK;
@@ -1234,6 +1294,11 @@ int plora_logit_rules(const void* logits, int64_t logits_stride, void* out, int6
       (biases && (bias_tokens_stride < 0 || bias_values_stride < 0)) ||
       (allowed && allowed_stride < 0))
     return fail(PLORA_ERR_INVALID_ARGUMENT, "row strides below the vocabulary, or negative");
+  const RulesPlan a = rules_plan(rows, vocab, history, biases, logits != out || logits_stride != out_stride || allowed);
+  if (workspace_size < a.bytes || (a.bytes && !workspace))
+    return fail(PLORA_ERR_WORKSPACE, "logit rules workspace %zu < %zu bytes", workspace_size, a.bytes);
+  if (reinterpret_cast<uintptr_t>(workspace) % 256)
+    return fail(PLORA_ERR_INVALID_ARGUMENT, "workspace must be 256-byte aligned");
   const uintptr_t el = elem_size(dtype) - 1;
   if ((reinterpret_cast<uintptr_t>(logits) & el) || (reinterpret_cast<uintptr_t>(out) & el))
     return fail(PLORA_ERR_INVALID_ARGUMENT, "logits or out not aligned to its type");
@@ -1248,21 +1313,17 @@ int plora_logit_rules(const void* logits, int64_t logits_stride, void* out, int6
   p.bias_tokens = bias_tokens, p.bias_row = bias_tokens_stride;
   p.bias_values = bias_values, p.value_row = bias_values_stride, p.biases = (int32_t)biases;
   p.allowed = reinterpret_cast<const uint32_t*>(allowed), p.mask_row = allowed_stride;
-  // the largest chunk that still makes eight CTAs for each SM, four of which its
-  // tables leave room for: a row's history is read once per chunk
-  p.chunk = kRulesStep;
-  const int64_t entries = history + biases;
-  for (int chunk = 2 * kRulesStep; chunk <= kRulesMaxChunk; chunk += kRulesStep)
-    if (rows * ((vocab + chunk - 1) / chunk) >= 8 * di->sm_count &&
-        rules_smem_bytes(chunk, entries, (int)biases) <= 48 * 1024)
-      p.chunk = chunk;
-  const size_t smem = entries ? (size_t)rules_smem_bytes(p.chunk, entries, (int)biases) : 0;
+  p.part = a.part;
+  if (a.lists) {
+    p.list = static_cast<RulesEntry*>(workspace);
+    p.listed = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(workspace) + a.listed_offset);
+  }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool wide = token_bytes == 8;
-  cudaError_t e = dtype == PLORA_DTYPE_F32   ? launch_rules<float>(p, wide, rows, smem, s)
-                  : dtype == PLORA_DTYPE_F16 ? launch_rules<__half>(p, wide, rows, smem, s)
-                                             : launch_rules<__nv_bfloat16>(p, wide, rows, smem, s);
-  PLORA_CUDA(e, "launch logit_rules_kernel");
+  cudaError_t e = dtype == PLORA_DTYPE_F32   ? launch_rules<float>(p, a, wide, rows, s)
+                  : dtype == PLORA_DTYPE_F16 ? launch_rules<__half>(p, a, wide, rows, s)
+                                             : launch_rules<__nv_bfloat16>(p, a, wide, rows, s);
+  PLORA_CUDA(e, "launch logit rules");
   return PLORA_OK;
 }
 

@@ -12,8 +12,9 @@ from dataclasses import dataclass
 
 import torch
 
-from .paged import _call, _no_grad
-from .sgmv import _as, _require_cuda, dtype_code
+from . import _native
+from .paged import _call, _no_grad, _same_device
+from .sgmv import _as, dtype_code
 
 
 @dataclass
@@ -67,22 +68,24 @@ def _ptr(t: torch.Tensor | None) -> int:
 
 
 def _row_stride(t: torch.Tensor | None) -> int:
-    return 0 if t is None else (t.stride(0) if t.shape[0] > 1 else t.shape[1])
+    return t.stride(0) if t is not None else 0
 
 
 def apply_logit_rules(logits: torch.Tensor, rules: LogitRules, out: torch.Tensor | None = None) -> torch.Tensor:
     """``rules`` on logits (B, V), computed in fp32 and rounded once to the
     logits' dtype; into ``out`` (which may be ``logits``) or a new tensor."""
-    dev = _require_cuda(logits, *rules.tensors())
+    dev = logits.get_device()
+    _same_device(dev, logits, *rules.tensors())
     _no_grad(logits)
     if logits.dim() != 2:
         raise ValueError("logits must be (B, V)")
     rows, vocab = logits.shape
-    if logits.shape[1] > 1 and logits.stride(1) != 1:
+    row, step = logits.stride()
+    if step != 1 and vocab > 1:
         raise ValueError("logits rows must be contiguous")
     if out is None:
         out = logits.new_empty((rows, vocab))
-    elif out.shape != logits.shape or out.dtype != logits.dtype or out.device != dev or (vocab > 1 and out.stride(1) != 1):
+    elif out.shape != logits.shape or out.dtype is not logits.dtype or out.get_device() != dev or (vocab > 1 and out.stride(1) != 1):
         raise ValueError("out must have the logits' shape, dtype and device, with contiguous rows")
     tokens, bias_tokens, bias_values, allowed = rules.tokens, rules.bias_tokens, rules.bias_values, rules.allowed
     width = None
@@ -116,13 +119,16 @@ def apply_logit_rules(logits: torch.Tensor, rules: LogitRules, out: torch.Tensor
     rep = _per_row(rules.repetition_penalty, rows, torch.float32, "repetition_penalty")
     pres = _per_row(rules.presence_penalty, rows, torch.float32, "presence_penalty")
     freq = _per_row(rules.frequency_penalty, rows, torch.float32, "frequency_penalty")
+    history, biases = tokens.shape[1] if tokens is not None else 0, bias_tokens.shape[1] if bias_tokens is not None else 0
+    ws_bytes = _native.load().plora_logit_rules_workspace(rows, vocab, history, biases)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=logits.device) if ws_bytes else None
     _call(
         dev, "plora_logit_rules",
-        logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, out.data_ptr(),
+        logits.data_ptr(), row if rows > 1 else vocab, out.data_ptr(),
         out.stride(0) if rows > 1 else vocab, rows, vocab, dtype_code(logits.dtype), _ptr(tokens),
-        _row_stride(tokens), tokens.shape[1] if tokens is not None else 0, _ptr(lens), _ptr(prompt), _ptr(rep),
+        _row_stride(tokens), history, _ptr(lens), _ptr(prompt), _ptr(rep),
         _ptr(pres), _ptr(freq), _ptr(bias_tokens), _row_stride(bias_tokens), _ptr(bias_values),
-        _row_stride(bias_values), bias_tokens.shape[1] if bias_tokens is not None else 0, _ptr(allowed),
-        _row_stride(allowed), 4 if width == torch.int32 else 8,
+        _row_stride(bias_values), biases, _ptr(allowed), _row_stride(allowed), 4 if width == torch.int32 else 8,
+        _ptr(ws), ws_bytes,
     )
     return out

@@ -42,49 +42,64 @@ def _no_grad(*tensors: torch.Tensor | None) -> None:
                 raise RuntimeError("the paged-cache and logit operators have no gradient: call them under torch.no_grad()")
 
 
-def _heads(t: torch.Tensor) -> tuple[torch.Tensor, tuple[int, ...]]:
-    """``t`` with dense last dimension and 16-byte aligned rows (a copy where
-    it has neither) and its strides, 0 for dimensions of one."""
-    vec = 16 // t.element_size()
-    if t.is_contiguous() and t.shape[-1] % vec == 0:
-        st = t.stride() if 1 not in t.shape else _strides(t)
-    else:
-        st = _strides(t)
-        if (t.shape[-1] > 1 and st[-1] != 1) or any(s % vec for s in st[:-1]):
-            t = t.contiguous()
-            st = _strides(t)
-    if t.data_ptr() % 16:
-        t = t.clone(memory_format=torch.contiguous_format)
-        st = _strides(t)
-    return t, st
+def _same_device(index: int, *tensors: torch.Tensor) -> None:
+    """All on CUDA device ``index``.  (Ordinals: a decode step's kernels take a
+    few microseconds, and comparing torch.device objects would take one.)"""
+    if index < 0:
+        _require_cuda(*tensors)
+    for t in tensors:
+        if t.get_device() != index:
+            raise ValueError(f"tensors on different devices: cuda:{index} and {t.device}")
 
 
 def _strides(t: torch.Tensor) -> tuple[int, ...]:
+    """Strides, 0 for dimensions of one."""
     return tuple([st if n > 1 else 0 for n, st in zip(t.shape, t.stride())])
 
 
+def _heads(t: torch.Tensor) -> tuple[torch.Tensor, tuple[int, ...], int]:
+    """``t`` with dense last dimension and 16-byte aligned rows (a copy where
+    it has neither), its strides and its address."""
+    vec = 16 // t.element_size()
+    ptr, st = t.data_ptr(), t.stride()
+    low = ptr // t.element_size()
+    for x in st[:-1]:
+        low |= x
+    if st[-1] == 1 and low % vec == 0:  # the rule, with any dimensions of one
+        return t, st, ptr
+    st = _strides(t)
+    if (t.shape[-1] > 1 and st[-1] != 1) or any([s % vec for s in st[:-1]]) or ptr % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+        st, ptr = _strides(t), t.data_ptr()
+    return t, st, ptr
+
+
 def _check_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor, rows: int, dim: int,
-                 dtype: torch.dtype) -> tuple[int, int, int, int, int]:
-    """(num_pages, kv_heads, page_size, k page stride, v page stride)."""
-    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape:
+                 dtype: torch.dtype) -> tuple[int, int, int, int, int, int]:
+    """(num_pages, kv_heads, page_size, k page stride, v page stride, page-table row stride)."""
+    shape = k_cache.shape
+    if len(shape) != 4 or shape != v_cache.shape:
         raise ValueError("k_cache and v_cache must both be (num_pages, kv_heads, page_size, head_dim)")
-    pages, kv_heads, size, d = k_cache.shape
+    pages, kv_heads, size, d = shape
     if d != dim:
         raise ValueError(f"head_dim mismatch: tokens={dim}, cache={d}")
-    if not (k_cache.dtype == v_cache.dtype == dtype):
+    if k_cache.dtype is not dtype or v_cache.dtype is not dtype:
         raise TypeError(f"dtype mismatch: tokens={dtype}, k_cache={k_cache.dtype}, v_cache={v_cache.dtype}")
+    page = kv_heads * size * d
+    k_page = v_page = page
     if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
         inner = (size * d, d, 1)
         for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
-            if any(st != want for n, st, want in zip(c.shape[1:], c.stride()[1:], inner) if n > 1):
+            if any([st != want for n, st, want in zip(c.shape[1:], c.stride()[1:], inner) if n > 1]):
                 raise ValueError(f"{name} pages must be contiguous")
-    if page_table.dim() != 2 or page_table.shape[0] != rows or page_table.dtype != torch.int32:
+        if pages > 1:
+            k_page, v_page = k_cache.stride(0), v_cache.stride(0)
+    if page_table.dtype is not torch.int32 or page_table.dim() != 2 or page_table.shape[0] != rows:
         raise ValueError(f"page_table must be int32 ({rows}, max_pages)")
-    if page_table.shape[1] > 1 and page_table.stride(1) != 1:
+    row, step = page_table.stride()
+    if step != 1 and page_table.shape[1] > 1:
         raise ValueError("page_table rows must be contiguous")
-    page = kv_heads * size * d
-    return (pages, kv_heads, size, k_cache.stride(0) if pages > 1 else page,
-            v_cache.stride(0) if pages > 1 else page)
+    return pages, kv_heads, size, k_page, v_page, row if rows > 1 else page_table.shape[1]
 
 
 def _lens(t: torch.Tensor, rows: int, name: str) -> torch.Tensor:
@@ -93,9 +108,8 @@ def _lens(t: torch.Tensor, rows: int, name: str) -> torch.Tensor:
     return _as(t, torch.int32)
 
 
-def _call(dev: torch.device, func: str, *args: object) -> None:
+def _call(index: int, func: str, *args: object) -> None:
     """The entry point on the device's current stream, with the device current."""
-    index = dev.index
     # the raw handle: a Stream object costs 2 us of a call whose kernel takes less than 3
     stream = torch._C._cuda_getCurrentRawStream(index)
     if index == torch.cuda.current_device():
@@ -131,40 +145,53 @@ def paged_append(
     the rotated queries and, with ``return_keys``, the rotated keys (padded
     tokens zero); None for what was not given or asked for.  Rows of one call
     must not write to the same page."""
-    dev = _require_cuda(k, v, k_cache, v_cache, page_table, past_lens,
-                        *[t for t in (q, new_lens, phases) if t is not None])
+    dev = k.get_device()
+    _same_device(dev, k, v, k_cache, v_cache, page_table, past_lens)
     _no_grad(q, k, v)
-    if k.dim() != 4 or v.shape != k.shape or (q is not None and (q.dim() != 4 or q.shape[:2] != k.shape[:2]
-                                                                 or q.shape[3] != k.shape[3])):
+    shape, dtype = k.shape, k.dtype
+    if len(shape) != 4 or v.shape != shape:
         raise ValueError("q must be (B, M, heads, D), k and v (B, M, kv_heads, D)")
-    if v.dtype != k.dtype or (q is not None and q.dtype != k.dtype):
+    rows, new, kv_heads, dim = shape
+    if v.dtype is not dtype:
         raise TypeError("q, k and v must share one dtype")
-    rows, new, kv_heads, dim = k.shape
-    pages, ckv, size, k_page, v_page = _check_cache(k_cache, v_cache, page_table, rows, dim, k.dtype)
+    pages, ckv, size, k_page, v_page, table_row = _check_cache(k_cache, v_cache, page_table, rows, dim, dtype)
     if ckv != kv_heads:
         raise ValueError(f"kv_heads mismatch: k={kv_heads}, cache={ckv}")
-    heads = q.shape[2] if q is not None else 0
     past = _lens(past_lens, rows, "past_lens")
-    news = _lens(new_lens, rows, "new_lens") if new_lens is not None else None
-    pairs = 0
+    news_ptr = phases_ptr = q_ptr = q_out_ptr = pairs = heads = 0
+    q_out = k_out = None
+    qs = (0, 0, 0)
+    if new_lens is not None:
+        _same_device(dev, new_lens)
+        new_lens = _lens(new_lens, rows, "new_lens")
+        news_ptr = new_lens.data_ptr()
     if phases is not None:
-        if phases.dim() != 1 or phases.dtype != torch.int64:
+        _same_device(dev, phases)
+        if phases.dim() != 1 or phases.dtype is not torch.int64:
             raise ValueError("phases must be the int64 tensor of rotary_phases()")
         pairs = phases.shape[0]
         phases = phases.contiguous()
-    kc, ks = _heads(k)
-    vc, vs = _heads(v)
-    qc, qs = _heads(q) if q is not None else (None, (0, 0, 0))
-    q_out = k.new_empty((rows, new, heads, dim)) if q is not None else None
-    k_out = k.new_empty((rows, new, kv_heads, dim)) if return_keys else None
+        phases_ptr = phases.data_ptr() if pairs else 0
+    if q is not None:
+        _same_device(dev, q)
+        if q.dim() != 4 or q.shape[0] != rows or q.shape[1] != new or q.shape[3] != dim:
+            raise ValueError("q must be (B, M, heads, D), k and v (B, M, kv_heads, D)")
+        if q.dtype is not dtype:
+            raise TypeError("q, k and v must share one dtype")
+        heads = q.shape[2]
+        q, qs, q_ptr = _heads(q)
+        q_out = k.new_empty((rows, new, heads, dim))
+        q_out_ptr = q_out.data_ptr()
+    k, ks, k_ptr = _heads(k)
+    v, vs, v_ptr = _heads(v)
+    if return_keys:
+        k_out = k.new_empty((rows, new, kv_heads, dim))
     _call(
         dev, "plora_paged_append",
-        qc.data_ptr() if qc is not None else 0, qs[0], qs[1], qs[2], kc.data_ptr(), ks[0], ks[1], ks[2],
-        vc.data_ptr(), vs[0], vs[1], vs[2], q_out.data_ptr() if q_out is not None else 0,
-        k_out.data_ptr() if k_out is not None else 0, k_cache.data_ptr(), v_cache.data_ptr(), k_page, v_page,
-        page_table.data_ptr(), page_table.stride(0) if rows > 1 else page_table.shape[1], past.data_ptr(),
-        news.data_ptr() if news is not None else 0, phases.data_ptr() if pairs else 0, pairs, int(interleaved),
-        rotary_scale, rows, new, heads, kv_heads, dim, size, pages, page_table.shape[1], dtype_code(k.dtype),
+        q_ptr, qs[0], qs[1], qs[2], k_ptr, ks[0], ks[1], ks[2], v_ptr, vs[0], vs[1], vs[2], q_out_ptr,
+        k_out.data_ptr() if return_keys else 0, k_cache.data_ptr(), v_cache.data_ptr(), k_page, v_page,
+        page_table.data_ptr(), table_row, past.data_ptr(), news_ptr, phases_ptr, pairs, interleaved,
+        rotary_scale, rows, new, heads, kv_heads, dim, size, pages, page_table.shape[1], dtype_code(dtype),
     )
     return q_out, k_out
 
@@ -184,28 +211,29 @@ def paged_attention(
     ``seq_lens[b]`` cached tokens (the last ``window`` of them if window > 0).
     ``scale`` defaults to D ** -0.5; rows without tokens give zeros.  Heads may
     be any multiple of the cache's kv_heads."""
-    dev = _require_cuda(q, k_cache, v_cache, page_table, seq_lens)
+    dev = q.get_device()
+    _same_device(dev, q, k_cache, v_cache, page_table, seq_lens)
     _no_grad(q)
     if q.dim() != 3:
         raise ValueError("q must be (B, heads, D)")
     rows, heads, dim = q.shape
-    pages, kv_heads, size, k_page, v_page = _check_cache(k_cache, v_cache, page_table, rows, dim, q.dtype)
-    if heads == 0 or heads % kv_heads:
+    dtype = q.dtype
+    pages, kv_heads, size, k_page, v_page, table_row = _check_cache(k_cache, v_cache, page_table, rows, dim, dtype)
+    if heads == 0 or kv_heads == 0 or heads % kv_heads:
         raise ValueError(f"{heads} heads over {kv_heads} kv heads")
     lens = _lens(seq_lens, rows, "seq_lens")
     if out is None:
         out = q.new_empty((rows, heads, dim))
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or not out.is_contiguous():
+    elif out.shape != q.shape or out.dtype is not dtype or out.get_device() != dev or not out.is_contiguous():
         raise ValueError("out must be a contiguous tensor of q's shape, dtype and device")
-    qc, qs = _heads(q)
-    code = dtype_code(q.dtype)
+    q, qs, q_ptr = _heads(q)
+    code = dtype_code(dtype)
     ws_bytes = _native.load().plora_paged_attention_workspace(rows, heads, kv_heads, dim, code)
     ws = lens.new_empty(max(ws_bytes, 256) // 4)
     _call(
         dev, "plora_paged_attention",
-        qc.data_ptr(), qs[0], qs[1], k_cache.data_ptr(), v_cache.data_ptr(), k_page, v_page, page_table.data_ptr(),
-        page_table.stride(0) if rows > 1 else page_table.shape[1], lens.data_ptr(), out.data_ptr(),
-        dim**-0.5 if scale is None else scale, window, rows, heads, kv_heads, dim, size, pages, page_table.shape[1],
-        code, ws.data_ptr(), ws_bytes,
+        q_ptr, qs[0], qs[1], k_cache.data_ptr(), v_cache.data_ptr(), k_page, v_page, page_table.data_ptr(),
+        table_row, lens.data_ptr(), out.data_ptr(), dim**-0.5 if scale is None else scale, window, rows, heads,
+        kv_heads, dim, size, pages, page_table.shape[1], code, ws.data_ptr(), ws_bytes,
     )
     return out

@@ -103,6 +103,11 @@ CASES = [
     (3, 20001, None, None, False, F32, False),
     (2, 9000, 0, 0, False, BF, True),
     (2, 300, 5000, 4096, True, BF, True),     # lists longer than the vocabulary: many repeats
+    (200, 3001, 60, 9, True, FH, True),       # rows by lists
+    (170, 3001, 600, None, False, BF, False),
+    (151, 900, None, 70, True, F32, True),
+    (3, 300000, 9000, 20, True, BF, True),    # more than one part of the vocabulary
+    (80, 300000, 40, 5, False, BF, True),
 ]
 
 

@@ -81,11 +81,11 @@ def test_rules_arguments_rejected_before_cuda(native):
 
     def rules(**kw):
         a = dict(x=D, xs=100, y=D, ys=100, rows=2, vocab=100, dtype=native.DTYPE_BF16, tok=D, tr=8, hist=8, bt=D, br=4,
-                 bv=D, vr=4, k=4, mask=None, mr=0, tb=8)
+                 bv=D, vr=4, k=4, mask=None, mr=0, tb=8, ws=D, wb=1 << 30)
         a.update(kw)
         return lib.plora_logit_rules(a["x"], a["xs"], a["y"], a["ys"], a["rows"], a["vocab"], a["dtype"], a["tok"], a["tr"],
                                      a["hist"], None, None, None, None, None, a["bt"], a["br"], a["bv"], a["vr"], a["k"],
-                                     a["mask"], a["mr"], a["tb"], None)
+                                     a["mask"], a["mr"], a["tb"], a["ws"], a["wb"], None)
 
     for kw in (dict(dtype=3), dict(rows=-1), dict(vocab=-1), dict(hist=-1), dict(k=-1), dict(tb=2), dict(x=None),
                dict(y=None), dict(tok=None), dict(bt=None), dict(bv=None), dict(xs=99), dict(ys=99), dict(tr=-1),
@@ -94,6 +94,14 @@ def test_rules_arguments_rejected_before_cuda(native):
     for kw in (dict(rows=70000), dict(vocab=1 << 31, xs=1 << 31, ys=1 << 31), dict(hist=1 << 30), dict(k=4097)):
         assert rules(**kw) == native.ERR_UNSUPPORTED, kw
     assert rules(rows=0) == native.OK and rules(vocab=0) == native.OK
+    assert rules(ws=D + 64) == native.ERR_INVALID_ARGUMENT
+    need = lib.plora_logit_rules_workspace(1000, 100, 8, 4)
+    assert need > 0 and lib.plora_logit_rules_workspace(2, 100, 8, 4) == 0
+    # the lists are for a copy, which a call in place without a mask does not make
+    assert rules(rows=1000, y=2 * D, wb=need - 1) == native.ERR_WORKSPACE
+    assert rules(rows=1000, y=2 * D, ws=None, wb=need) == native.ERR_WORKSPACE
+    for bad in ((-1, 100, 8, 4), (1000, 1 << 31, 8, 4), (1000, 100, -1, 4), (1000, 100, 8, 5000)):
+        assert lib.plora_logit_rules_workspace(*bad) == 0
 
 
 def test_cpu_tensors_are_refused():
@@ -128,7 +136,7 @@ def test_heads_copies_only_what_it_must():
     for same in (t, t.transpose(0, 1), t[:, :, 1:3], t[:, :, :1].expand(2, 3, 4, 16)):
         assert _heads(same)[0].data_ptr() == same.data_ptr()
     for other in (t.transpose(-1, -2), t[..., 1:9], torch.zeros(2, 3, 4, 12, dtype=torch.bfloat16)[..., :8]):
-        got, st = _heads(other)
-        assert got.is_contiguous() and got.data_ptr() % 16 == 0
+        got, st, ptr = _heads(other)
+        assert got.is_contiguous() and got.data_ptr() == ptr and ptr % 16 == 0
         assert other.shape[-1] % 8 or all(s % 8 == 0 for s in st[:-1])  # heads that the operators take
-    assert _heads(t[:1])[1][0] == 0
+    assert _heads(torch.zeros(1, 2, 4, 16, dtype=torch.bfloat16).as_strided((1, 2, 4, 16), (7, 64, 16, 1)))[1][0] % 8 == 0
