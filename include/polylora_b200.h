@@ -342,8 +342,8 @@ int plora_peft_pack(const char* path, const char* const* modules, int32_t num_mo
  * head_dim).  A token on a page outside [0, num_pages) reads as zeros, and
  * seq_lens beyond the table's reach are clamped to it; the first raises
  * PLORA_DEV_PAGE_RANGE.  Sums in fp32; repeated calls agree bit for bit.  The
- * workspace (plora_paged_attention_workspace bytes, 256-byte aligned; 0 for
- * arguments the call rejects) needs no initialisation; calls that may overlap
+ * workspace (plora_paged_attention_workspace bytes, 256-byte aligned; 0 for few
+ * short rows and for arguments the call rejects) needs no initialisation; calls that may overlap
  * need one each. */
 int plora_paged_append(const void* q, int64_t q_row_stride, int64_t q_token_stride, int64_t q_head_stride,
                        const void* k, int64_t k_row_stride, int64_t k_token_stride, int64_t k_head_stride,
@@ -355,7 +355,8 @@ int plora_paged_append(const void* q, int64_t q_row_stride, int64_t q_token_stri
                        int32_t kv_heads, int32_t head_dim, int32_t page_size, int64_t num_pages, int64_t max_pages,
                        int32_t dtype, void* stream);
 
-size_t plora_paged_attention_workspace(int64_t rows, int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t dtype);
+size_t plora_paged_attention_workspace(int64_t rows, int32_t heads, int32_t kv_heads, int32_t head_dim,
+                                       int32_t page_size, int64_t max_pages, int64_t window, int32_t dtype);
 
 int plora_paged_attention(const void* q, int64_t q_row_stride, int64_t q_head_stride, const void* k_cache,
                           const void* v_cache, int64_t k_page_stride, int64_t v_page_stride,

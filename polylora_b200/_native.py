@@ -163,7 +163,7 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
             _i32, _i32, ctypes.c_float, _i64, _i64, _i32, _i32, _i32, _i32, _i64, _i64, _i32, _c_void_p,
         ],
     ),
-    "plora_paged_attention_workspace": (_size, [_i64, _i32, _i32, _i32, _i32]),
+    "plora_paged_attention_workspace": (_size, [_i64, _i32, _i32, _i32, _i32, _i64, _i64, _i32]),
     "plora_paged_attention": (
         ctypes.c_int,
         [

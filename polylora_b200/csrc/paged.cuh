@@ -285,6 +285,10 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const Appe
 // segments' bounds depend on the lengths only, not on who takes them, and an item
 // cut by them is put together in the order of the list (attn_join_kernel), so
 // results do not depend on timing.
+//
+// Few items of few tiles, which the SMs hold at once, need no list: a cluster of
+// CTAs takes an item, its warps equal parts of the tiles, and puts them together
+// through distributed shared memory, in one launch.
 constexpr int kAttnTile = 16;
 
 // 2^x to 2 ulp; results below 2^-126 are zero, next to a largest term of 1.
@@ -302,6 +306,7 @@ struct AttnParams {
   int64_t q_row, q_head;
   int32_t rows, group, blocks, block_heads, window;  // blocks of block_heads query heads cover a group
   float scale_log2;                                  // scale * log2(e)
+  int32_t direct;                                    // CTAs of an item's cluster; 0: by the list
   // workspace
   struct AttnWork* work;
   int64_t* before;  // (rows): tiles of the rows before, per item
@@ -327,9 +332,8 @@ struct AttnRow {
   int lo, n;   // tokens [lo, n)
   int t0, t1;  // tiles [t0, t1), at least one
 };
-__device__ __forceinline__ AttnRow attn_row(const AttnParams& p, int row) {
+__device__ __forceinline__ AttnRow attn_row(const AttnParams& p, int64_t n) {  // n: its seq_lens
   AttnRow r;
-  int64_t n = p.seq_lens[row];
   n = n < 0 ? 0 : (n > p.c.capacity ? p.c.capacity : n);
   r.n = (int)n;
   r.lo = p.window > 0 ? max(0, r.n - p.window) : 0;
@@ -342,14 +346,19 @@ __device__ __forceinline__ AttnRow attn_row(const AttnParams& p, int row) {
 // a group's query heads, tiles.
 struct AttnCursor {
   int row, kv, blk, tile;
+  int next_n;  // the next row's length, on its way since this row began
   AttnRow r;
+  __device__ __forceinline__ void enter(const AttnParams& p, int64_t n) {
+    r = attn_row(p, n);
+    next_n = row + 1 < p.rows ? p.seq_lens[row + 1] : 0;
+  }
   __device__ __forceinline__ void next(const AttnParams& p) {
     if (++tile < r.t1) return;
     if (++blk == p.blocks) {
       blk = 0;
       if (++kv == p.c.kv_heads) {
         kv = 0;
-        if (++row < p.rows) r = attn_row(p, row);
+        if (++row < p.rows) enter(p, next_n);
       }
     }
     tile = r.t0;
@@ -388,6 +397,7 @@ __host__ __device__ constexpr int attn_asked_max(int warps, int block_heads) {
 constexpr int kAttnPlanThreads = 1024;
 constexpr int kAttnDealOnly = 32;   // tiles a warp up to which all are dealt
 constexpr int kAttnChunk = 8;       // smallest chunk: a loader's lead of up to 5 tiles then spans two segments
+constexpr int kAttnDirect = 8;      // most tiles of a warp without a list
 constexpr int kAttnAsk = 4;         // tiles ahead of which the next segment is asked for
 
 // Counts the tiles of the rows and cuts their list.  One CTA.
@@ -400,7 +410,7 @@ __global__ void __launch_bounds__(kAttnPlanThreads) attn_plan_kernel(const AttnP
     const int row = first + threadIdx.x;
     int n = 0, sum;
     if (row < p.rows) {
-      const AttnRow r = attn_row(p, row);
+      const AttnRow r = attn_row(p, p.seq_lens[row]);
       n = r.t1 - r.t0;
     }
     const int before = block_scan<kAttnPlanThreads / 32>(n, s_warp, &sum);
@@ -481,7 +491,7 @@ struct AttnList {
       hi = min(hi, lo + step);
     }
     s.at.row = lo;
-    s.at.r = attn_row(p, lo);
+    s.at.enter(p, p.seq_lens[lo]);
     const int n = s.at.r.t1 - s.at.r.t0;
     const int rest = (int)(s.begin - first), item = rest / n;
     s.at.kv = item / p.blocks;
@@ -501,11 +511,25 @@ struct AttnWalk {
   bool have_nxt;
   // False when this warp has nothing to do.
   __device__ __forceinline__ bool start(const AttnParams& p) {
+    more = have_nxt = false;
+    if (p.direct) {
+      const int item = blockIdx.x / p.direct, rank = blockIdx.x - item * p.direct, per_row = p.c.kv_heads * p.blocks;
+      const int parts = p.direct * (blockDim.x >> 5), id = (threadIdx.x >> 5) * p.direct + rank;
+      cur.at.row = item / per_row;
+      cur.at.kv = (item - cur.at.row * per_row) / p.blocks;
+      cur.at.blk = item - cur.at.row * per_row - cur.at.kv * p.blocks;
+      cur.at.enter(p, p.seq_lens[cur.at.row]);
+      const int n = cur.at.r.t1 - cur.at.r.t0, first = (int)((int64_t)n * id / parts);
+      cur.at.tile = cur.at.r.t0 + first;
+      cur.id = 0, cur.begin = 0;
+      cur.count = (int)((int64_t)n * (id + 1) / parts) - first;
+      return cur.count > 0;
+    }
     list.read(p);
     // few segments spread over the SMs
     const int id = (threadIdx.x >> 5) * gridDim.x + blockIdx.x;
     if (id >= list.w.dealt) return false;
-    more = list.w.asked > 0, have_nxt = false;
+    more = list.w.asked > 0;
     cur = list.segment(p, id);
     return true;
   }
@@ -529,6 +553,12 @@ struct AttnWalk {
     return true;
   }
 };
+
+__device__ __forceinline__ float2 ld_cluster_f2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
 
 // cp_async16 that writes zeros instead where `ok` is false.
 __device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool ok) {
@@ -664,23 +694,80 @@ struct AttnTmaLoader {
 
 constexpr int kJoinAlone = 32;  // parts that one warp joins
 
-// Where the sums of an item go whose part of segment `s` ends with its i-th tile:
-// the output, or row `part` of the parts.
+// Where the sums of an item go whose part of segment `s` ends with its i-th tile.
 struct AttnPlace {
-  bool whole;
-  int64_t part;
+  bool whole;   // to the output
+  float* sums;  // else here, rows of `pitch`
+  float2* ml;
+  int pitch;
 };
+// Direct: the warp's ring (rows of DP + 4 floats: fragment rows then fall into
+// different banks) and its row of `s_ml`.
+template <int DP>
 __device__ __forceinline__ AttnPlace attn_place(const AttnParams& p, const AttnList& list, const AttnSegment& s,
-                                                const AttnCursor& at, int i, bool begun, bool done) {
+                                                const AttnCursor& at, int i, bool begun, bool done, float* ring,
+                                                float2* s_ml) {
   AttnPlace o;
+  if (p.direct) {
+    __syncwarp();  // the last tile has been read
+    o.whole = false, o.sums = ring, o.ml = s_ml, o.pitch = DP + 4;
+    return o;
+  }
   o.whole = begun && done;
-  o.part = (s.id * 2ll + (begun ? 1 : 0)) * p.block_heads;
+  const int64_t part = (s.id * 2ll + (begun ? 1 : 0)) * p.block_heads;
+  o.sums = p.part_o + part * p.c.dim, o.ml = p.part_ml + part, o.pitch = p.c.dim;
   if (begun && !done && (threadIdx.x & 31) == 0) {  // it goes on in the next segments, to the one of its last tile
     const int segments = list.holder(s.begin + i + (at.r.t1 - 1 - at.tile)) - s.id + 1;
     const int far = segments > kJoinAlone, n = atomicAdd(&p.work->cuts[far], 1);
     p.cut[far ? p.cut_room - 1 - n : n] = make_int4(at.row, at.kv * p.blocks + at.blk, s.id, segments);
   }
   return o;
+}
+
+// Direct: the cluster's warps' sums of its item, added in the order of CTAs and
+// warps; a thread takes four elements of a head.  `rings`: of this CTA, `pitch`
+// bytes apart; s_ml[warp][head].
+template <typename T, int WARPS, int HEADS, int DP>
+__device__ __forceinline__ void attn_gather(const AttnParams& p, const unsigned char* rings, int pitch,
+                                            const float2 (*s_ml)[HEADS]) {
+  cluster_sync();
+  const int item = blockIdx.x / p.direct, rank = blockIdx.x - item * p.direct, per_row = p.c.kv_heads * p.blocks;
+  const int row = item / per_row, kv = (item - row * per_row) / p.blocks, blk = item - row * per_row - kv * p.blocks;
+  const int h0 = blk * p.block_heads, nh = min(p.block_heads, p.group - h0), quads = p.c.dim / 4;
+  for (int t = rank * WARPS * 32 + threadIdx.x; t < nh * quads; t += p.direct * WARPS * 32) {
+    const int h = t / quads, e = (t - h * quads) * 4;
+    float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int c = 0; c < p.direct; ++c) {
+      const uint32_t ml0 = cluster_map(smem_u32(&s_ml[0][h]), c);
+      const uint32_t o0 = cluster_map(smem_u32(rings), c) + (h * (DP + 4) + e) * 4;
+      float2 ml[WARPS];
+      float4 v[WARPS];
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) {
+        ml[w] = ld_cluster_f2(ml0 + w * HEADS * 8);
+        v[w] = ld_cluster_f4(o0 + w * pitch);
+      }
+      float top = m;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) top = fmaxf(top, ml[w].x);
+      const float base = top == -INFINITY ? 0.f : top, keep = exp2_fast(m - base);
+      m = top, l *= keep;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) o[k] *= keep;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) {
+        if (ml[w].x == -INFINITY && ml[w].y == 0.f) continue;  // a warp without tiles, whose ring holds no sums
+        const float f = exp2_fast(ml[w].x - base);
+        l += ml[w].y * f;
+        o[0] += v[w].x * f, o[1] += v[w].y * f, o[2] += v[w].z * f, o[3] += v[w].w * f;
+      }
+    }
+    const float f = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // NaN stays
+    T* out = (T*)p.out + (((int64_t)row * p.c.kv_heads + kv) * p.group + h0 + h) * p.c.dim + e;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) out[k] = Chunk<T>::put(o[k] * f);
+  }
+  cluster_sync();  // no CTA leaves while another reads it
 }
 
 template <int DP, int H>
@@ -704,19 +791,23 @@ __global__ void __launch_bounds__(AttnSimtCfg<DP, H>::kWarps * 32, 1) attn_simt_
   using Tile = AttnTileCfg<4, DP>;
   constexpr int N = Chunk<T>::N, E = DP / 32;
   extern __shared__ __align__(128) unsigned char attn_smem[];
+  __shared__ float2 s_ml[Cfg::kWarps][H];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   unsigned char* mine = attn_smem + warp * Cfg::kWarpBytes;
   float* sq = reinterpret_cast<float*>(mine + Cfg::kStages * Tile::kStageBytes);  // [H][DP]
   float* sp = sq + H * DP;                                                        // [16][H]
   if (p.c.dim < DP)  // columns that no copy fills
     for (int i = lane; i < Cfg::kWarpBytes / 16; i += 32) reinterpret_cast<uint4*>(mine)[i] = make_uint4(0, 0, 0, 0);
+  if (lane < H) s_ml[warp][lane] = make_float2(-INFINITY, 0.f);
   __syncwarp();
   griddep_wait();
   griddep_launch();
   AttnWalk walk;
-  if (!walk.start(p)) return;
+  const bool busy = walk.start(p);
+  if (!busy && !p.direct) return;
   AttnCopyLoader<4, DP> load;
-  load.start(p, walk.cur);
+  load.left = 0, load.page = -1;
+  if (busy) load.start(p, walk.cur);
   const uint32_t ring = smem_u32(mine);
   auto refill = [&](int to) {
     if (walk.look_ahead(p, load.left)) load.start(p, walk.nxt);
@@ -729,7 +820,7 @@ __global__ void __launch_bounds__(AttnSimtCfg<DP, H>::kWarps * 32, 1) attn_simt_
   bool begun = at.tile == at.r.t0, fresh = true;
   float m[H], l[H], o[H][E];
   int stage = 0;
-  for (int i = 0;;) {
+  for (int i = 0; busy;) {
     const int kv = at.kv, h0 = at.blk * p.block_heads, nh = min(p.block_heads, p.group - h0);
     if (fresh) {
       const T* q = (const T*)p.q + at.row * p.q_row + (kv * p.group + h0) * p.q_head;
@@ -805,16 +896,16 @@ __global__ void __launch_bounds__(AttnSimtCfg<DP, H>::kWarps * 32, 1) attn_simt_
 
     const bool done = at.tile + 1 == at.r.t1, end = i + 1 == walk.cur.count;
     if (done || end) {
-      const AttnPlace to = attn_place(p, walk.list, walk.cur, at, i, begun, done);
+      const AttnPlace to = attn_place<DP>(p, walk.list, walk.cur, at, i, begun, done, reinterpret_cast<float*>(mine), s_ml[warp]);
 #pragma unroll
       for (int h = 0; h < H; ++h) {
 #pragma unroll
         for (int d = 16; d; d >>= 1) l[h] += __shfl_xor_sync(0xffffffffu, l[h], d);
         if (h >= nh) continue;
         const float f = to.whole ? (l[h] > 0.f ? 1.f / l[h] : (l[h] == 0.f ? 0.f : l[h])) : 1.f;  // NaN stays
-        if (!to.whole && lane == 0) p.part_ml[to.part + h] = make_float2(m[h], l[h]);
+        if (!to.whole && lane == 0) to.ml[h] = make_float2(m[h], l[h]);
         float* out = to.whole ? (float*)p.out + (((int64_t)at.row * p.c.kv_heads + kv) * p.group + h0 + h) * p.c.dim
-                              : p.part_o + (to.part + h) * p.c.dim;
+                              : to.sums + h * to.pitch;
 #pragma unroll
         for (int e = 0; e < E; e += 2) {
           const int d = e * 32 + 2 * lane;
@@ -825,13 +916,14 @@ __global__ void __launch_bounds__(AttnSimtCfg<DP, H>::kWarps * 32, 1) attn_simt_
     }
     __syncwarp();
     if (end) {
-      if (!walk.step()) return;
+      if (!walk.step()) break;
       at = walk.cur.at, i = 0;
       begun = at.tile == at.r.t0;
     } else {
       at.next(p), ++i;
     }
   }
+  if (p.direct) attn_gather<float, Cfg::kWarps, H, DP>(p, attn_smem, Cfg::kWarpBytes, s_ml);
 }
 
 template <int DP, int NT>
@@ -868,7 +960,9 @@ __global__ void __launch_bounds__(AttnMmaCfg<DP, NT>::kWarps * 32, 1)
   __shared__ uint64_t bars[TMA ? Cfg::kWarps * STAGES : 1];
   __shared__ int abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  unsigned char* mine = attn_smem + ((1024 - (smem_u32(attn_smem) & 1023)) & 1023) + warp * Cfg::kWarpBytes;
+  __shared__ float2 s_ml[Cfg::kWarps][Cfg::kHeads];
+  unsigned char* rings = attn_smem + ((1024 - (smem_u32(attn_smem) & 1023)) & 1023);
+  unsigned char* mine = rings + warp * Cfg::kWarpBytes;
   const uint32_t ring = smem_u32(mine), sq = ring + STAGES * Tile::kStageBytes;
   uint64_t* bar = bars + (TMA ? warp * STAGES : 0);
   if constexpr (TMA) {
@@ -882,15 +976,46 @@ __global__ void __launch_bounds__(AttnMmaCfg<DP, NT>::kWarps * 32, 1)
   } else if (p.c.dim < DP) {  // columns that no copy fills
     for (int i = lane; i < STAGES * Tile::kStageBytes / 16; i += 32) reinterpret_cast<uint4*>(mine)[i] = make_uint4(0, 0, 0, 0);
   }
+  if (lane < Cfg::kHeads) s_ml[warp][lane] = make_float2(-INFINITY, 0.f);
   if constexpr (TMA) __syncthreads();  // abort_flag
   __syncwarp();
   griddep_wait();
   griddep_launch();
   AttnWalk walk;
-  if (!walk.start(p)) return;
+  const bool busy = walk.start(p);
+  if (!busy && !p.direct) return;
+
+  // the item's queries: B fragments in registers, or rows in shared memory (cp.async)
+  uint32_t qf[Cfg::kQShared ? 1 : NT][Cfg::kQShared ? 1 : KS][2];
+  auto load_q = [&](const AttnCursor& c) {
+    const int h0 = c.blk * p.block_heads, nh = min(p.block_heads, p.group - h0);
+    const T* q = (const T*)p.q + c.row * p.q_row + (c.kv * p.group + h0) * p.q_head;
+    if constexpr (Cfg::kQShared) {
+      for (int j = lane; j < Cfg::kHeads * Tile::kChunks; j += 32) {
+        const int h = j / Tile::kChunks, c = j % Tile::kChunks;
+        const bool ok = h < nh && c * 8 < p.c.dim;
+        cp_async16_or_zero(sq + h * (DP * 2) + ((c ^ (h & 7)) << 4), ok ? q + h * p.q_head + c * 8 : q, ok);
+      }
+      cp_async_commit();
+    } else {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const int h = nt * 8 + (lane >> 2);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int d = ks * 16 + j * 8 + (lane & 3) * 2;
+            qf[nt][ks][j] = h < nh && d < p.c.dim ? *reinterpret_cast<const uint32_t*>(q + h * p.q_head + d) : 0u;
+          }
+      }
+    }
+  };
+  if (busy) load_q(walk.cur.at);  // on their way while the first pages are looked up
 
   std::conditional_t<TMA, AttnTmaLoader<DP>, AttnCopyLoader<2, DP>> load;
-  load.start(p, walk.cur);
+  load.left = 0, load.page = -1;
+  if (busy) load.start(p, walk.cur);
   int flying = 0;  // TMA: tiles whose copies have not been waited for
   auto refill = [&](int to) {
     if (walk.look_ahead(p, load.left)) load.start(p, walk.nxt);
@@ -916,35 +1041,13 @@ __global__ void __launch_bounds__(AttnMmaCfg<DP, NT>::kWarps * 32, 1)
   }
   AttnCursor at = walk.cur.at;
   bool begun = at.tile == at.r.t0, fresh = true;
-  uint32_t qf[Cfg::kQShared ? 1 : NT][Cfg::kQShared ? 1 : KS][2];
   float m[NT][2], l[NT][2], o[NT][KS][4];
   int stage = 0;
   uint32_t parity = 0;
-  for (int i = 0;;) {
+  for (int i = 0; busy;) {
     if (fresh) {
-      const int h0 = at.blk * p.block_heads, nh = min(p.block_heads, p.group - h0);
-      const T* q = (const T*)p.q + at.row * p.q_row + (at.kv * p.group + h0) * p.q_head;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        if constexpr (Cfg::kQShared) {
-          for (int j = lane; j < 8 * Tile::kChunks; j += 32) {
-            const int h = nt * 8 + j / Tile::kChunks, c = j % Tile::kChunks;
-            uint4 u = make_uint4(0, 0, 0, 0);
-            if (h < nh && c * 8 < p.c.dim) u = *reinterpret_cast<const uint4*>(q + h * p.q_head + c * 8);
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(sq + h * (DP * 2) + ((c ^ (h & 7)) << 4)),
-                         "r"(u.x), "r"(u.y), "r"(u.z), "r"(u.w)
-                         : "memory");
-          }
-        } else {
-          const int h = nt * 8 + (lane >> 2);
-#pragma unroll
-          for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              const int d = ks * 16 + j * 8 + (lane & 3) * 2;
-              qf[nt][ks][j] = h < nh && d < p.c.dim ? *reinterpret_cast<const uint32_t*>(q + h * p.q_head + d) : 0u;
-            }
-        }
 #pragma unroll
         for (int j = 0; j < 2; ++j) m[nt][j] = -INFINITY, l[nt][j] = 0.f;
 #pragma unroll
@@ -952,7 +1055,6 @@ __global__ void __launch_bounds__(AttnMmaCfg<DP, NT>::kWarps * 32, 1)
 #pragma unroll
           for (int j = 0; j < 4; ++j) o[nt][mt][j] = 0.f;
       }
-      fresh = false;
     }
     if constexpr (TMA) {
       refill(stage == 0 ? STAGES - 1 : stage - 1);  // read in the last round: free again
@@ -962,14 +1064,23 @@ __global__ void __launch_bounds__(AttnMmaCfg<DP, NT>::kWarps * 32, 1)
           mbar_drain(bar + stage, parity);
           if (++stage == STAGES) stage = 0, parity ^= 1;
         }
-        return;
+        break;
       }
       --flying;
+      if (Cfg::kQShared && fresh) {
+        cp_async_wait<0>();
+        __syncwarp();
+      }
     } else {
-      cp_async_wait<STAGES - 2>();
+      // an item's queries are a group of their own among the tiles'; the first of its tiles waits for all
+      if (Cfg::kQShared && fresh)
+        cp_async_wait<0>();
+      else
+        cp_async_wait<STAGES - 2>();
       __syncwarp();
       refill(stage == 0 ? STAGES - 1 : stage - 1);
     }
+    fresh = false;
     const uint32_t base = ring + stage * Tile::kStageBytes;
     const bool inner = at.tile * kAttnTile >= at.r.lo && (at.tile + 1) * kAttnTile <= at.r.n;
     if (TMA && !inner) {
@@ -1061,10 +1172,19 @@ __global__ void __launch_bounds__(AttnMmaCfg<DP, NT>::kWarps * 32, 1)
     if (++stage == STAGES) stage = 0, parity ^= 1;
 
     const bool done = at.tile + 1 == at.r.t1, end = i + 1 == walk.cur.count;
+    const AttnCursor was = at;
+    if (!end) {
+      at.next(p);
+      if (done) {  // the next item's queries, on their way while this one's sums are written
+        __syncwarp();
+        load_q(at);
+      }
+    }
     if (done || end) {
-      const AttnPlace to = attn_place(p, walk.list, walk.cur, at, i, begun, done);
-      const int h0 = at.blk * p.block_heads, nh = min(p.block_heads, p.group - h0);
-      const int64_t head0 = ((int64_t)at.row * p.c.kv_heads + at.kv) * p.group + h0;
+      const AttnPlace to = attn_place<DP>(p, walk.list, walk.cur, was, i, begun, done, reinterpret_cast<float*>(mine),
+                                          s_ml[warp]);
+      const int h0 = was.blk * p.block_heads, nh = min(p.block_heads, p.group - h0);
+      const int64_t head0 = ((int64_t)was.row * p.c.kv_heads + was.kv) * p.group + h0;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -1076,9 +1196,9 @@ __global__ void __launch_bounds__(AttnMmaCfg<DP, NT>::kWarps * 32, 1)
           const int h = nt * 8 + (lane & 3) * 2 + j;
           if (h >= nh) continue;
           const float f = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);  // NaN stays
-          if (!to.whole && lane < 4) p.part_ml[to.part + h] = make_float2(m[nt][j], sum);
+          if (!to.whole && lane < 4) to.ml[h] = make_float2(m[nt][j], sum);
           T* out = (T*)p.out + (head0 + h) * p.c.dim;
-          float* part = p.part_o + (to.part + h) * p.c.dim;
+          float* part = to.sums + h * to.pitch;
 #pragma unroll
           for (int mt = 0; mt < KS; ++mt)
 #pragma unroll
@@ -1095,14 +1215,15 @@ __global__ void __launch_bounds__(AttnMmaCfg<DP, NT>::kWarps * 32, 1)
       begun = true, fresh = true;
     }
     __syncwarp();
+    ++i;
     if (end) {
-      if (!walk.step()) return;
+      if (!walk.step()) break;
       at = walk.cur.at, i = 0;
       begun = at.tile == at.r.t0;
-    } else {
-      at.next(p), ++i;
+      load_q(at);
     }
   }
+  if (p.direct) attn_gather<T, Cfg::kWarps, Cfg::kHeads, DP>(p, rings, Cfg::kWarpBytes, s_ml);
 }
 
 // Joins the parts of the items that segments cut.  Of an item of up to 32 parts a

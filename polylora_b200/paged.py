@@ -228,12 +228,13 @@ def paged_attention(
         raise ValueError("out must be a contiguous tensor of q's shape, dtype and device")
     q, qs, q_ptr = _heads(q)
     code = dtype_code(dtype)
-    ws_bytes = _native.load().plora_paged_attention_workspace(rows, heads, kv_heads, dim, code)
-    ws = lens.new_empty(max(ws_bytes, 256) // 4)
+    max_pages = page_table.shape[1]
+    ws_bytes = _native.load().plora_paged_attention_workspace(rows, heads, kv_heads, dim, size, max_pages, window, code)
+    ws = lens.new_empty(ws_bytes // 4) if ws_bytes else None
     _call(
         dev, "plora_paged_attention",
         q_ptr, qs[0], qs[1], k_cache.data_ptr(), v_cache.data_ptr(), k_page, v_page, page_table.data_ptr(),
         table_row, lens.data_ptr(), out.data_ptr(), dim**-0.5 if scale is None else scale, window, rows, heads,
-        kv_heads, dim, size, pages, page_table.shape[1], code, ws.data_ptr(), ws_bytes,
+        kv_heads, dim, size, pages, max_pages, code, ws.data_ptr() if ws_bytes else 0, ws_bytes,
     )
     return out

@@ -225,6 +225,17 @@ ATTEND = [
     ([513, 20], 4, 2, 8, 3, BF, 0),
     ([31] * 300, 2, 1, 64, 16, BF, 0),         # more rows than threads of a CTA
     (list(range(700)), 4, 2, 32, 8, FH, 0),
+    # few short rows: clusters of one to eight CTAs, warps without a tile, empty rows
+    ([17], 4, 2, 128, 16, BF, 0),
+    ([130, 0, 129], 4, 1, 128, 16, FH, 0),
+    ([2000, 1, 900], 8, 2, 64, 16, BF, 0),
+    ([1500, 0, 333, 12], 16, 1, 256, 16, BF, 0),
+    ([1500, 200], 24, 1, 128, 8, BF, 0),
+    ([600, 31], 3, 1, 128, 16, F32, 0),
+    ([300, 0], 2, 1, 256, 16, F32, 0),
+    ([600, 31, 5], 8, 1, 64, 4, F32, 50),
+    ([40000, 20000], 4, 2, 64, 16, FH, 0),   # long rows: segments asked for
+    ([50000, 33], 2, 1, 128, 16, F32, 0),
 ]
 
 

@@ -67,12 +67,15 @@ def test_attention_arguments_rejected_before_cuda(native):
     for kw in (dict(heads=0), dict(window=-1), dict(q=None), dict(lens=None), dict(out=None), dict(out=D + 8),
                dict(qs=(1024, 4)), dict(ws=D + 16)):
         assert _attend(lib, native, **kw) == native.ERR_INVALID_ARGUMENT, kw
-    need = lib.plora_paged_attention_workspace(2, 16, 4, 64, native.DTYPE_BF16)
-    assert need > 0
-    assert _attend(lib, native, wb=need - 1) == native.ERR_WORKSPACE
-    assert _attend(lib, native, ws=None) == native.ERR_WORKSPACE
+    assert lib.plora_paged_attention_workspace(2, 16, 4, 64, 16, 4, 0, native.DTYPE_BF16) == 0  # 64 tokens
+    need = lib.plora_paged_attention_workspace(2, 16, 4, 64, 16, 4000, 0, native.DTYPE_BF16)
+    assert need > 0 and lib.plora_paged_attention_workspace(2, 16, 4, 64, 16, 4000, 100, native.DTYPE_BF16) == 0
+    assert _attend(lib, native, width=4000, ts=4000, wb=need - 1) == native.ERR_WORKSPACE
+    assert _attend(lib, native, width=4000, ts=4000, ws=None, wb=need) == native.ERR_WORKSPACE
     assert _attend(lib, native, rows=0) == native.OK
-    for bad in ((2, 16, 5, 64, 2), (2, 0, 4, 64, 2), (2, 16, 4, 65, 2), (2, 16, 4, 512, 2), (2, 16, 4, 64, 7), (-1, 16, 4, 64, 2)):
+    for bad in ((2, 16, 5, 64, 16, 4000, 0, 2), (2, 0, 4, 64, 16, 4000, 0, 2), (2, 16, 4, 65, 16, 4000, 0, 2),
+                (2, 16, 4, 512, 16, 4000, 0, 2), (2, 16, 4, 64, 16, 4000, 0, 7), (-1, 16, 4, 64, 16, 4000, 0, 2),
+                (2, 16, 4, 64, 0, 4000, 0, 2), (2, 16, 4, 64, 16, 4000, -1, 2), (2, 16, 4, 64, 1 << 20, 4000, 0, 2)):
         assert lib.plora_paged_attention_workspace(*bad) == 0
 
 
