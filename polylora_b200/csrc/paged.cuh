@@ -554,6 +554,17 @@ struct AttnWalk {
   }
 };
 
+// Two fused products at once.
+__device__ __forceinline__ float2 fma2(const float2& a, const float2& b, const float2& c) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+
 __device__ __forceinline__ float2 ld_cluster_f2(uint32_t addr) {
   float2 v;
   asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
@@ -725,47 +736,65 @@ __device__ __forceinline__ AttnPlace attn_place(const AttnParams& p, const AttnL
 }
 
 // Direct: the cluster's warps' sums of its item, added in the order of CTAs and
-// warps; a thread takes four elements of a head.  `rings`: of this CTA, `pitch`
-// bytes apart; s_ml[warp][head].
+// warps.  Every CTA works out the parts' weights for itself, and takes a share of the
+// elements, four of a head a thread.  `rings`: of this CTA, `pitch` bytes apart;
+// s_ml[warp][head].
+constexpr int kAttnClusterCtas = 8;
 template <typename T, int WARPS, int HEADS, int DP>
 __device__ __forceinline__ void attn_gather(const AttnParams& p, const unsigned char* rings, int pitch,
                                             const float2 (*s_ml)[HEADS]) {
+  __shared__ float s_f[kAttnClusterCtas * WARPS][HEADS];  // of a part: weight / sum of all
   cluster_sync();
   const int item = blockIdx.x / p.direct, rank = blockIdx.x - item * p.direct, per_row = p.c.kv_heads * p.blocks;
   const int row = item / per_row, kv = (item - row * per_row) / p.blocks, blk = item - row * per_row - kv * p.blocks;
   const int h0 = blk * p.block_heads, nh = min(p.block_heads, p.group - h0), quads = p.c.dim / 4;
+  const int parts = p.direct * WARPS, lane = threadIdx.x & 31;
+  for (int h = threadIdx.x >> 5; h < nh; h += WARPS) {
+    constexpr int PER = (kAttnClusterCtas * WARPS + 31) / 32;
+    float2 ml[PER];
+    float top = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      const int i = lane + 32 * k;
+      ml[k] = make_float2(-INFINITY, 0.f);
+      if (i < parts) ml[k] = ld_cluster_f2(cluster_map(smem_u32(&s_ml[i % WARPS][h]), i / WARPS));
+      top = fmaxf(top, ml[k].x);
+    }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      ml[k].x = exp2_fast(ml[k].x - base);
+      sum += ml[k].y * ml[k].x;
+    }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);  // NaN stays
+#pragma unroll
+    for (int k = 0; k < PER; ++k)
+      if (lane + 32 * k < parts) s_f[lane + 32 * k][h] = ml[k].x * inv;
+  }
+  __syncthreads();
   for (int t = rank * WARPS * 32 + threadIdx.x; t < nh * quads; t += p.direct * WARPS * 32) {
     const int h = t / quads, e = (t - h * quads) * 4;
-    float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+    float o[4] = {0.f, 0.f, 0.f, 0.f};
+    const uint32_t own = smem_u32(rings) + (h * (DP + 4) + e) * 4;
     for (int c = 0; c < p.direct; ++c) {
-      const uint32_t ml0 = cluster_map(smem_u32(&s_ml[0][h]), c);
-      const uint32_t o0 = cluster_map(smem_u32(rings), c) + (h * (DP + 4) + e) * 4;
-      float2 ml[WARPS];
+      const uint32_t from = cluster_map(own, c);
       float4 v[WARPS];
 #pragma unroll
-      for (int w = 0; w < WARPS; ++w) {
-        ml[w] = ld_cluster_f2(ml0 + w * HEADS * 8);
-        v[w] = ld_cluster_f4(o0 + w * pitch);
-      }
-      float top = m;
-#pragma unroll
-      for (int w = 0; w < WARPS; ++w) top = fmaxf(top, ml[w].x);
-      const float base = top == -INFINITY ? 0.f : top, keep = exp2_fast(m - base);
-      m = top, l *= keep;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) o[k] *= keep;
+      for (int w = 0; w < WARPS; ++w) v[w] = ld_cluster_f4(from + w * pitch);
 #pragma unroll
       for (int w = 0; w < WARPS; ++w) {
-        if (ml[w].x == -INFINITY && ml[w].y == 0.f) continue;  // a warp without tiles, whose ring holds no sums
-        const float f = exp2_fast(ml[w].x - base);
-        l += ml[w].y * f;
+        const float f = s_f[c * WARPS + w][h];
+        if (f == 0.f) continue;  // a warp without tiles, whose ring holds no sums
         o[0] += v[w].x * f, o[1] += v[w].y * f, o[2] += v[w].z * f, o[3] += v[w].w * f;
       }
     }
-    const float f = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // NaN stays
     T* out = (T*)p.out + (((int64_t)row * p.c.kv_heads + kv) * p.group + h0 + h) * p.c.dim + e;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) out[k] = Chunk<T>::put(o[k] * f);
+    for (int k = 0; k < 4; ++k) out[k] = Chunk<T>::put(o[k]);
   }
   cluster_sync();  // no CTA leaves while another reads it
 }
@@ -774,28 +803,29 @@ template <int DP, int H>
 struct AttnSimtCfg {
   using Tile = AttnTileCfg<4, DP>;
   static constexpr int kHeads = H;  // query heads of a block
-  static constexpr int kStages = DP == 256 ? 2 : 3;
-  static constexpr int kWarps = DP == 256 ? 3 : (DP == 128 ? 4 : 8);
-  static constexpr int kQBytes = kHeads * DP * 4, kPBytes = (kAttnTile * kHeads * 4 + 127) & ~127;
+  static constexpr int kStages = DP == 64 ? 3 : 2;
+  static constexpr int kWarps = DP == 256 ? 3 : (DP == 128 ? 6 : 8);
+  static constexpr int kQBytes = kHeads * DP * 4, kPBytes = kAttnTile * kHeads * 8;
   static constexpr int kWarpBytes = kStages * Tile::kStageBytes + kQBytes + kPBytes;
   static constexpr int kSmemBytes = kWarps * kWarpBytes;
 };
 
 // CUDA-core attention for fp32 (TF32 products would lose 13 bits of it).
 // Scores: lanes l and l + 16 take token l & 15, each half of the head's
-// elements.  Sums: a lane owns DP / 32 elements of all heads.
+// elements.  Sums: a lane owns DP / 32 elements of all heads.  Products come in
+// pairs (fma.rn.f32x2): issue slots are the bound, not memory.
 template <int DP, int H>
 __global__ void __launch_bounds__(AttnSimtCfg<DP, H>::kWarps * 32, 1) attn_simt_kernel(const AttnParams p) {
   using T = float;
   using Cfg = AttnSimtCfg<DP, H>;
   using Tile = AttnTileCfg<4, DP>;
-  constexpr int N = Chunk<T>::N, E = DP / 32;
+  constexpr int N = 4, E = DP / 32, W = E < 4 ? E : 4;  // elements of a lane, W in a run
   extern __shared__ __align__(128) unsigned char attn_smem[];
   __shared__ float2 s_ml[Cfg::kWarps][H];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   unsigned char* mine = attn_smem + warp * Cfg::kWarpBytes;
   float* sq = reinterpret_cast<float*>(mine + Cfg::kStages * Tile::kStageBytes);  // [H][DP]
-  float* sp = sq + H * DP;                                                        // [16][H]
+  float2* sp = reinterpret_cast<float2*>(sq + H * DP);                            // [16][H]: twice the same
   if (p.c.dim < DP)  // columns that no copy fills
     for (int i = lane; i < Cfg::kWarpBytes / 16; i += 32) reinterpret_cast<uint4*>(mine)[i] = make_uint4(0, 0, 0, 0);
   if (lane < H) s_ml[warp][lane] = make_float2(-INFINITY, 0.f);
@@ -805,6 +835,17 @@ __global__ void __launch_bounds__(AttnSimtCfg<DP, H>::kWarps * 32, 1) attn_simt_
   AttnWalk walk;
   const bool busy = walk.start(p);
   if (!busy && !p.direct) return;
+  auto load_q = [&](const AttnCursor& c) {
+    const int first = c.blk * p.block_heads, n = min(p.block_heads, p.group - first), quads = p.c.dim / 4;
+    const float* q = (const float*)p.q + c.row * p.q_row + (c.kv * p.group + first) * p.q_head;
+    for (int j = lane; j < H * (DP / 4); j += 32) {
+      const int h = j / (DP / 4), e = j % (DP / 4);
+      const bool ok = h < n && e < quads;
+      cp_async16_or_zero(smem_u32(sq + h * DP + e * 4), ok ? q + h * p.q_head + e * 4 : q, ok);
+    }
+    cp_async_commit();
+  };
+  if (busy) load_q(walk.cur.at);  // on their way while the first pages are looked up
   AttnCopyLoader<4, DP> load;
   load.left = 0, load.page = -1;
   if (busy) load.start(p, walk.cur);
@@ -818,51 +859,51 @@ __global__ void __launch_bounds__(AttnSimtCfg<DP, H>::kWarps * 32, 1) attn_simt_
 
   AttnCursor at = walk.cur.at;
   bool begun = at.tile == at.r.t0, fresh = true;
-  float m[H], l[H], o[H][E];
+  float m[H], l[H];
+  float2 o[H][E / 2];
   int stage = 0;
   for (int i = 0; busy;) {
     const int kv = at.kv, h0 = at.blk * p.block_heads, nh = min(p.block_heads, p.group - h0);
     if (fresh) {
-      const T* q = (const T*)p.q + at.row * p.q_row + (kv * p.group + h0) * p.q_head;
-      for (int h = 0; h < H; ++h)
-        for (int d = lane; d < p.c.dim; d += 32) sq[h * DP + d] = h < nh ? Chunk<T>::get(q[h * p.q_head + d]) * p.scale_log2 : 0.f;
 #pragma unroll
       for (int h = 0; h < H; ++h) {
         m[h] = -INFINITY, l[h] = 0.f;
 #pragma unroll
-        for (int e = 0; e < E; ++e) o[h][e] = 0.f;
+        for (int e = 0; e < E / 2; ++e) o[h][e] = make_float2(0.f, 0.f);
       }
-      fresh = false;
     }
-    cp_async_wait<Cfg::kStages - 2>();
+    // an item's queries are a group of copies of their own; its first tile waits for all
+    if (fresh)
+      cp_async_wait<0>();
+    else
+      cp_async_wait<Cfg::kStages - 2>();
+    fresh = false;
     __syncwarp();
     // the stage read in the last round is free again
     refill(stage == 0 ? Cfg::kStages - 1 : stage - 1);
 
     const unsigned char* ks = mine + stage * Tile::kStageBytes;
     const int tok = lane & 15, half = lane >> 4;
-    float acc[H];
+    float2 acc[H];
 #pragma unroll
-    for (int h = 0; h < H; ++h) acc[h] = 0.f;
+    for (int h = 0; h < H; ++h) acc[h] = make_float2(0.f, 0.f);
 #pragma unroll 4
-    for (int c = half * (Tile::kChunks / 2); c < (half + 1) * (Tile::kChunks / 2); ++c) {
-      float kf[N];
-      Chunk<T>::load(*reinterpret_cast<const uint4*>(ks + Tile::offset(tok, c)), kf);
+    for (int c = half * (p.c.dim / 8); c < (half + 1) * (p.c.dim / 8); ++c) {
+      const float4 kf = *reinterpret_cast<const float4*>(ks + Tile::offset(tok, c));
 #pragma unroll
       for (int h = 0; h < H; ++h) {
-#pragma unroll
-        for (int j = 0; j < N; j += 4) {
-          const float4 qv = *reinterpret_cast<const float4*>(sq + h * DP + c * N + j);
-          acc[h] = fmaf(qv.x, kf[j], fmaf(qv.y, kf[j + 1], fmaf(qv.z, kf[j + 2], fmaf(qv.w, kf[j + 3], acc[h]))));
-        }
+        const float4 qv = *reinterpret_cast<const float4*>(sq + h * DP + c * N);
+        acc[h] = fma2(make_float2(qv.x, qv.y), make_float2(kf.x, kf.y), acc[h]);
+        acc[h] = fma2(make_float2(qv.z, qv.w), make_float2(kf.z, kf.w), acc[h]);
       }
     }
     const int at_pos = at.tile * kAttnTile + tok;
     const bool live = at_pos >= at.r.lo && at_pos < at.r.n;
 #pragma unroll
     for (int h = 0; h < H; ++h) {
-      float x = acc[h] + __shfl_xor_sync(0xffffffffu, acc[h], 16);
-      x = live ? x : -INFINITY;
+      const float half_sum = acc[h].x + acc[h].y;
+      float x = half_sum + __shfl_xor_sync(0xffffffffu, half_sum, 16);
+      x = live ? x * p.scale_log2 : -INFINITY;
       float mx = x;
 #pragma unroll
       for (int d = 8; d; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
@@ -870,26 +911,30 @@ __global__ void __launch_bounds__(AttnSimtCfg<DP, H>::kWarps * 32, 1) attn_simt_
       const float keep = exp2_fast(m[h] - base), pr = exp2_fast(x - base);
       m[h] = m2;
       l[h] = l[h] * keep + (half ? 0.f : pr);  // per lane; added over the lanes at the item's end
-      if (half == 0) sp[tok * H + h] = pr;
+      if (half == 0) sp[tok * H + h] = make_float2(pr, pr);
 #pragma unroll
-      for (int e = 0; e < E; ++e) o[h][e] *= keep;
+      for (int e = 0; e < E / 2; ++e) o[h][e].x *= keep, o[h][e].y *= keep;
     }
     __syncwarp();
     const unsigned char* vs = ks + Tile::kTileBytes;
-#pragma unroll 2
+#pragma unroll 4
     for (int t = 0; t < kAttnTile; ++t) {
-      float vf[E];
+      float2 vf[E / 2];
 #pragma unroll
-      for (int e = 0; e < E; e += 2) {  // elements 2 lane, 2 lane + 1 of every 64
-        const int d = e * 32 + 2 * lane;
-        const T* src = reinterpret_cast<const T*>(vs + Tile::offset(t, d / N)) + d % N;
-        vf[e] = Chunk<T>::get(src[0]), vf[e + 1] = Chunk<T>::get(src[1]);
+      for (int e = 0; e < E; e += W) {  // elements W lane .. of every 32 W
+        const unsigned char* from = vs + Tile::offset(t, (e * 32 + W * lane) / N) + (W * lane) % N * 4;
+        if constexpr (W == 4) {
+          const float4 v = *reinterpret_cast<const float4*>(from);
+          vf[e / 2] = make_float2(v.x, v.y), vf[e / 2 + 1] = make_float2(v.z, v.w);
+        } else {
+          vf[e / 2] = *reinterpret_cast<const float2*>(from);
+        }
       }
 #pragma unroll
       for (int h = 0; h < H; ++h) {
-        const float pr = sp[t * H + h];
+        const float2 pr = sp[t * H + h];
 #pragma unroll
-        for (int e = 0; e < E; ++e) o[h][e] = fmaf(pr, vf[e], o[h][e]);
+        for (int e = 0; e < E / 2; ++e) o[h][e] = fma2(pr, vf[e], o[h][e]);
       }
     }
     stage = stage + 1 == Cfg::kStages ? 0 : stage + 1;
@@ -908,8 +953,8 @@ __global__ void __launch_bounds__(AttnSimtCfg<DP, H>::kWarps * 32, 1) attn_simt_
                               : to.sums + h * to.pitch;
 #pragma unroll
         for (int e = 0; e < E; e += 2) {
-          const int d = e * 32 + 2 * lane;
-          if (d < p.c.dim) *reinterpret_cast<float2*>(out + d) = make_float2(o[h][e] * f, o[h][e + 1] * f);
+          const int d = e / W * (32 * W) + W * lane + e % W;
+          if (d < p.c.dim) *reinterpret_cast<float2*>(out + d) = make_float2(o[h][e / 2].x * f, o[h][e / 2].y * f);
         }
       }
       begun = true, fresh = true;
@@ -919,8 +964,10 @@ __global__ void __launch_bounds__(AttnSimtCfg<DP, H>::kWarps * 32, 1) attn_simt_
       if (!walk.step()) break;
       at = walk.cur.at, i = 0;
       begun = at.tile == at.r.t0;
+      load_q(at);
     } else {
       at.next(p), ++i;
+      if (done) load_q(at);
     }
   }
   if (p.direct) attn_gather<float, Cfg::kWarps, H, DP>(p, attn_smem, Cfg::kWarpBytes, s_ml);

@@ -700,11 +700,14 @@ AttnPlan attn_plan(int64_t rows, int32_t heads, int32_t kv_heads, int32_t dim, i
   // of 200 tokens: 5 us against 10.
   const int64_t tokens = window > 0 ? std::min(capacity, window + kAttnTile - 1) : capacity;
   const int64_t tiles = (tokens + kAttnTile - 1) / kAttnTile, items = rows * kv_heads * a.blocks;
+  // Clusters of 1, 2, ... CTAs, one CTA an SM, that the GPU holds at once (what
+  // cudaOccupancyMaxActiveClusters says there, a few left out): a cluster lies in one GPC.
+  constexpr int kClusters[kAttnClusterCtas] = {kAttnGrid, 74, 44, 32, 25, 21, 15, 15};
   a.direct = 0;
-  if (items > 0 && items <= kAttnGrid) {
-    const int64_t ctas = std::min(std::min<int64_t>(8, kAttnGrid / items), (tiles + a.warps - 1) / a.warps);
-    if (tiles <= ctas * a.warps * kAttnDirect) a.direct = (int)ctas;
-  }
+  for (int ctas = 1; ctas <= kAttnClusterCtas && items > 0 && !a.direct; ++ctas)  // the fewest that have enough warps
+    if (items <= kClusters[ctas - 1] && tiles <= ctas * a.warps * kAttnDirect) a.direct = ctas;
+  for (int ctas = a.direct; a.direct && ctas <= kAttnClusterCtas; ++ctas)  // and more, down to a tile a warp
+    if (items <= kClusters[ctas - 1] && tiles > (ctas - 1) * a.warps) a.direct = ctas;
   a.bytes = 0;
   if (a.direct) return a;
   const size_t segments = (size_t)kAttnGrid * a.warps + attn_asked_max(kAttnGrid * a.warps, a.block_heads);
