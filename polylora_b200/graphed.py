@@ -33,6 +33,9 @@ from typing import Any
 import torch
 
 from .context import LoraBatchContext, use_lora_context
+from .kv_cache import PagedBatch, use_paged_batch
+from .logits import LogitRules
+from .model import apply_output_rules
 
 
 @contextlib.contextmanager
@@ -95,10 +98,22 @@ class GraphedForward:
     with the host, which a capture cannot contain.  Given neither a mask nor
     position ids, the capture takes the eager mode's attention-mask decisions
     (``eager_mask_decisions``).
+
+    With ``paged`` the step runs on the model's paged cache (see
+    ``PolyLoraModel.attach_kv_cache``): sequences may grow, come and go between
+    calls, as long as batches keep the example's rows, page-table width and new
+    tokens (``PagedKVCache.batch(..., width=)``).  The example batch is appended
+    during the warm-up, as the first call with it would.  ``logit_rules`` are
+    applied to the output's logits; later calls' rules are copied into the
+    example's memory.
     """
 
-    def __init__(self, model: Any, adapter_ids: list[str], warmup: int = 2, output=None, **inputs: torch.Tensor):
+    def __init__(self, model: Any, adapter_ids: list[str], warmup: int = 2, output=None,
+                 paged: PagedBatch | None = None, logit_rules: LogitRules | None = None, **inputs: torch.Tensor):
         self.model = model
+        self.paged = paged.clone() if paged is not None else None
+        self.rules = logit_rules.clone() if logit_rules is not None else None
+        self.options = {"use_cache": False} if paged is not None else {}
         self.static = {k: v.clone() for k, v in inputs.items()}
         self.output = output or (lambda out: getattr(out, "last_hidden_state", out))
         batch, seq, device, _ = model._infer_forward_shape(**self.static)
@@ -107,7 +122,7 @@ class GraphedForward:
         model.adapter_cache.to(device, dtype)
         ctx = self._host_part(adapter_ids)
         self.weight_indices = ctx.weight_indices.clone()
-        self.seq_lens = ctx.seq_lens.clone()
+        self.seq_lens = ctx.seq_lens.clone() if paged is None else self.paged.new_lens
         torch.cuda.synchronize(device)  # refills of the example batch are done
 
         def device_part():
@@ -115,8 +130,11 @@ class GraphedForward:
                 adapter_ids=list(adapter_ids), weight_indices=self.weight_indices, seq_lens=self.seq_lens,
                 attention_mask=self.static.get("attention_mask"), table_ranks=ctx.table_ranks, ready_event=None,
             )
-            with use_lora_context(gctx):
-                return self.output(model.base_model(**self.static))
+            with use_lora_context(gctx), use_paged_batch(self.paged):
+                out = model.base_model(**self.static, **self.options)
+            if self.rules is not None:
+                apply_output_rules(out, self.rules)
+            return self.output(out)
 
         side = torch.cuda.Stream(device)
         side.wait_stream(torch.cuda.current_stream(device))
@@ -137,9 +155,19 @@ class GraphedForward:
             adapter_ids, self.static.get("attention_mask"), self.batch, self.seq, self.device
         )
 
-    def __call__(self, adapter_ids: list[str], **inputs: torch.Tensor) -> torch.Tensor:
+    def __call__(self, adapter_ids: list[str], paged: PagedBatch | None = None, logit_rules: LogitRules | None = None,
+                 **inputs: torch.Tensor) -> torch.Tensor:
         """Runs one forward with new inputs (same shapes) and adapter ids; the
-        returned tensor is the graph's output buffer, overwritten by the next call."""
+        returned tensor is the graph's output buffer, overwritten by the next call.
+        Captured with ``paged``, every call needs its batch; rules not given stay."""
+        if (paged is None) != (self.paged is None):
+            raise ValueError("a forward captured with a paged batch takes one with every call, others take none")
+        if logit_rules is not None and self.rules is None:
+            raise ValueError("the forward was captured without logit_rules")
+        if paged is not None:
+            self.paged.copy_(paged)
+        if logit_rules is not None:
+            self.rules.copy_(logit_rules)
         for k, v in inputs.items():
             self.static[k].copy_(v, non_blocking=True)
         ctx = self._host_part(adapter_ids)
@@ -147,7 +175,8 @@ class GraphedForward:
         if ctx.ready_event is not None:
             stream.wait_event(ctx.ready_event)
         self.weight_indices.copy_(ctx.weight_indices, non_blocking=True)
-        self.seq_lens.copy_(ctx.seq_lens, non_blocking=True)
+        if paged is None:
+            self.seq_lens.copy_(ctx.seq_lens, non_blocking=True)
         self.graph.replay()
         cache = self.model.adapter_cache
         slots = {cache.adapter_to_slot[a] for a in set(adapter_ids) if a != self.model.config.base_adapter_id}

@@ -43,6 +43,18 @@ class LogitRules:
     bias_values: torch.Tensor | None = None
     allowed: torch.Tensor | None = None
 
+    def clone(self) -> "LogitRules":
+        return LogitRules(**{k: v.clone() if v is not None else None for k, v in vars(self).items()})
+
+    def copy_(self, other: "LogitRules") -> None:
+        """Takes another's values into this one's memory (for a captured call)."""
+        for name, mine in vars(self).items():
+            theirs = getattr(other, name)
+            if (mine is None) != (theirs is None) or (mine is not None and mine.shape != theirs.shape):
+                raise ValueError(f"{name}: a captured call takes rules of the same kinds and shapes")
+            if mine is not None:
+                mine.copy_(theirs, non_blocking=True)
+
     def tensors(self) -> list[torch.Tensor]:
         every = (self.tokens, self.token_lens, self.prompt_lens, self.repetition_penalty, self.presence_penalty,
                  self.frequency_penalty, self.bias_tokens, self.bias_values, self.allowed)

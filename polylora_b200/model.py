@@ -14,6 +14,8 @@ then adds its LoRA delta with the native kernels.
 
 from __future__ import annotations
 
+import contextlib
+import dataclasses
 from typing import Any, Iterator
 
 import torch
@@ -23,7 +25,9 @@ from .cache import GpuAdapterCache, ModuleSpec
 from .config import PolyLoraConfig
 from . import _native
 from .context import RIGHT_PADDING_ERROR, LoraBatchContext, assert_right_padded, use_lora_context
+from .kv_cache import PagedBatch, PagedKVCache, attach, use_paged_batch
 from .layers import MultiLoraLinear
+from .logits import LogitRules, apply_logit_rules
 from .store import CpuAdapterStore, DiskAdapterCache
 
 _NO_TARGETS = "No nn.Linear modules matched the PolyLoRA module selection"
@@ -67,6 +71,18 @@ def _batch_tensor(args: tuple, kwargs: dict) -> torch.Tensor:
         if torch.is_tensor(arg):
             return arg
     raise ValueError(_NO_BATCH_TENSOR)
+
+
+def apply_output_rules(out: Any, rules: LogitRules) -> None:
+    """``rules`` in place on an output's logits (B, V) or (B, 1, V)."""
+    logits = getattr(out, "logits", out)
+    if not torch.is_tensor(logits):
+        raise ValueError("logit_rules need an output with logits")
+    if logits.dim() == 3 and logits.shape[1] == 1:
+        logits = logits[:, 0]
+    if logits.dim() != 2:
+        raise ValueError(f"logit_rules apply to the logits of one token per row, got {tuple(logits.shape)}")
+    apply_logit_rules(logits, rules, out=logits)
 
 
 class PolyLoraModel(nn.Module):
@@ -116,12 +132,41 @@ class PolyLoraModel(nn.Module):
                                                   module_names=self.target_module_names,
                                                   peft_adapter_name=peft_adapter_name)
 
-    def forward(self, *args: Any, adapter_ids: list[str] | None = None, **kwargs: Any) -> Any:
-        if adapter_ids is None:
-            return self.base_model(*args, **kwargs)
+    def attach_kv_cache(self, cache: PagedKVCache, inv_freq: torch.Tensor | None = None,
+                        rotary_scale: float | None = None, interleaved: bool = False) -> None:
+        """Lets ``forward(..., paged=batch)`` run the base model's attention on
+        ``cache``.  For decoders whose attention modules hold q_proj, k_proj,
+        v_proj and o_proj and rotate queries and keys (in halves, or as
+        neighbouring pairs with ``interleaved``) by ``inv_freq``, by default the
+        model's own rotary embedding's.  Forwards without a batch are unchanged.
+        No counterpart in the reference."""
+        attach(self.base_model, cache, inv_freq, rotary_scale, interleaved)
+
+    def forward(self, *args: Any, adapter_ids: list[str] | None = None, paged: PagedBatch | None = None,
+                logit_rules: LogitRules | None = None, **kwargs: Any) -> Any:
+        """``paged`` (see ``attach_kv_cache``): the new tokens of each row, right
+        padded to ``paged.max_new``, are appended to their sequences and attend to
+        them.  ``logit_rules``: applied in place to the output's logits, of one
+        token per row.  Neither has a counterpart in the reference."""
+        if paged is not None:
+            if kwargs.get("attention_mask") is not None:
+                raise ValueError("a paged batch carries its rows' lengths: pass no attention_mask")
+            kwargs.setdefault("use_cache", False)
+        with use_paged_batch(paged) if paged is not None else contextlib.nullcontext():
+            if adapter_ids is None:
+                out = self.base_model(*args, **kwargs)
+            else:
+                out = self._lora_forward(args, adapter_ids, paged, kwargs)
+        if logit_rules is not None:
+            apply_output_rules(out, logit_rules)
+        return out
+
+    def _lora_forward(self, args: tuple, adapter_ids: list[str], paged: PagedBatch | None, kwargs: dict) -> Any:
         batch_size, seq_len, device, _ = self._infer_forward_shape(*args, **kwargs)
         self.adapter_cache.to(device, _param_device_dtype(self.base_model)[1])
         ctx = self.prepare_lora_context(adapter_ids, kwargs.get("attention_mask"), batch_size, seq_len, device)
+        if paged is not None:
+            ctx = dataclasses.replace(ctx, seq_lens=paged.new_lens)
         with use_lora_context(ctx):
             out = self.base_model(*args, **kwargs)
         # the slots this batch read may be refilled only after the work enqueued so far
