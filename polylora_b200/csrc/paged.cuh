@@ -399,6 +399,7 @@ constexpr int kAttnDealOnly = 32;   // tiles a warp up to which all are dealt
 constexpr int kAttnChunk = 8;       // smallest chunk: a loader's lead of up to 5 tiles then spans two segments
 constexpr int kAttnDirect = 8;      // most tiles of a warp without a list
 constexpr int kAttnAsk = 4;         // tiles ahead of which the next segment is asked for
+static_assert(kAttnChunk > kAttnAsk && kAttnDealOnly > 2 * kAttnAsk, "segments that are followed by others are longer");
 
 // Counts the tiles of the rows and cuts their list.  One CTA.
 __global__ void __launch_bounds__(kAttnPlanThreads) attn_plan_kernel(const AttnParams p, int warps) {
@@ -538,14 +539,19 @@ struct AttnWalk {
   // nothing left moves the loader to it.
   __device__ __forceinline__ bool look_ahead(const AttnParams& p, int left) {
     if (!more) return false;
-    if (left == kAttnAsk && (threadIdx.x & 31) == 0) asked = list.w.dealt + atomicAdd(&p.work->next, 1);
+    if (left == kAttnAsk) ask(p);
     if (left > 0) return false;
     const int id = __shfl_sync(0xffffffffu, asked, 0), ids = list.w.dealt + list.w.asked;
     more = id + 1 < ids;
     if (id >= ids) return false;
     nxt = list.segment(p, id);
     have_nxt = true;
+    // a segment of kAttnAsk tiles or fewer never has that many left after its first
+    if (more && nxt.count <= kAttnAsk) ask(p);
     return true;
+  }
+  __device__ __forceinline__ void ask(const AttnParams& p) {
+    if ((threadIdx.x & 31) == 0) asked = list.w.dealt + atomicAdd(&p.work->next, 1);
   }
   __device__ __forceinline__ bool step() {
     if (!have_nxt) return false;

@@ -87,7 +87,12 @@ def apply_logit_rules(logits: torch.Tensor, rules: LogitRules, out: torch.Tensor
     """``rules`` on logits (B, V), computed in fp32 and rounded once to the
     logits' dtype; into ``out`` (which may be ``logits``) or a new tensor."""
     dev = logits.get_device()
-    _same_device(dev, logits, *rules.tensors())
+    tokens, bias_tokens, bias_values, allowed = rules.tokens, rules.bias_tokens, rules.bias_values, rules.allowed
+    for t in rules.tensors():
+        if t.get_device() != dev or dev < 0:
+            _same_device(dev, logits, t)
+    if dev < 0:
+        _same_device(dev, logits)
     _no_grad(logits)
     if logits.dim() != 2:
         raise ValueError("logits must be (B, V)")
@@ -96,34 +101,38 @@ def apply_logit_rules(logits: torch.Tensor, rules: LogitRules, out: torch.Tensor
     if step != 1 and vocab > 1:
         raise ValueError("logits rows must be contiguous")
     if out is None:
-        out = logits.new_empty((rows, vocab))
-    elif out.shape != logits.shape or out.dtype is not logits.dtype or out.get_device() != dev or (vocab > 1 and out.stride(1) != 1):
+        out = torch.empty_like(logits) if logits.is_contiguous() else logits.new_empty((rows, vocab))
+    elif out is not logits and (out.shape != logits.shape or out.dtype is not logits.dtype or out.get_device() != dev
+                                or (vocab > 1 and out.stride(1) != 1)):
         raise ValueError("out must have the logits' shape, dtype and device, with contiguous rows")
-    tokens, bias_tokens, bias_values, allowed = rules.tokens, rules.bias_tokens, rules.bias_values, rules.allowed
     width = None
-    for name, t in (("tokens", tokens), ("bias_tokens", bias_tokens)):
-        if t is not None and t.dtype not in (torch.int32, torch.int64):
-            raise TypeError(f"{name} must be int32 or int64, got {t.dtype}")
+    history = biases = 0
     if tokens is not None:
-        tokens = _rows_of(tokens, rows, "tokens")
         width = tokens.dtype
+        if width is not torch.int64 and width is not torch.int32:
+            raise TypeError(f"tokens must be int32 or int64, got {width}")
+        tokens = _rows_of(tokens, rows, "tokens")
+        history = tokens.shape[1]
     elif not (rules.token_lens is rules.prompt_lens is rules.repetition_penalty is rules.presence_penalty
               is rules.frequency_penalty is None):
         raise ValueError("penalties and lengths need tokens")
     if (bias_tokens is None) != (bias_values is None):
         raise ValueError("bias_tokens and bias_values go together")
     if bias_tokens is not None:
+        if bias_tokens.dtype is not torch.int64 and bias_tokens.dtype is not torch.int32:
+            raise TypeError(f"bias_tokens must be int32 or int64, got {bias_tokens.dtype}")
         if bias_tokens.shape != bias_values.shape:
             raise ValueError("bias_tokens and bias_values must have one shape")
         bias_tokens = _rows_of(bias_tokens, rows, "bias_tokens")
-        if width is not None and bias_tokens.dtype != width:  # both as the wider: narrowing could alias ids
+        if width is not None and bias_tokens.dtype is not width:  # both as the wider: narrowing could alias ids
             tokens, bias_tokens = tokens.to(torch.int64), bias_tokens.to(torch.int64)
         width = bias_tokens.dtype
-        if bias_values.dtype != torch.float32:
+        if bias_values.dtype is not torch.float32:
             bias_values = bias_values.to(torch.float32)
         bias_values = _rows_of(bias_values, rows, "bias_values")
+        biases = bias_tokens.shape[1]
     if allowed is not None:
-        if allowed.dtype != torch.int32 or allowed.dim() != 2 or allowed.shape[1] < (vocab + 31) // 32:
+        if allowed.dtype is not torch.int32 or allowed.dim() != 2 or allowed.shape[1] < (vocab + 31) // 32:
             raise ValueError(f"allowed must be int32 ({rows}, at least {(vocab + 31) // 32})")
         allowed = _rows_of(allowed, rows, "allowed")
     lens = _per_row(rules.token_lens, rows, torch.int32, "token_lens")
@@ -131,7 +140,6 @@ def apply_logit_rules(logits: torch.Tensor, rules: LogitRules, out: torch.Tensor
     rep = _per_row(rules.repetition_penalty, rows, torch.float32, "repetition_penalty")
     pres = _per_row(rules.presence_penalty, rows, torch.float32, "presence_penalty")
     freq = _per_row(rules.frequency_penalty, rows, torch.float32, "frequency_penalty")
-    history, biases = tokens.shape[1] if tokens is not None else 0, bias_tokens.shape[1] if bias_tokens is not None else 0
     ws_bytes = _native.load().plora_logit_rules_workspace(rows, vocab, history, biases)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=logits.device) if ws_bytes else None
     _call(

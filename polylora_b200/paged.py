@@ -30,9 +30,10 @@ def rotary_phases(inv_freq: torch.Tensor) -> torch.Tensor:
     host = inv_freq.detach().double().cpu()
     if not bool(torch.isfinite(host).all()):
         raise ValueError("inv_freq must be finite")
-    turns = [round(math.ldexp(math.fmod(f, 2 * math.pi) / (2 * math.pi), 64)) for f in host.tolist()]
-    signed = [((t + (1 << 63)) % (1 << 64)) - (1 << 63) for t in turns]
-    return torch.tensor(signed, dtype=torch.int64).to(inv_freq.device)
+    turn = torch.remainder(host / (2 * math.pi), 1.0) * 2.0**32
+    high = turn.floor()
+    low = ((turn - high) * 2.0**32).round()
+    return ((high.to(torch.int64) << 32) + low.to(torch.int64)).to(inv_freq.device)  # mod 2^64
 
 
 def _no_grad(*tensors: torch.Tensor | None) -> None:
@@ -146,7 +147,9 @@ def paged_append(
     tokens zero); None for what was not given or asked for.  Rows of one call
     must not write to the same page."""
     dev = k.get_device()
-    _same_device(dev, k, v, k_cache, v_cache, page_table, past_lens)
+    if dev < 0 or not (v.get_device() == k_cache.get_device() == v_cache.get_device() == page_table.get_device()
+                       == past_lens.get_device() == dev):
+        _same_device(dev, k, v, k_cache, v_cache, page_table, past_lens)
     _no_grad(q, k, v)
     shape, dtype = k.shape, k.dtype
     if len(shape) != 4 or v.shape != shape:
@@ -180,7 +183,7 @@ def paged_append(
             raise TypeError("q, k and v must share one dtype")
         heads = q.shape[2]
         q, qs, q_ptr = _heads(q)
-        q_out = k.new_empty((rows, new, heads, dim))
+        q_out = torch.empty_like(q) if q.is_contiguous() else q.new_empty((rows, new, heads, dim))
         q_out_ptr = q_out.data_ptr()
     k, ks, k_ptr = _heads(k)
     v, vs, v_ptr = _heads(v)
@@ -212,7 +215,9 @@ def paged_attention(
     ``scale`` defaults to D ** -0.5; rows without tokens give zeros.  Heads may
     be any multiple of the cache's kv_heads."""
     dev = q.get_device()
-    _same_device(dev, q, k_cache, v_cache, page_table, seq_lens)
+    if dev < 0 or not (k_cache.get_device() == v_cache.get_device() == page_table.get_device() == seq_lens.get_device()
+                       == dev):
+        _same_device(dev, q, k_cache, v_cache, page_table, seq_lens)
     _no_grad(q)
     if q.dim() != 3:
         raise ValueError("q must be (B, heads, D)")
@@ -223,7 +228,7 @@ def paged_attention(
         raise ValueError(f"{heads} heads over {kv_heads} kv heads")
     lens = _lens(seq_lens, rows, "seq_lens")
     if out is None:
-        out = q.new_empty((rows, heads, dim))
+        out = torch.empty_like(q) if q.is_contiguous() else q.new_empty((rows, heads, dim))
     elif out.shape != q.shape or out.dtype is not dtype or out.get_device() != dev or not out.is_contiguous():
         raise ValueError("out must be a contiguous tensor of q's shape, dtype and device")
     q, qs, q_ptr = _heads(q)
