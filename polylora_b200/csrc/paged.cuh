@@ -607,14 +607,17 @@ struct AttnCopyLoader {
   using Tile = AttnTileCfg<EB, DP>;
   AttnCursor at;
   int left;
-  int page, inner;  // of this lane's token of tile `at`; page -1: reads as zeros
+  // of this lane's token of tile `at`: page (-1: reads as zeros), byte offsets of its
+  // heads in the two caches
+  int page;
+  int64_t k_at, v_at;
 
   __device__ __forceinline__ void start(const AttnParams& p, const AttnSegment& s) {
     at = s.at, left = s.count;
     look_up(p);
   }
   __device__ __forceinline__ void look_up(const AttnParams& p) {
-    page = -1, inner = 0;
+    page = -1, k_at = v_at = 0;
     if (left <= 0) return;
     const int pos = at.tile * kAttnTile + (threadIdx.x & 15);
     if (pos >= at.r.lo && pos < at.r.n) {
@@ -623,8 +626,11 @@ struct AttnCopyLoader {
       if ((uint32_t)page >= (uint32_t)p.c.num_pages) {
         raise_status(PLORA_DEV_PAGE_RANGE);
         page = -1;
+      } else {
+        const int inner = (at.kv * p.c.page_size + pos - e * p.c.page_size) * p.c.dim;
+        k_at = (page * p.c.k_page + inner) * EB;
+        v_at = (page * p.c.v_page + inner) * EB;
       }
-      inner = (at.kv * p.c.page_size + pos - e * p.c.page_size) * p.c.dim;
     }
   }
   // Starts the copies of tile `at` (none past the share's end) and steps on.
@@ -632,13 +638,13 @@ struct AttnCopyLoader {
     if (left > 0) {
       constexpr int LANES = Tile::kChunks < 32 ? Tile::kChunks : 32;  // lanes of a row
       const int lane = threadIdx.x & 31, lc = lane % LANES;
+      const bool live = page >= 0;
 #pragma unroll
       for (int r0 = 0; r0 < kAttnTile; r0 += 32 / LANES) {
         const int row = r0 + lane / LANES;
-        const int pg = __shfl_sync(0xffffffffu, page, row), in = __shfl_sync(0xffffffffu, inner, row);
-        const bool ok = pg >= 0;
-        const char* k = (const char*)p.c.k + (ok ? (pg * p.c.k_page + in) * EB : 0);
-        const char* v = (const char*)p.c.v + (ok ? (pg * p.c.v_page + in) * EB : 0);
+        const bool ok = __shfl_sync(0xffffffffu, live, row);
+        const char* k = (const char*)p.c.k + __shfl_sync(0xffffffffu, k_at, row);
+        const char* v = (const char*)p.c.v + __shfl_sync(0xffffffffu, v_at, row);
 #pragma unroll
         for (int c = lc; c < Tile::kChunks; c += LANES) {
           if (c * (16 / EB) < p.c.dim) {  // columns past dim stay zero
@@ -788,14 +794,19 @@ __device__ __forceinline__ void attn_gather(const AttnParams& p, const unsigned 
     const uint32_t own = smem_u32(rings) + (h * (DP + 4) + e) * 4;
     for (int c = 0; c < p.direct; ++c) {
       const uint32_t from = cluster_map(own, c);
-      float4 v[WARPS];
+      constexpr int AT_ONCE = WARPS < 8 ? WARPS : 8;
+      static_assert(WARPS % AT_ONCE == 0, "");
+#pragma unroll 1
+      for (int w0 = 0; w0 < WARPS; w0 += AT_ONCE) {
+        float4 v[AT_ONCE];
 #pragma unroll
-      for (int w = 0; w < WARPS; ++w) v[w] = ld_cluster_f4(from + w * pitch);
+        for (int w = 0; w < AT_ONCE; ++w) v[w] = ld_cluster_f4(from + (w0 + w) * pitch);
 #pragma unroll
-      for (int w = 0; w < WARPS; ++w) {
-        const float f = s_f[c * WARPS + w][h];
-        if (f == 0.f) continue;  // a warp without tiles, whose ring holds no sums
-        o[0] += v[w].x * f, o[1] += v[w].y * f, o[2] += v[w].z * f, o[3] += v[w].w * f;
+        for (int w = 0; w < AT_ONCE; ++w) {
+          const float f = s_f[c * WARPS + w0 + w][h];
+          if (f == 0.f) continue;  // a warp without tiles, whose ring holds no sums
+          o[0] += v[w].x * f, o[1] += v[w].y * f, o[2] += v[w].z * f, o[3] += v[w].w * f;
+        }
       }
     }
     T* out = (T*)p.out + (((int64_t)row * p.c.kv_heads + kv) * p.group + h0 + h) * p.c.dim + e;
@@ -985,10 +996,12 @@ struct AttnMmaCfg {
   static constexpr int kHeads = 8 * NT;            // query heads of a block
   static constexpr bool kQShared = NT * DP > 256;  // query fragments in shared memory, not registers
   static constexpr int kQBytes = kQShared ? kHeads * DP * 2 : 0;
-  static constexpr int kStages = DP == 256 ? 2 : (DP == 128 ? 3 : 6);
+  // heads of 64: tiles of half the bytes and nearly the instructions, so twice the warps
+  static constexpr bool kMany = DP == 64 && NT == 1;
+  static constexpr int kStages = DP == 256 ? 2 : (DP == 128 || kMany ? 3 : 6);
   static constexpr int kWarpBytes = kStages * Tile::kStageBytes + kQBytes;
-  static constexpr int kFit = 220 * 1024 / kWarpBytes;
-  static constexpr int kWarps = kFit < 8 ? kFit : 8;
+  static constexpr int kFit = 220 * 1024 / kWarpBytes, kMost = kMany ? 16 : 8;
+  static constexpr int kWarps = kFit < kMost ? kFit : kMost;
   static constexpr int kSmemBytes = 1024 + kWarps * kWarpBytes;  // aligned to 1024 bytes
 };
 
