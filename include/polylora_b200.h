@@ -345,25 +345,53 @@ int plora_peft_pack(const char* path, const char* const* modules, int32_t num_mo
  * workspace (plora_paged_attention_workspace bytes, 256-byte aligned; 0 for few
  * short rows and for arguments the call rejects) needs no initialisation; calls that may overlap
  * need one each. */
-int plora_paged_append(const void* q, int64_t q_row_stride, int64_t q_token_stride, int64_t q_head_stride,
-                       const void* k, int64_t k_row_stride, int64_t k_token_stride, int64_t k_head_stride,
-                       const void* v, int64_t v_row_stride, int64_t v_token_stride, int64_t v_head_stride,
-                       void* q_out, void* k_out, void* k_cache, void* v_cache, int64_t k_page_stride,
-                       int64_t v_page_stride, const int32_t* page_table, int64_t table_stride,
-                       const int32_t* past_lens, const int32_t* new_lens, const int64_t* phases, int32_t pairs,
-                       int32_t interleaved, float rotary_scale, int64_t rows, int64_t max_new, int32_t q_heads,
-                       int32_t kv_heads, int32_t head_dim, int32_t page_size, int64_t num_pages, int64_t max_pages,
-                       int32_t dtype, void* stream);
+
+typedef struct plora_paged_cache {
+  void* k_cache;
+  void* v_cache;
+  int64_t k_page_stride, v_page_stride;
+  const int32_t* page_table;
+  int64_t table_stride;
+  int64_t rows, heads, kv_heads, head_dim; /* heads: of q */
+  int64_t page_size, num_pages, max_pages;
+  int64_t dtype;
+} plora_paged_cache;
+
+typedef struct plora_paged_append_args {
+  plora_paged_cache cache;
+  const void* q; /* null: none */
+  int64_t q_row_stride, q_token_stride, q_head_stride;
+  const void* k;
+  int64_t k_row_stride, k_token_stride, k_head_stride;
+  const void* v;
+  int64_t v_row_stride, v_token_stride, v_head_stride;
+  void* q_out;
+  void* k_out;               /* null: not wanted */
+  const int32_t* past_lens;
+  const int32_t* new_lens;   /* null: max_new each */
+  const int64_t* phases;
+  int64_t pairs, interleaved, max_new;
+  double rotary_scale;
+} plora_paged_append_args;
+
+int plora_paged_append(const plora_paged_append_args* args, void* stream);
+
+typedef struct plora_paged_attention_args {
+  plora_paged_cache cache;
+  const void* q; /* (rows, heads, head_dim) */
+  int64_t q_row_stride, q_head_stride;
+  const int32_t* seq_lens;
+  void* out;
+  double scale;
+  int64_t window;
+  void* workspace;
+  int64_t workspace_size;
+} plora_paged_attention_args;
 
 size_t plora_paged_attention_workspace(int64_t rows, int32_t heads, int32_t kv_heads, int32_t head_dim,
                                        int32_t page_size, int64_t max_pages, int64_t window, int32_t dtype);
 
-int plora_paged_attention(const void* q, int64_t q_row_stride, int64_t q_head_stride, const void* k_cache,
-                          const void* v_cache, int64_t k_page_stride, int64_t v_page_stride,
-                          const int32_t* page_table, int64_t table_stride, const int32_t* seq_lens, void* out,
-                          float scale, int64_t window, int64_t rows, int32_t heads, int32_t kv_heads,
-                          int32_t head_dim, int32_t page_size, int64_t num_pages, int64_t max_pages, int32_t dtype,
-                          void* workspace, size_t workspace_size, void* stream);
+int plora_paged_attention(const plora_paged_attention_args* args, void* stream);
 
 /* ---------------------------------------------------------------------------
  * Each row's own rules on its logits (no counterpart in the reference).
@@ -386,13 +414,30 @@ int plora_paged_attention(const void* q, int64_t q_row_stride, int64_t q_head_st
  * need one each. */
 size_t plora_logit_rules_workspace(int64_t rows, int64_t vocab, int64_t history, int64_t biases);
 
-int plora_logit_rules(const void* logits, int64_t logits_stride, void* out, int64_t out_stride, int64_t rows,
-                      int64_t vocab, int32_t dtype, const void* tokens, int64_t tokens_stride, int64_t history,
-                      const int32_t* token_lens, const int32_t* prompt_lens, const float* repetition,
-                      const float* presence, const float* frequency, const void* bias_tokens,
-                      int64_t bias_tokens_stride, const float* bias_values, int64_t bias_values_stride,
-                      int64_t biases, const int32_t* allowed, int64_t allowed_stride, int32_t token_bytes,
-                      void* workspace, size_t workspace_size, void* stream);
+typedef struct plora_logit_rules_args {
+  const void* logits;
+  int64_t logits_stride;
+  void* out;
+  int64_t out_stride;
+  int64_t rows, vocab, dtype;
+  const void* tokens;
+  int64_t tokens_stride, history;
+  const int32_t* token_lens;
+  const int32_t* prompt_lens;
+  const float* repetition;
+  const float* presence;
+  const float* frequency;
+  const void* bias_tokens;
+  int64_t bias_tokens_stride;
+  const float* bias_values;
+  int64_t bias_values_stride, biases;
+  const int32_t* allowed;
+  int64_t allowed_stride, token_bytes;
+  void* workspace;
+  int64_t workspace_size;
+} plora_logit_rules_args;
+
+int plora_logit_rules(const plora_logit_rules_args* args, void* stream);
 
 #ifdef __cplusplus
 }

@@ -8,6 +8,7 @@ is no CPU fallback.
 from __future__ import annotations
 
 import ctypes
+import struct
 import threading
 from pathlib import Path
 
@@ -77,6 +78,12 @@ class SlotRecord(ctypes.Structure):
         ("scale", ctypes.c_float),
     ]
 
+
+# plora_paged_append_args, plora_paged_attention_args, plora_logit_rules_args: fields of
+# 8 bytes, packed into bytes (ctypes takes 3 us to convert as many single arguments)
+PAGED_APPEND_ARGS = struct.Struct("=14q12q8qd")
+PAGED_ATTENTION_ARGS = struct.Struct("=14q5qd3q")
+LOGIT_RULES_ARGS = struct.Struct("=25q")
 
 # name -> (restype, argtypes)
 _SIGNATURES: dict[str, tuple[object, list[object]]] = {
@@ -155,31 +162,11 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
             _i64, _i64, _i64, _i64, _i32, _i32, _i32, _c_void_p,
         ],
     ),
-    "plora_paged_append": (
-        ctypes.c_int,
-        [
-            _c_void_p, _i64, _i64, _i64, _c_void_p, _i64, _i64, _i64, _c_void_p, _i64, _i64, _i64,
-            _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i64, _c_void_p, _i64, _c_void_p, _c_void_p, _c_void_p,
-            _i32, _i32, ctypes.c_float, _i64, _i64, _i32, _i32, _i32, _i32, _i64, _i64, _i32, _c_void_p,
-        ],
-    ),
+    "plora_paged_append": (ctypes.c_int, [ctypes.c_char_p, _c_void_p]),
     "plora_paged_attention_workspace": (_size, [_i64, _i32, _i32, _i32, _i32, _i64, _i64, _i32]),
-    "plora_paged_attention": (
-        ctypes.c_int,
-        [
-            _c_void_p, _i64, _i64, _c_void_p, _c_void_p, _i64, _i64, _c_void_p, _i64, _c_void_p, _c_void_p,
-            ctypes.c_float, _i64, _i64, _i32, _i32, _i32, _i32, _i64, _i64, _i32, _c_void_p, _size, _c_void_p,
-        ],
-    ),
+    "plora_paged_attention": (ctypes.c_int, [ctypes.c_char_p, _c_void_p]),
     "plora_logit_rules_workspace": (_size, [_i64, _i64, _i64, _i64]),
-    "plora_logit_rules": (
-        ctypes.c_int,
-        [
-            _c_void_p, _i64, _c_void_p, _i64, _i64, _i64, _i32, _c_void_p, _i64, _i64, _c_void_p, _c_void_p,
-            _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p, _i64, _i64, _c_void_p, _i64, _i32, _c_void_p,
-            _size, _c_void_p,
-        ],
-    ),
+    "plora_logit_rules": (ctypes.c_int, [ctypes.c_char_p, _c_void_p]),
     "plora_slot_fill": (
         ctypes.c_int,
         [_c_void_p, _i32, _i32, _i32, _i64, _i32, _c_void_p, _size, _c_void_p, _size, _c_void_p],

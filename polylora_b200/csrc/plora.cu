@@ -722,40 +722,42 @@ AttnPlan attn_plan(int64_t rows, int32_t heads, int32_t kv_heads, int32_t dim, i
 }
 
 // Arguments that both paged entry points share.
-int paged_view(PagedView* c, const void* k_cache, const void* v_cache, int64_t k_page_stride, int64_t v_page_stride,
-               const int32_t* page_table, int64_t table_stride, int64_t rows, int32_t heads, int32_t kv_heads,
-               int32_t head_dim, int32_t page_size, int64_t num_pages, int64_t max_pages, int32_t dtype) {
-  if (!valid_dtype(dtype)) return fail(PLORA_ERR_INVALID_ARGUMENT, "unknown dtype %d", dtype);
-  if (rows < 0 || kv_heads < 1 || heads < 0 || head_dim < 1 || page_size < 1 || num_pages < 1 || max_pages < 1)
+int paged_view(PagedView* c, const plora_paged_cache& a, int64_t heads) {
+  const int64_t head_dim = a.head_dim, page_size = a.page_size, kv_heads = a.kv_heads;
+  if (a.dtype < 0 || a.dtype > INT32_MAX || !valid_dtype((int)a.dtype))
+    return fail(PLORA_ERR_INVALID_ARGUMENT, "unknown dtype %lld", (long long)a.dtype);
+  if (a.rows < 0 || kv_heads < 1 || heads < 0 || head_dim < 1 || page_size < 1 || a.num_pages < 1 || a.max_pages < 1)
     return fail(PLORA_ERR_INVALID_ARGUMENT, "rows, heads, head_dim, page_size or page counts not positive");
-  if (heads % kv_heads) return fail(PLORA_ERR_INVALID_ARGUMENT, "%d heads over %d kv heads", heads, kv_heads);
+  if (heads % kv_heads)
+    return fail(PLORA_ERR_INVALID_ARGUMENT, "%lld heads over %lld kv heads", (long long)heads, (long long)kv_heads);
   if (head_dim % 8 || head_dim > 256)
-    return fail(PLORA_ERR_UNSUPPORTED, "head_dim %d is no multiple of 8 up to 256", head_dim);
-  if (rows > kPagedMaxRows || heads > 65535 || kv_heads > 65535)
-    return fail(PLORA_ERR_UNSUPPORTED, "%lld rows, %d heads", (long long)rows, heads);
-  if (num_pages > INT32_MAX || max_pages > INT32_MAX / page_size)
-    return fail(PLORA_ERR_UNSUPPORTED, "num_pages, or positions of max_pages pages, beyond int32");
-  const int64_t page_elems = (int64_t)kv_heads * head_dim;  // kv_heads <= 65535, head_dim <= 256
+    return fail(PLORA_ERR_UNSUPPORTED, "head_dim %lld is no multiple of 8 up to 256", (long long)head_dim);
+  if (a.rows > kPagedMaxRows || heads > 65535 || kv_heads > 65535)
+    return fail(PLORA_ERR_UNSUPPORTED, "%lld rows, %lld heads", (long long)a.rows, (long long)heads);
+  if (page_size > INT32_MAX || a.num_pages > INT32_MAX || a.max_pages > INT32_MAX / page_size)
+    return fail(PLORA_ERR_UNSUPPORTED, "page_size, num_pages, or positions of max_pages pages, beyond int32");
+  const int64_t page_elems = kv_heads * head_dim;  // kv_heads <= 65535, head_dim <= 256
   if (page_elems > INT32_MAX / page_size) return fail(PLORA_ERR_UNSUPPORTED, "elements of a page beyond int32");
-  if (k_page_stride < page_elems * page_size || v_page_stride < page_elems * page_size || table_stride < max_pages)
+  if (a.k_page_stride < page_elems * page_size || a.v_page_stride < page_elems * page_size ||
+      a.table_stride < a.max_pages)
     return fail(PLORA_ERR_INVALID_ARGUMENT, "page or page-table stride below its extent");
-  const int64_t vec = 16 / (int64_t)elem_size(dtype);
-  if (k_page_stride % vec || v_page_stride % vec || !aligned16(k_cache) || !aligned16(v_cache))
+  const int64_t vec = 16 / (int64_t)elem_size((int)a.dtype);
+  if (a.k_page_stride % vec || a.v_page_stride % vec || !aligned16(a.k_cache) || !aligned16(a.v_cache))
     return fail(PLORA_ERR_INVALID_ARGUMENT, "cache pages must be 16-byte aligned");
-  if (num_pages > INT64_MAX / 16 / std::max(k_page_stride, v_page_stride))
+  if (a.num_pages > INT64_MAX / 16 / std::max(a.k_page_stride, a.v_page_stride))
     return fail(PLORA_ERR_INVALID_ARGUMENT, "cache size overflows");
-  if (rows > 0 && (!k_cache || !v_cache || !page_table)) return fail(PLORA_ERR_INVALID_ARGUMENT, "null pointer");
-  c->k = const_cast<void*>(k_cache);
-  c->v = const_cast<void*>(v_cache);
-  c->table = page_table;
-  c->table_stride = table_stride;
-  c->k_page = k_page_stride;
-  c->v_page = v_page_stride;
-  c->capacity = max_pages * page_size;
-  c->num_pages = (int32_t)num_pages;
-  c->kv_heads = kv_heads;
-  c->page_size = page_size;
-  c->dim = head_dim;
+  if (a.rows > 0 && (!a.k_cache || !a.v_cache || !a.page_table)) return fail(PLORA_ERR_INVALID_ARGUMENT, "null pointer");
+  c->k = a.k_cache;
+  c->v = a.v_cache;
+  c->table = a.page_table;
+  c->table_stride = a.table_stride;
+  c->k_page = a.k_page_stride;
+  c->v_page = a.v_page_stride;
+  c->capacity = a.max_pages * page_size;
+  c->num_pages = (int32_t)a.num_pages;
+  c->kv_heads = (int32_t)kv_heads;
+  c->page_size = (int32_t)page_size;
+  c->dim = (int32_t)head_dim;
   c->page.set((uint32_t)page_size);
   return PLORA_OK;
 }
@@ -1176,43 +1178,42 @@ int plora_slot_fill(const plora_slot_module* modules, int32_t num_modules, int32
   return check_launch("slot_fill_kernel");
 }
 
-int plora_paged_append(const void* q, int64_t q_row_stride, int64_t q_token_stride, int64_t q_head_stride,
-                       const void* k, int64_t k_row_stride, int64_t k_token_stride, int64_t k_head_stride,
-                       const void* v, int64_t v_row_stride, int64_t v_token_stride, int64_t v_head_stride,
-                       void* q_out, void* k_out, void* k_cache, void* v_cache, int64_t k_page_stride,
-                       int64_t v_page_stride, const int32_t* page_table, int64_t table_stride,
-                       const int32_t* past_lens, const int32_t* new_lens, const int64_t* phases, int32_t pairs,
-                       int32_t interleaved, float rotary_scale, int64_t rows, int64_t max_new, int32_t q_heads,
-                       int32_t kv_heads, int32_t head_dim, int32_t page_size, int64_t num_pages, int64_t max_pages,
-                       int32_t dtype, void* stream) {
+int plora_paged_append(const plora_paged_append_args* args, void* stream) {
   g_last_error.clear();
+  if (!args) return fail(PLORA_ERR_INVALID_ARGUMENT, "null arguments");
+  const plora_paged_cache& c = args->cache;
+  const void *q = args->q, *k = args->k, *v = args->v;
+  const int64_t pairs = args->pairs, max_new = args->max_new, rows = c.rows;
   AppendParams p = {};
-  int st = paged_view(&p.c, k_cache, v_cache, k_page_stride, v_page_stride, page_table, table_stride, rows,
-                      q ? q_heads : 0, kv_heads, head_dim, page_size, num_pages, max_pages, dtype);
+  int st = paged_view(&p.c, c, q ? c.heads : 0);
   if (st) return st;
-  if (max_new < 0 || pairs < 0 || 2 * (int64_t)pairs > head_dim)
-    return fail(PLORA_ERR_INVALID_ARGUMENT, "max_new negative, or %d rotated pairs in a head of %d", pairs, head_dim);
+  if (max_new < 0 || pairs < 0 || pairs > c.head_dim / 2)
+    return fail(PLORA_ERR_INVALID_ARGUMENT, "max_new negative, or %lld rotated pairs in a head of %lld",
+                (long long)pairs, (long long)c.head_dim);
+  const int dtype = (int)c.dtype, head_dim = (int)c.head_dim, kv_heads = (int)c.kv_heads;
   if (!token_count_ok(rows, max_new)) return fail(PLORA_ERR_UNSUPPORTED, "rows * max_new beyond int32");
   if (rows == 0 || max_new == 0) return PLORA_OK;
-  if (!k || !v || !past_lens || (q && !q_out) || (pairs && !phases))
+  if (!k || !v || !args->past_lens || (q && !args->q_out) || (pairs && !args->phases))
     return fail(PLORA_ERR_INVALID_ARGUMENT, "null pointer");
   const int64_t vec = 16 / (int64_t)elem_size(dtype);
-  const int64_t strides[9] = {q ? q_row_stride : 0, q ? q_token_stride : 0, q ? q_head_stride : 0,
-                              k_row_stride, k_token_stride, k_head_stride, v_row_stride, v_token_stride, v_head_stride};
+  const int64_t strides[9] = {q ? args->q_row_stride : 0, q ? args->q_token_stride : 0, q ? args->q_head_stride : 0,
+                              args->k_row_stride, args->k_token_stride, args->k_head_stride,
+                              args->v_row_stride, args->v_token_stride, args->v_head_stride};
   for (int64_t x : strides)
     if (x < 0 || x % vec) return fail(PLORA_ERR_INVALID_ARGUMENT, "token strides must be multiples of 16 bytes");
-  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(q_out) || !aligned16(k_out))
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(args->q_out) ||
+      !aligned16(args->k_out))
     return fail(PLORA_ERR_INVALID_ARGUMENT, "token pointers must be 16-byte aligned");
   DeviceInfo* di = nullptr;
   if ((st = device_info(&di))) return st;
-  p.q = q, p.k = k, p.v = v, p.q_out = q_out, p.k_out = k_out;
+  p.q = q, p.k = k, p.v = v, p.q_out = args->q_out, p.k_out = args->k_out;
   p.q_row = strides[0], p.q_tok = strides[1], p.q_head = strides[2];
   p.k_row = strides[3], p.k_tok = strides[4], p.k_head = strides[5];
   p.v_row = strides[6], p.v_tok = strides[7], p.v_head = strides[8];
-  p.past = past_lens, p.news = new_lens;
-  p.phases = reinterpret_cast<const uint64_t*>(phases);
-  p.q_heads = q ? q_heads : 0;
-  p.pairs = pairs, p.interleaved = interleaved != 0, p.scale = rotary_scale;
+  p.past = args->past_lens, p.news = args->new_lens;
+  p.phases = reinterpret_cast<const uint64_t*>(args->phases);
+  p.q_heads = q ? (int32_t)c.heads : 0;
+  p.pairs = (int32_t)pairs, p.interleaved = args->interleaved != 0, p.scale = (float)args->rotary_scale;
   p.max_new = (int32_t)max_new, p.tokens = (int32_t)(rows * max_new);
   // one token a CTA until that fills the SMs
   p.cta_tokens = p.tokens <= 8 * di->sm_count ? 1 : kAppendTokens;
@@ -1220,7 +1221,7 @@ int plora_paged_append(const void* q, int64_t q_row_stride, int64_t q_token_stri
   p.by_new.set((uint32_t)max_new);
   p.by_head.set((uint32_t)per_head);
   p.by_item.set((uint32_t)(per_head * (p.q_heads + 2 * kv_heads)));
-  const bool whole = interleaved ? 2 * pairs % n == 0 : pairs % n == 0;
+  const bool whole = p.interleaved ? 2 * pairs % n == 0 : pairs % n == 0;
   const unsigned grid = (unsigned)((p.tokens + p.cta_tokens - 1) / p.cta_tokens);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e = dtype == PLORA_DTYPE_F32   ? launch_append<float>(p, whole, grid, s)
@@ -1239,38 +1240,37 @@ size_t plora_paged_attention_workspace(int64_t rows, int32_t heads, int32_t kv_h
   return attn_plan(rows, heads, kv_heads, head_dim, max_pages * page_size, window, dtype).bytes;
 }
 
-int plora_paged_attention(const void* q, int64_t q_row_stride, int64_t q_head_stride, const void* k_cache,
-                          const void* v_cache, int64_t k_page_stride, int64_t v_page_stride,
-                          const int32_t* page_table, int64_t table_stride, const int32_t* seq_lens, void* out,
-                          float scale, int64_t window, int64_t rows, int32_t heads, int32_t kv_heads,
-                          int32_t head_dim, int32_t page_size, int64_t num_pages, int64_t max_pages, int32_t dtype,
-                          void* workspace, size_t workspace_size, void* stream) {
+int plora_paged_attention(const plora_paged_attention_args* args, void* stream) {
   g_last_error.clear();
+  if (!args) return fail(PLORA_ERR_INVALID_ARGUMENT, "null arguments");
+  const plora_paged_cache& c = args->cache;
+  const int64_t rows = c.rows, window = args->window;
+  const void* q = args->q;
   AttnParams p = {};
-  int st = paged_view(&p.c, k_cache, v_cache, k_page_stride, v_page_stride, page_table, table_stride, rows, heads,
-                      kv_heads, head_dim, page_size, num_pages, max_pages, dtype);
+  int st = paged_view(&p.c, c, c.heads);
   if (st) return st;
+  const int dtype = (int)c.dtype, heads = (int)c.heads, kv_heads = (int)c.kv_heads, head_dim = (int)c.head_dim;
   if (heads < 1) return fail(PLORA_ERR_INVALID_ARGUMENT, "no heads");
   if (window < 0) return fail(PLORA_ERR_INVALID_ARGUMENT, "window %lld is negative", (long long)window);
   if (rows == 0) return PLORA_OK;
-  if (!q || !seq_lens || !out) return fail(PLORA_ERR_INVALID_ARGUMENT, "null pointer");
-  const size_t elem = elem_size(dtype);
-  if (q_row_stride < 0 || q_head_stride < 0 || q_row_stride * elem % 16 || q_head_stride * elem % 16 ||
-      !aligned16(q) || !aligned16(out))
+  if (!q || !args->seq_lens || !args->out) return fail(PLORA_ERR_INVALID_ARGUMENT, "null pointer");
+  const int64_t vec = 16 / (int64_t)elem_size(dtype);
+  if (args->q_row_stride < 0 || args->q_head_stride < 0 || args->q_row_stride % vec || args->q_head_stride % vec ||
+      !aligned16(q) || !aligned16(args->out))
     return fail(PLORA_ERR_INVALID_ARGUMENT, "q and out must be 16-byte aligned, with q's strides multiples of 16 bytes");
   const AttnPlan a = attn_plan(rows, heads, kv_heads, head_dim, p.c.capacity, window, dtype);
-  if (workspace_size < a.bytes || (a.bytes && !workspace))
-    return fail(PLORA_ERR_WORKSPACE, "attention workspace %zu < %zu bytes", workspace_size, a.bytes);
-  if (reinterpret_cast<uintptr_t>(workspace) % 256)
+  if (a.bytes && (!args->workspace || args->workspace_size < (int64_t)a.bytes))
+    return fail(PLORA_ERR_WORKSPACE, "attention workspace %lld < %zu bytes", (long long)args->workspace_size, a.bytes);
+  if (reinterpret_cast<uintptr_t>(args->workspace) % 256)
     return fail(PLORA_ERR_INVALID_ARGUMENT, "workspace must be 256-byte aligned");
   DeviceInfo* di = nullptr;
   if ((st = device_info(&di))) return st;
-  p.q = q, p.out = out, p.seq_lens = seq_lens;
-  p.q_row = q_row_stride, p.q_head = q_head_stride;
+  p.q = q, p.out = args->out, p.seq_lens = args->seq_lens;
+  p.q_row = args->q_row_stride, p.q_head = args->q_head_stride;
   p.rows = (int32_t)rows, p.group = heads / kv_heads, p.blocks = a.blocks, p.block_heads = a.block_heads;
   p.window = (int32_t)std::min<int64_t>(window, INT32_MAX);
-  p.scale_log2 = scale * 1.4426950408889634f;
-  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  p.scale_log2 = (float)(args->scale * 1.4426950408889634);  // log2(e)
+  uint8_t* ws = static_cast<uint8_t*>(args->workspace);
   p.work = reinterpret_cast<AttnWork*>(ws);
   p.before = reinterpret_cast<int64_t*>(ws + a.before_offset);
   p.cut = reinterpret_cast<int4*>(ws + a.cut_offset);
@@ -1281,8 +1281,8 @@ int plora_paged_attention(const void* q, int64_t q_row_stride, int64_t q_head_st
   p.direct = a.direct;
   CUtensorMap mk = {}, mv = {};
   const bool tma = attn_by_tma(p.c, a);
-  if (tma && ((st = make_map_cache(&mk, k_cache, dtype, p.c, k_page_stride)) ||
-              (st = make_map_cache(&mv, v_cache, dtype, p.c, v_page_stride))))
+  if (tma && ((st = make_map_cache(&mk, c.k_cache, dtype, p.c, c.k_page_stride)) ||
+              (st = make_map_cache(&mv, c.v_cache, dtype, p.c, c.v_page_stride))))
     return st;
   PLORA_CUDA(launch_attn(p, a, dtype, tma, mk, mv, s), "launch paged attention");
   return PLORA_OK;
@@ -1295,31 +1295,33 @@ size_t plora_logit_rules_workspace(int64_t rows, int64_t vocab, int64_t history,
   return rules_plan(rows, vocab, history, biases, true).bytes;
 }
 
-int plora_logit_rules(const void* logits, int64_t logits_stride, void* out, int64_t out_stride, int64_t rows,
-                      int64_t vocab, int32_t dtype, const void* tokens, int64_t tokens_stride, int64_t history,
-                      const int32_t* token_lens, const int32_t* prompt_lens, const float* repetition,
-                      const float* presence, const float* frequency, const void* bias_tokens,
-                      int64_t bias_tokens_stride, const float* bias_values, int64_t bias_values_stride,
-                      int64_t biases, const int32_t* allowed, int64_t allowed_stride, int32_t token_bytes,
-                      void* workspace, size_t workspace_size, void* stream) {
+int plora_logit_rules(const plora_logit_rules_args* args, void* stream) {
   g_last_error.clear();
-  if (!valid_dtype(dtype)) return fail(PLORA_ERR_INVALID_ARGUMENT, "unknown dtype %d", dtype);
+  if (!args) return fail(PLORA_ERR_INVALID_ARGUMENT, "null arguments");
+  const void *logits = args->logits, *tokens = args->tokens, *bias_tokens = args->bias_tokens;
+  void *out = args->out, *workspace = args->workspace;
+  const int64_t rows = args->rows, vocab = args->vocab, history = args->history, biases = args->biases;
+  const int64_t logits_stride = args->logits_stride, out_stride = args->out_stride;
+  if (args->dtype < 0 || args->dtype > INT32_MAX || !valid_dtype((int)args->dtype))
+    return fail(PLORA_ERR_INVALID_ARGUMENT, "unknown dtype %lld", (long long)args->dtype);
+  const int dtype = (int)args->dtype;
   if (rows < 0 || vocab < 0 || history < 0 || biases < 0)
     return fail(PLORA_ERR_INVALID_ARGUMENT, "negative rows, vocab, history or biases");
-  if (token_bytes != 4 && token_bytes != 8) return fail(PLORA_ERR_INVALID_ARGUMENT, "token ids of %d bytes", token_bytes);
+  if (args->token_bytes != 4 && args->token_bytes != 8)
+    return fail(PLORA_ERR_INVALID_ARGUMENT, "token ids of %lld bytes", (long long)args->token_bytes);
   if (rows > 65535 || vocab > (1 << 30) || history > (1 << 30) - 1 || biases > kRulesMaxBiases)
     return fail(PLORA_ERR_UNSUPPORTED, "rows > 65535, vocab or history beyond 2^30, or more than %d biases a row",
                 kRulesMaxBiases);
   if (rows == 0 || vocab == 0) return PLORA_OK;
-  if (!logits || !out || (history && !tokens) || (biases && (!bias_tokens || !bias_values)))
+  if (!logits || !out || (history && !tokens) || (biases && (!bias_tokens || !args->bias_values)))
     return fail(PLORA_ERR_INVALID_ARGUMENT, "null pointer");
-  if (logits_stride < vocab || out_stride < vocab || (history && tokens_stride < 0) ||
-      (biases && (bias_tokens_stride < 0 || bias_values_stride < 0)) ||
-      (allowed && allowed_stride < 0))
+  if (logits_stride < vocab || out_stride < vocab || (history && args->tokens_stride < 0) ||
+      (biases && (args->bias_tokens_stride < 0 || args->bias_values_stride < 0)) ||
+      (args->allowed && args->allowed_stride < 0))
     return fail(PLORA_ERR_INVALID_ARGUMENT, "row strides below the vocabulary, or negative");
-  const RulesPlan a = rules_plan(rows, vocab, history, biases, logits != out || logits_stride != out_stride || allowed);
-  if (workspace_size < a.bytes || (a.bytes && !workspace))
-    return fail(PLORA_ERR_WORKSPACE, "logit rules workspace %zu < %zu bytes", workspace_size, a.bytes);
+  const RulesPlan a = rules_plan(rows, vocab, history, biases, logits != out || logits_stride != out_stride || args->allowed);
+  if (a.bytes && (!workspace || args->workspace_size < (int64_t)a.bytes))
+    return fail(PLORA_ERR_WORKSPACE, "logit rules workspace %lld < %zu bytes", (long long)args->workspace_size, a.bytes);
   if (reinterpret_cast<uintptr_t>(workspace) % 256)
     return fail(PLORA_ERR_INVALID_ARGUMENT, "workspace must be 256-byte aligned");
   const uintptr_t el = elem_size(dtype) - 1;
@@ -1330,19 +1332,19 @@ int plora_logit_rules(const void* logits, int64_t logits_stride, void* out, int6
   if (st) return st;
   RulesParams p = {};
   p.x = logits, p.y = out, p.x_row = logits_stride, p.y_row = out_stride, p.vocab = vocab;
-  p.tokens = tokens, p.token_row = tokens_stride, p.history = (int32_t)history;
-  p.token_lens = token_lens, p.prompt_lens = prompt_lens;
-  p.repetition = repetition, p.presence = presence, p.frequency = frequency;
-  p.bias_tokens = bias_tokens, p.bias_row = bias_tokens_stride;
-  p.bias_values = bias_values, p.value_row = bias_values_stride, p.biases = (int32_t)biases;
-  p.allowed = reinterpret_cast<const uint32_t*>(allowed), p.mask_row = allowed_stride;
+  p.tokens = tokens, p.token_row = args->tokens_stride, p.history = (int32_t)history;
+  p.token_lens = args->token_lens, p.prompt_lens = args->prompt_lens;
+  p.repetition = args->repetition, p.presence = args->presence, p.frequency = args->frequency;
+  p.bias_tokens = bias_tokens, p.bias_row = args->bias_tokens_stride;
+  p.bias_values = args->bias_values, p.value_row = args->bias_values_stride, p.biases = (int32_t)biases;
+  p.allowed = reinterpret_cast<const uint32_t*>(args->allowed), p.mask_row = args->allowed_stride;
   p.part = a.part;
   if (a.lists) {
     p.list = static_cast<RulesEntry*>(workspace);
     p.listed = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(workspace) + a.listed_offset);
   }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const bool wide = token_bytes == 8;
+  const bool wide = args->token_bytes == 8;
   cudaError_t e = dtype == PLORA_DTYPE_F32   ? launch_rules<float>(p, a, wide, rows, s)
                   : dtype == PLORA_DTYPE_F16 ? launch_rules<__half>(p, a, wide, rows, s)
                                              : launch_rules<__nv_bfloat16>(p, a, wide, rows, s);

@@ -13,7 +13,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _native
-from .paged import _call, _no_grad, _same_device
+from .paged import _current_device, _no_grad, _raw_stream, _same_device
 from .sgmv import _as, dtype_code
 
 
@@ -93,6 +93,9 @@ def apply_logit_rules(logits: torch.Tensor, rules: LogitRules, out: torch.Tensor
             _same_device(dev, logits, t)
     if dev < 0:
         _same_device(dev, logits)
+    if dev != _current_device():
+        with torch.cuda.device(dev):
+            return apply_logit_rules(logits, rules, out)
     _no_grad(logits)
     if logits.dim() != 2:
         raise ValueError("logits must be (B, V)")
@@ -140,15 +143,17 @@ def apply_logit_rules(logits: torch.Tensor, rules: LogitRules, out: torch.Tensor
     rep = _per_row(rules.repetition_penalty, rows, torch.float32, "repetition_penalty")
     pres = _per_row(rules.presence_penalty, rows, torch.float32, "presence_penalty")
     freq = _per_row(rules.frequency_penalty, rows, torch.float32, "frequency_penalty")
-    ws_bytes = _native.load().plora_logit_rules_workspace(rows, vocab, history, biases)
+    lib = _native.load()
+    ws_bytes = lib.plora_logit_rules_workspace(rows, vocab, history, biases)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=logits.device) if ws_bytes else None
-    _call(
-        dev, "plora_logit_rules",
-        logits.data_ptr(), row if rows > 1 else vocab, out.data_ptr(),
-        out.stride(0) if rows > 1 else vocab, rows, vocab, dtype_code(logits.dtype), _ptr(tokens),
-        _row_stride(tokens), history, _ptr(lens), _ptr(prompt), _ptr(rep),
+    args = _native.LOGIT_RULES_ARGS.pack(
+        logits.data_ptr(), row if rows > 1 else vocab, out.data_ptr(), out.stride(0) if rows > 1 else vocab, rows, vocab,
+        dtype_code(logits.dtype), _ptr(tokens), _row_stride(tokens), history, _ptr(lens), _ptr(prompt), _ptr(rep),
         _ptr(pres), _ptr(freq), _ptr(bias_tokens), _row_stride(bias_tokens), _ptr(bias_values),
-        _row_stride(bias_values), biases, _ptr(allowed), _row_stride(allowed), 4 if width == torch.int32 else 8,
+        _row_stride(bias_values), biases, _ptr(allowed), _row_stride(allowed), 4 if width is torch.int32 else 8,
         _ptr(ws), ws_bytes,
     )
+    status = lib.plora_logit_rules(args, _raw_stream(dev))
+    if status:
+        _native.check("plora_logit_rules", status)
     return out

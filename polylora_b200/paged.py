@@ -76,8 +76,8 @@ def _heads(t: torch.Tensor) -> tuple[torch.Tensor, tuple[int, ...], int]:
 
 
 def _check_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor, rows: int, dim: int,
-                 dtype: torch.dtype) -> tuple[int, int, int, int, int, int]:
-    """(num_pages, kv_heads, page_size, k page stride, v page stride, page-table row stride)."""
+                 dtype: torch.dtype) -> tuple[int, int, int, int, int, int, int]:
+    """(num_pages, kv_heads, page_size, k page stride, v page stride, page-table row stride, max_pages)."""
     shape = k_cache.shape
     if len(shape) != 4 or shape != v_cache.shape:
         raise ValueError("k_cache and v_cache must both be (num_pages, kv_heads, page_size, head_dim)")
@@ -95,12 +95,13 @@ def _check_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch
                 raise ValueError(f"{name} pages must be contiguous")
         if pages > 1:
             k_page, v_page = k_cache.stride(0), v_cache.stride(0)
-    if page_table.dtype is not torch.int32 or page_table.dim() != 2 or page_table.shape[0] != rows:
+    table = page_table.shape
+    if page_table.dtype is not torch.int32 or len(table) != 2 or table[0] != rows:
         raise ValueError(f"page_table must be int32 ({rows}, max_pages)")
     row, step = page_table.stride()
-    if step != 1 and page_table.shape[1] > 1:
+    if step != 1 and table[1] > 1:
         raise ValueError("page_table rows must be contiguous")
-    return pages, kv_heads, size, k_page, v_page, row if rows > 1 else page_table.shape[1]
+    return pages, kv_heads, size, k_page, v_page, row if rows > 1 else table[1], table[1]
 
 
 def _lens(t: torch.Tensor, rows: int, name: str) -> torch.Tensor:
@@ -109,15 +110,9 @@ def _lens(t: torch.Tensor, rows: int, name: str) -> torch.Tensor:
     return _as(t, torch.int32)
 
 
-def _call(index: int, func: str, *args: object) -> None:
-    """The entry point on the device's current stream, with the device current."""
-    # the raw handle: a Stream object costs 2 us of a call whose kernel takes less than 3
-    stream = torch._C._cuda_getCurrentRawStream(index)
-    if index == torch.cuda.current_device():
-        _native.call(func, *args, stream)
-    else:
-        with torch.cuda.device(index):
-            _native.call(func, *args, stream)
+# The current stream's raw handle: a Stream object costs 2 us of a call whose kernel takes less than 3.
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch.cuda.current_device
 
 
 def paged_append(
@@ -150,6 +145,10 @@ def paged_append(
     if dev < 0 or not (v.get_device() == k_cache.get_device() == v_cache.get_device() == page_table.get_device()
                        == past_lens.get_device() == dev):
         _same_device(dev, k, v, k_cache, v_cache, page_table, past_lens)
+    if dev != _current_device():
+        with torch.cuda.device(dev):
+            return paged_append(q, k, v, k_cache, v_cache, page_table, past_lens, new_lens, phases=phases,
+                                interleaved=interleaved, rotary_scale=rotary_scale, return_keys=return_keys)
     _no_grad(q, k, v)
     shape, dtype = k.shape, k.dtype
     if len(shape) != 4 or v.shape != shape:
@@ -157,45 +156,52 @@ def paged_append(
     rows, new, kv_heads, dim = shape
     if v.dtype is not dtype:
         raise TypeError("q, k and v must share one dtype")
-    pages, ckv, size, k_page, v_page, table_row = _check_cache(k_cache, v_cache, page_table, rows, dim, dtype)
+    pages, ckv, size, k_page, v_page, table_row, max_pages = _check_cache(k_cache, v_cache, page_table, rows, dim, dtype)
     if ckv != kv_heads:
         raise ValueError(f"kv_heads mismatch: k={kv_heads}, cache={ckv}")
     past = _lens(past_lens, rows, "past_lens")
-    news_ptr = phases_ptr = q_ptr = q_out_ptr = pairs = heads = 0
+    news_ptr = phases_ptr = q_ptr = q_out_ptr = k_out_ptr = pairs = heads = 0
     q_out = k_out = None
     qs = (0, 0, 0)
     if new_lens is not None:
-        _same_device(dev, new_lens)
+        if new_lens.get_device() != dev:
+            _same_device(dev, new_lens)
         new_lens = _lens(new_lens, rows, "new_lens")
         news_ptr = new_lens.data_ptr()
     if phases is not None:
-        _same_device(dev, phases)
+        if phases.get_device() != dev:
+            _same_device(dev, phases)
         if phases.dim() != 1 or phases.dtype is not torch.int64:
             raise ValueError("phases must be the int64 tensor of rotary_phases()")
         pairs = phases.shape[0]
         phases = phases.contiguous()
         phases_ptr = phases.data_ptr() if pairs else 0
     if q is not None:
-        _same_device(dev, q)
-        if q.dim() != 4 or q.shape[0] != rows or q.shape[1] != new or q.shape[3] != dim:
-            raise ValueError("q must be (B, M, heads, D), k and v (B, M, kv_heads, D)")
+        if q.get_device() != dev:
+            _same_device(dev, q)
         if q.dtype is not dtype:
             raise TypeError("q, k and v must share one dtype")
-        heads = q.shape[2]
-        q, qs, q_ptr = _heads(q)
-        q_out = torch.empty_like(q) if q.is_contiguous() else q.new_empty((rows, new, heads, dim))
+        shape = q.shape
+        if len(shape) != 4 or shape[0] != rows or shape[1] != new or shape[3] != dim:
+            raise ValueError("q must be (B, M, heads, D), k and v (B, M, kv_heads, D)")
+        heads = shape[2]
+        q_out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(shape)
         q_out_ptr = q_out.data_ptr()
+        q, qs, q_ptr = _heads(q)
     k, ks, k_ptr = _heads(k)
     v, vs, v_ptr = _heads(v)
     if return_keys:
         k_out = k.new_empty((rows, new, kv_heads, dim))
-    _call(
-        dev, "plora_paged_append",
-        q_ptr, qs[0], qs[1], qs[2], k_ptr, ks[0], ks[1], ks[2], v_ptr, vs[0], vs[1], vs[2], q_out_ptr,
-        k_out.data_ptr() if return_keys else 0, k_cache.data_ptr(), v_cache.data_ptr(), k_page, v_page,
-        page_table.data_ptr(), table_row, past.data_ptr(), news_ptr, phases_ptr, pairs, interleaved,
-        rotary_scale, rows, new, heads, kv_heads, dim, size, pages, page_table.shape[1], dtype_code(dtype),
+        k_out_ptr = k_out.data_ptr()
+    args = _native.PAGED_APPEND_ARGS.pack(
+        k_cache.data_ptr(), v_cache.data_ptr(), k_page, v_page, page_table.data_ptr(), table_row, rows, heads, kv_heads,
+        dim, size, pages, max_pages, dtype_code(dtype),
+        q_ptr, qs[0], qs[1], qs[2], k_ptr, ks[0], ks[1], ks[2], v_ptr, vs[0], vs[1], vs[2],
+        q_out_ptr, k_out_ptr, past.data_ptr(), news_ptr, phases_ptr, pairs, interleaved, new, rotary_scale,
     )
+    status = _native.load().plora_paged_append(args, _raw_stream(dev))
+    if status:
+        _native.check("plora_paged_append", status)
     return q_out, k_out
 
 
@@ -218,28 +224,34 @@ def paged_attention(
     if dev < 0 or not (k_cache.get_device() == v_cache.get_device() == page_table.get_device() == seq_lens.get_device()
                        == dev):
         _same_device(dev, q, k_cache, v_cache, page_table, seq_lens)
+    if dev != _current_device():
+        with torch.cuda.device(dev):
+            return paged_attention(q, k_cache, v_cache, page_table, seq_lens, scale=scale, window=window, out=out)
     _no_grad(q)
-    if q.dim() != 3:
+    shape, dtype = q.shape, q.dtype
+    if len(shape) != 3:
         raise ValueError("q must be (B, heads, D)")
-    rows, heads, dim = q.shape
-    dtype = q.dtype
-    pages, kv_heads, size, k_page, v_page, table_row = _check_cache(k_cache, v_cache, page_table, rows, dim, dtype)
+    rows, heads, dim = shape
+    pages, kv_heads, size, k_page, v_page, table_row, max_pages = _check_cache(k_cache, v_cache, page_table, rows, dim,
+                                                                               dtype)
     if heads == 0 or kv_heads == 0 or heads % kv_heads:
         raise ValueError(f"{heads} heads over {kv_heads} kv heads")
     lens = _lens(seq_lens, rows, "seq_lens")
     if out is None:
-        out = torch.empty_like(q) if q.is_contiguous() else q.new_empty((rows, heads, dim))
-    elif out.shape != q.shape or out.dtype is not dtype or out.get_device() != dev or not out.is_contiguous():
+        out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(shape)
+    elif out.shape != shape or out.dtype is not dtype or out.get_device() != dev or not out.is_contiguous():
         raise ValueError("out must be a contiguous tensor of q's shape, dtype and device")
     q, qs, q_ptr = _heads(q)
-    code = dtype_code(dtype)
-    max_pages = page_table.shape[1]
-    ws_bytes = _native.load().plora_paged_attention_workspace(rows, heads, kv_heads, dim, size, max_pages, window, code)
+    code, lib = dtype_code(dtype), _native.load()
+    ws_bytes = lib.plora_paged_attention_workspace(rows, heads, kv_heads, dim, size, max_pages, window, code)
     ws = lens.new_empty(ws_bytes // 4) if ws_bytes else None
-    _call(
-        dev, "plora_paged_attention",
-        q_ptr, qs[0], qs[1], k_cache.data_ptr(), v_cache.data_ptr(), k_page, v_page, page_table.data_ptr(),
-        table_row, lens.data_ptr(), out.data_ptr(), dim**-0.5 if scale is None else scale, window, rows, heads,
-        kv_heads, dim, size, pages, max_pages, code, ws.data_ptr() if ws_bytes else 0, ws_bytes,
+    args = _native.PAGED_ATTENTION_ARGS.pack(
+        k_cache.data_ptr(), v_cache.data_ptr(), k_page, v_page, page_table.data_ptr(), table_row, rows, heads, kv_heads,
+        dim, size, pages, max_pages, code,
+        q_ptr, qs[0], qs[1], lens.data_ptr(), out.data_ptr(), dim**-0.5 if scale is None else scale, window,
+        ws.data_ptr() if ws_bytes else 0, ws_bytes,
     )
+    status = lib.plora_paged_attention(args, _raw_stream(dev))
+    if status:
+        _native.check("plora_paged_attention", status)
     return out

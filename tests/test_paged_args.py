@@ -17,19 +17,21 @@ def _append(lib, native, **kw):
              kp=4096, vp=4096, table=D, ts=4, past=D, news=None, phases=D, pairs=32, inter=0, scale=1.0, rows=2, new=2,
              heads=16, kv=4, dim=64, page=16, pages=8, width=4, dtype=native.DTYPE_BF16)
     a.update(kw)
-    return lib.plora_paged_append(a["q"], *a["qs"], a["k"], *a["ks"], a["v"], *a["vs"], a["q_out"], a["k_out"], a["kc"],
-                                  a["vc"], a["kp"], a["vp"], a["table"], a["ts"], a["past"], a["news"], a["phases"],
-                                  a["pairs"], a["inter"], a["scale"], a["rows"], a["new"], a["heads"], a["kv"], a["dim"],
-                                  a["page"], a["pages"], a["width"], a["dtype"], None)
+    return lib.plora_paged_append(native.PAGED_APPEND_ARGS.pack(
+        a["kc"] or 0, a["vc"] or 0, a["kp"], a["vp"], a["table"] or 0, a["ts"], a["rows"], a["heads"], a["kv"], a["dim"],
+        a["page"], a["pages"], a["width"], a["dtype"], a["q"] or 0, *a["qs"], a["k"] or 0, *a["ks"], a["v"] or 0, *a["vs"],
+        a["q_out"] or 0, a["k_out"] or 0, a["past"] or 0, a["news"] or 0, a["phases"] or 0, a["pairs"], a["inter"], a["new"],
+        a["scale"]), None)
 
 
 def _attend(lib, native, **kw):
     a = dict(q=D, qs=(1024, 64), kc=D, vc=D, kp=4096, vp=4096, table=D, ts=4, lens=D, out=D, scale=0.125, window=0,
              rows=2, heads=16, kv=4, dim=64, page=16, pages=8, width=4, dtype=native.DTYPE_BF16, ws=D, wb=1 << 30)
     a.update(kw)
-    return lib.plora_paged_attention(a["q"], *a["qs"], a["kc"], a["vc"], a["kp"], a["vp"], a["table"], a["ts"], a["lens"],
-                                     a["out"], a["scale"], a["window"], a["rows"], a["heads"], a["kv"], a["dim"],
-                                     a["page"], a["pages"], a["width"], a["dtype"], a["ws"], a["wb"], None)
+    return lib.plora_paged_attention(native.PAGED_ATTENTION_ARGS.pack(
+        a["kc"] or 0, a["vc"] or 0, a["kp"], a["vp"], a["table"] or 0, a["ts"], a["rows"], a["heads"], a["kv"], a["dim"],
+        a["page"], a["pages"], a["width"], a["dtype"], a["q"] or 0, *a["qs"], a["lens"] or 0, a["out"] or 0, a["scale"],
+        a["window"], a["ws"] or 0, a["wb"]), None)
 
 
 SHARED = [
@@ -39,7 +41,8 @@ SHARED = [
     (dict(width=1 << 28, ts=1 << 28), "UNSUPPORTED"), (dict(kp=4095), "INVALID"), (dict(vp=4100), "INVALID"),
     (dict(ts=3), "INVALID"), (dict(kc=D + 8), "INVALID"), (dict(kc=None), "INVALID"), (dict(table=None), "INVALID"),
     (dict(q=D + 2), "INVALID"), (dict(kv=60000, heads=60000, page=1 << 20), "UNSUPPORTED"),
-    (dict(pages=1 << 30, kp=1 << 40, vp=1 << 40), "INVALID"),
+    (dict(pages=1 << 30, kp=1 << 40, vp=1 << 40), "INVALID"), (dict(dtype=1 << 32), "INVALID"),
+    (dict(heads=1 << 40), "UNSUPPORTED"), (dict(page=1 << 33), "UNSUPPORTED"), (dict(dim=(1 << 32) + 64), "UNSUPPORTED"),
 ]
 
 
@@ -86,9 +89,10 @@ def test_rules_arguments_rejected_before_cuda(native):
         a = dict(x=D, xs=100, y=D, ys=100, rows=2, vocab=100, dtype=native.DTYPE_BF16, tok=D, tr=8, hist=8, bt=D, br=4,
                  bv=D, vr=4, k=4, mask=None, mr=0, tb=8, ws=D, wb=1 << 30)
         a.update(kw)
-        return lib.plora_logit_rules(a["x"], a["xs"], a["y"], a["ys"], a["rows"], a["vocab"], a["dtype"], a["tok"], a["tr"],
-                                     a["hist"], None, None, None, None, None, a["bt"], a["br"], a["bv"], a["vr"], a["k"],
-                                     a["mask"], a["mr"], a["tb"], a["ws"], a["wb"], None)
+        return lib.plora_logit_rules(native.LOGIT_RULES_ARGS.pack(
+            a["x"] or 0, a["xs"], a["y"] or 0, a["ys"], a["rows"], a["vocab"], a["dtype"], a["tok"] or 0, a["tr"], a["hist"],
+            0, 0, 0, 0, 0, a["bt"] or 0, a["br"], a["bv"] or 0, a["vr"], a["k"], a["mask"] or 0, a["mr"], a["tb"],
+            a["ws"] or 0, a["wb"]), None)
 
     for kw in (dict(dtype=3), dict(rows=-1), dict(vocab=-1), dict(hist=-1), dict(k=-1), dict(tb=2), dict(x=None),
                dict(y=None), dict(tok=None), dict(bt=None), dict(bv=None), dict(xs=99), dict(ys=99), dict(tr=-1),
@@ -143,3 +147,32 @@ def test_heads_copies_only_what_it_must():
         assert got.is_contiguous() and got.data_ptr() == ptr and ptr % 16 == 0
         assert other.shape[-1] % 8 or all(s % 8 == 0 for s in st[:-1])  # heads that the operators take
     assert _heads(torch.zeros(1, 2, 4, 16, dtype=torch.bfloat16).as_strided((1, 2, 4, 16), (7, 64, 16, 1)))[1][0] % 8 == 0
+
+
+def test_argument_structs_match_the_header(native, tmp_path):
+    """The packed layouts are the C structs' (sizes and the offset of every
+    section, from a compiled program), and null arguments are refused."""
+    import shutil
+    import subprocess
+    from pathlib import Path
+
+    lib = native.load()
+    for fn in (lib.plora_paged_append, lib.plora_paged_attention, lib.plora_logit_rules):
+        assert fn(None, None) == native.ERR_INVALID_ARGUMENT
+    cc = shutil.which("gcc") or shutil.which("cc")
+    if cc is None:
+        pytest.skip("no C compiler")
+    src = tmp_path / "sizes.c"
+    src.write_text('#include "polylora_b200.h"\n#include <stdio.h>\n#define P(x) printf("%d\\n", (int)(x))\n'
+                   "int main(void) { P(sizeof(plora_paged_append_args)); P(sizeof(plora_paged_attention_args));"
+                   "P(sizeof(plora_logit_rules_args)); P(offsetof(plora_paged_append_args, q));"
+                   "P(offsetof(plora_paged_append_args, q_out)); P(offsetof(plora_paged_append_args, rotary_scale));"
+                   "P(offsetof(plora_paged_attention_args, q)); P(offsetof(plora_paged_attention_args, scale));"
+                   "P(offsetof(plora_paged_attention_args, workspace)); P(offsetof(plora_logit_rules_args, allowed));"
+                   "return 0; }\n")
+    include = Path(__file__).resolve().parents[1] / "include"
+    subprocess.run([cc, "-std=c11", f"-I{include}", str(src), "-o", str(tmp_path / "sizes")], check=True)
+    got = subprocess.run([str(tmp_path / "sizes")], capture_output=True, text=True, check=True).stdout.split()
+    want = [native.PAGED_APPEND_ARGS.size, native.PAGED_ATTENTION_ARGS.size, native.LOGIT_RULES_ARGS.size, 14 * 8, 26 * 8,
+            34 * 8, 14 * 8, 19 * 8, 21 * 8, 20 * 8]
+    assert [int(x) for x in got] == want
