@@ -1099,9 +1099,10 @@ __global__ void __launch_bounds__(AttnMmaCfg<DP, NT>::kWarps * 32, 1)
   // transposed (token (l & 7) + 8 (l / 16), chunk 2 mt + (l / 8) % 2); four chunk
   // pairs make a block, so step j adds a block and one of four offsets
   const int krow = lane & 15, vrow = (lane & 7) + ((lane >> 4) << 3);
-  uint32_t koff[4], voff[4];
+  uint32_t koff[4], voff[4], qoff[4];  // qoff: shared queries, head (l & 7) + 8 (l / 16), chunk 2 ks + (l / 8) % 2
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
+    qoff[j] = vrow * DP * 2 + (((2 * j + ((lane >> 3) & 1)) ^ (lane & 7)) << 4);
     koff[j] = Tile::offset(krow, 2 * j + (lane >> 4));
     voff[j] = Tile::kTileBytes + Tile::offset(vrow, 2 * j + ((lane >> 3) & 1));
   }
@@ -1174,16 +1175,18 @@ __global__ void __launch_bounds__(AttnMmaCfg<DP, NT>::kWarps * 32, 1)
       if (!TMA && ks * 16 >= p.c.dim) break;
       uint32_t a[4];
       ldsm_x4(base + koff[ks & 3] + (ks >> 2) * (kAttnTile * 128), a);
+      if constexpr (Cfg::kQShared) {
+        static_assert(!Cfg::kQShared || NT % 2 == 0, "two groups of eight heads at a time");
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        if constexpr (Cfg::kQShared) {
-          uint32_t b[4];  // two matrices, named by both halves of the warp
-          const int h = nt * 8 + (lane & 7);
-          ldsm_x4(sq + h * (DP * 2) + (((2 * ks + ((lane >> 3) & 1)) ^ (h & 7)) << 4), b);
+        for (int nt = 0; nt < NT; nt += 2) {
+          uint32_t b[4];
+          ldsm_x4(sq + qoff[ks & 3] + nt * 8 * DP * 2 + (ks >> 2) * 128, b);
           mma_16816<BF16>(sc[nt][ks & 1], a, b[0], b[1]);
-        } else {
-          mma_16816<BF16>(sc[nt][ks & 1], a, qf[nt][ks][0], qf[nt][ks][1]);
+          mma_16816<BF16>(sc[nt + 1][ks & 1], a, b[2], b[3]);
         }
+      } else {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) mma_16816<BF16>(sc[nt][ks & 1], a, qf[nt][ks][0], qf[nt][ks][1]);
       }
     }
     const int p0 = at.tile * kAttnTile + (lane >> 2);  // this lane's tokens: p0, p0 + 8
