@@ -278,7 +278,7 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const Appe
 // segments, which warps stream through a ring of shared-memory stages of their
 // own, with no barrier between them.
 //
-// Where there is much to do, the first three quarters of the list are dealt in
+// Where there is much to do, the first 13/16 of the list are dealt in
 // equal segments to the grid's warps and the rest in small ones to whoever asks
 // next: SMs of a GPC share its way to memory, and with equal shares alone the
 // slowest warp of a 2 GB call ended 17 % after the mean (325 and 277 us).  The
@@ -429,7 +429,7 @@ __global__ void __launch_bounds__(kAttnPlanThreads) attn_plan_kernel(const AttnP
       w.asked = 0, w.chunk = 1;
     } else {
       w.dealt = warps;
-      w.base = (int)(w.total / 4 * 3 / warps);
+      w.base = (int)(w.total / 16 * 13 / warps);
       w.rem = 0;
       const int64_t rest = w.total - (int64_t)w.base * warps;
       const int most = attn_asked_max(warps, p.block_heads);
@@ -1298,7 +1298,7 @@ __global__ void __launch_bounds__(AttnMmaCfg<DP, NT>::kWarps * 32, 1)
 // Joins the parts of the items that segments cut.  Of an item of up to 32 parts a
 // warp takes a head, one part after the other; of more parts, a CTA takes 32
 // elements of a head, each warp a run of parts, four of them at a time.
-constexpr int kJoinWarps = 8, kJoinGrid = 4 * 148, kJoinSlice = 32;
+constexpr int kJoinWarps = 8, kJoinGrid = 3 * 148, kJoinSlice = 32;
 
 // Sums of one head of an item from its parts; a lane holds four elements.
 struct AttnSum {
