@@ -698,7 +698,7 @@ AttnPlan attn_plan(int64_t rows, int32_t heads, int32_t kv_heads, int32_t dim, i
   // Without a list where the SMs hold all items at once with few tiles a warp, as
   // far as the page table's width tells: the lengths are on the device.  One row
   // of 200 tokens: 5 us against 10.
-  const int64_t tokens = window > 0 ? std::min(capacity, window + kAttnTile - 1) : capacity;
+  const int64_t tokens = window > 0 && window < capacity ? std::min(capacity, window + kAttnTile - 1) : capacity;
   const int64_t tiles = (tokens + kAttnTile - 1) / kAttnTile, items = rows * kv_heads * a.blocks;
   // Clusters of 1, 2, ... CTAs, one CTA an SM, that the GPU holds at once (what
   // cudaOccupancyMaxActiveClusters says there, a few left out): a cluster lies in one GPC.

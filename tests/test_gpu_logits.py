@@ -180,9 +180,9 @@ def test_strided_lists_and_mixed_types(cuda_status_clean):
     _check(apply_logit_rules(x.to(dev), d), ref, slack, FH)
 
 
-def test_captured_rules_follow_their_buffers(cuda_status_clean):
+@pytest.mark.parametrize("B,V", [(3, 40000), (300, 5000)])  # rules by their finders, and by lists
+def test_captured_rules_follow_their_buffers(cuda_status_clean, B, V):
     dev, g = torch.device("cuda"), torch.Generator().manual_seed(4)
-    B, V = 3, 40000
     x = torch.randn(B, V, generator=g).to(BF).to(dev)
     r = _to(_rules(g, B, V, 64, 16, True, True), dev)
     out = torch.empty_like(x)
@@ -190,11 +190,32 @@ def test_captured_rules_follow_their_buffers(cuda_status_clean):
     apply_logit_rules(x, r, out=out)
     with torch.cuda.graph(gr):
         apply_logit_rules(x, r, out=out)
-    r.tokens.random_(0, V)
-    r.token_lens.fill_(64)
-    x.mul_(0.5)
-    gr.replay()
-    assert torch.equal(out, apply_logit_rules(x, r))
+    for k in range(3):
+        r.tokens.random_(0, V)
+        r.token_lens.fill_(64 - k)
+        x.mul_(0.5)
+        gr.replay()
+        assert torch.equal(out, apply_logit_rules(x, r))
+        got = x.clone()
+        assert torch.equal(apply_logit_rules(got, r, out=got), out)
+
+
+def test_two_streams_of_listed_rules(cuda_status_clean):
+    dev, g = torch.device("cuda"), torch.Generator().manual_seed(5)
+    B, V = 300, 20000
+    xs = [torch.randn(B, V, generator=g).to(BF).to(dev) for _ in range(2)]
+    rs = [_to(_rules(g, B, V, 200, 16, True, True), dev) for _ in range(2)]
+    want = [apply_logit_rules(x, r) for x, r in zip(xs, rs)]
+    streams = [torch.cuda.Stream() for _ in xs]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(6):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(apply_logit_rules(xs[i], rs[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(y, want[i]) for y in got[i])
 
 
 def test_empty(cuda_status_clean):

@@ -336,15 +336,17 @@ def test_attention_past_32_bit_offsets(cuda_status_clean):
     assert torch.equal(paged_attention(q[:, 0], kc, vc, table, lens), paged_attention(q[:, 0], sk, sv, small, lens))
 
 
-def test_two_streams_and_two_graphs(cuda_status_clean):
+@pytest.mark.parametrize("longest,width", [(3000, 256), (60000, 4096)])
+def test_two_streams_and_two_graphs(cuda_status_clean, longest, width):
     """Calls on two streams at once, and two graphs captured one after the
-    other and replayed at once with new lengths, give the single calls' bits."""
+    other and replayed at once with new lengths, give the single calls' bits;
+    short rows (one launch) and long ones (a list of segments)."""
     g, dev = _gen(12), _dev()
     H, KV, D, page = 16, 4, 128, 16
     sets = []
-    for n in (3000, 2500):
+    for n in (longest, longest - 500):
         lens = [n, 17, n // 2]
-        table, pages = _table(lens, page, g, width=256)
+        table, pages = _table(lens, page, g, width=width)
         sets.append([torch.randn(3, H, D, generator=g).to(BF).to(dev)]
                     + [torch.randn(pages, KV, page, D, generator=g).to(BF).to(dev) for _ in range(2)]
                     + [table.to(dev), torch.tensor(lens, dtype=torch.int32, device=dev)])
@@ -410,3 +412,29 @@ def test_expired_wait_is_reported_and_clears(native, lens):
     assert status in ((0, _native.DEV_WAIT_TIMEOUT) if lens[0] < 1000 else (_native.DEV_WAIT_TIMEOUT,))
     assert torch.equal(paged_attention(*args), want)
     assert native.device_status(clear=True) == 0
+
+
+def test_shared_prefix_of_many_rows_and_a_window_of_any_size(cuda_status_clean):
+    """Rows that read the same pages, and windows beyond the tokens up to the
+    largest number, agree with the plain call."""
+    g, dev = _gen(14), _dev()
+    kc, vc = (torch.randn(20, 2, 16, 64, generator=g).to(BF).to(dev) for _ in range(2))
+    table = torch.arange(20, dtype=torch.int32, device=dev).view(1, 20).expand(300, 20).contiguous()
+    lens = torch.arange(300, dtype=torch.int32, device=dev)
+    q = torch.randn(1, 4, 64, generator=g).to(BF).to(dev).expand(300, 4, 64)
+    want = paged_attention(q, kc, vc, table, lens)
+    assert torch.equal(paged_attention(q, kc, vc, table, lens, window=2**63 - 1), want)
+    one = paged_attention(q[250:251], kc, vc, table[:1], lens[250:251])
+    assert torch.allclose(one.float(), want[250:251].float(), atol=2 * HALF[BF], rtol=2 * HALF[BF])
+    assert torch.equal(paged_attention(q, kc, vc, table, lens, out=torch.empty_like(want)), want)
+
+
+def test_queries_may_be_overwritten(cuda_status_clean):
+    g, dev = _gen(15), _dev()
+    for lens, width in (([70, 3], 8), ([30000, 20000], 2000)):
+        table, pages = _table(lens, 16, g, width=width)
+        q = torch.randn(2, 8, 128, generator=g).to(BF).to(dev)
+        kc, vc = (torch.randn(pages, 2, 16, 128, generator=g).to(BF).to(dev) for _ in range(2))
+        n = torch.tensor(lens, dtype=torch.int32, device=dev)
+        want = paged_attention(q, kc, vc, table.to(dev), n)
+        assert torch.equal(paged_attention(q, kc, vc, table.to(dev), n, out=q), want) and torch.equal(q, want)
