@@ -14,7 +14,7 @@ import torch
 
 from . import _native
 from .paged import _current_device, _no_grad, _raw_stream, _same_device
-from .sgmv import _as, dtype_code
+from .sgmv import dtype_code
 
 
 @dataclass
@@ -55,42 +55,30 @@ class LogitRules:
             if mine is not None:
                 mine.copy_(theirs, non_blocking=True)
 
-    def tensors(self) -> list[torch.Tensor]:
-        every = (self.tokens, self.token_lens, self.prompt_lens, self.repetition_penalty, self.presence_penalty,
-                 self.frequency_penalty, self.bias_tokens, self.bias_values, self.allowed)
-        return [t for t in every if t is not None]
+
+def _matrix(t: torch.Tensor, dev: int, rows: int, name: str) -> torch.Tensor:
+    """A (rows, n) list with dense rows (a copy where they are not)."""
+    if t.get_device() != dev:
+        _same_device(dev, t)
+    shape = t.shape
+    if len(shape) != 2 or shape[0] != rows:
+        raise ValueError(f"{name} must be 2D with {rows} rows, got {tuple(shape)}")
+    return t if shape[1] <= 1 or t.stride(1) == 1 else t.contiguous()
 
 
-def _rows_of(t: torch.Tensor, rows: int, name: str) -> torch.Tensor:
-    if t.dim() != 2 or t.shape[0] != rows:
-        raise ValueError(f"{name} must be 2D with {rows} rows, got {tuple(t.shape)}")
-    return t if t.shape[1] <= 1 or t.stride(1) == 1 else t.contiguous()
-
-
-def _per_row(t: torch.Tensor | None, rows: int, dtype: torch.dtype, name: str) -> torch.Tensor | None:
-    if t is None:
-        return None
+def _vector(t: torch.Tensor, dev: int, rows: int, dtype: torch.dtype, name: str) -> torch.Tensor:
+    """One dense value of ``dtype`` per row."""
+    if t.get_device() != dev:
+        _same_device(dev, t)
     if t.dim() != 1 or t.shape[0] != rows:
         raise ValueError(f"{name} must have shape ({rows},), got {tuple(t.shape)}")
-    return _as(t, dtype)
-
-
-def _ptr(t: torch.Tensor | None) -> int:
-    return t.data_ptr() if t is not None else 0
-
-
-def _row_stride(t: torch.Tensor | None) -> int:
-    return t.stride(0) if t is not None else 0
+    return t if t.dtype is dtype and t.is_contiguous() else t.to(dtype).contiguous()
 
 
 def apply_logit_rules(logits: torch.Tensor, rules: LogitRules, out: torch.Tensor | None = None) -> torch.Tensor:
     """``rules`` on logits (B, V), computed in fp32 and rounded once to the
     logits' dtype; into ``out`` (which may be ``logits``) or a new tensor."""
     dev = logits.get_device()
-    tokens, bias_tokens, bias_values, allowed = rules.tokens, rules.bias_tokens, rules.bias_values, rules.allowed
-    for t in rules.tensors():
-        if t.get_device() != dev or dev < 0:
-            _same_device(dev, logits, t)
     if dev < 0:
         _same_device(dev, logits)
     if dev != _current_device():
@@ -108,16 +96,34 @@ def apply_logit_rules(logits: torch.Tensor, rules: LogitRules, out: torch.Tensor
     elif out is not logits and (out.shape != logits.shape or out.dtype is not logits.dtype or out.get_device() != dev
                                 or (vocab > 1 and out.stride(1) != 1)):
         raise ValueError("out must have the logits' shape, dtype and device, with contiguous rows")
+    lens, prompt, rep, pres, freq = (rules.token_lens, rules.prompt_lens, rules.repetition_penalty,
+                                     rules.presence_penalty, rules.frequency_penalty)
+    tokens, bias_tokens, bias_values, allowed = rules.tokens, rules.bias_tokens, rules.bias_values, rules.allowed
     width = None
-    history = biases = 0
+    history = biases = token_row = bias_row = value_row = mask_row = 0
+    lens_ptr = prompt_ptr = rep_ptr = pres_ptr = freq_ptr = 0
     if tokens is not None:
         width = tokens.dtype
         if width is not torch.int64 and width is not torch.int32:
             raise TypeError(f"tokens must be int32 or int64, got {width}")
-        tokens = _rows_of(tokens, rows, "tokens")
+        tokens = _matrix(tokens, dev, rows, "tokens")
         history = tokens.shape[1]
-    elif not (rules.token_lens is rules.prompt_lens is rules.repetition_penalty is rules.presence_penalty
-              is rules.frequency_penalty is None):
+        if lens is not None:
+            lens = _vector(lens, dev, rows, torch.int32, "token_lens")
+            lens_ptr = lens.data_ptr()
+        if prompt is not None:
+            prompt = _vector(prompt, dev, rows, torch.int32, "prompt_lens")
+            prompt_ptr = prompt.data_ptr()
+        if rep is not None:
+            rep = _vector(rep, dev, rows, torch.float32, "repetition_penalty")
+            rep_ptr = rep.data_ptr()
+        if pres is not None:
+            pres = _vector(pres, dev, rows, torch.float32, "presence_penalty")
+            pres_ptr = pres.data_ptr()
+        if freq is not None:
+            freq = _vector(freq, dev, rows, torch.float32, "frequency_penalty")
+            freq_ptr = freq.data_ptr()
+    elif not (lens is prompt is rep is pres is freq is None):
         raise ValueError("penalties and lengths need tokens")
     if (bias_tokens is None) != (bias_values is None):
         raise ValueError("bias_tokens and bias_values go together")
@@ -126,32 +132,30 @@ def apply_logit_rules(logits: torch.Tensor, rules: LogitRules, out: torch.Tensor
             raise TypeError(f"bias_tokens must be int32 or int64, got {bias_tokens.dtype}")
         if bias_tokens.shape != bias_values.shape:
             raise ValueError("bias_tokens and bias_values must have one shape")
-        bias_tokens = _rows_of(bias_tokens, rows, "bias_tokens")
+        bias_tokens = _matrix(bias_tokens, dev, rows, "bias_tokens")
         if width is not None and bias_tokens.dtype is not width:  # both as the wider: narrowing could alias ids
             tokens, bias_tokens = tokens.to(torch.int64), bias_tokens.to(torch.int64)
         width = bias_tokens.dtype
         if bias_values.dtype is not torch.float32:
             bias_values = bias_values.to(torch.float32)
-        bias_values = _rows_of(bias_values, rows, "bias_values")
-        biases = bias_tokens.shape[1]
+        bias_values = _matrix(bias_values, dev, rows, "bias_values")
+        biases, bias_row, value_row = bias_tokens.shape[1], bias_tokens.stride(0), bias_values.stride(0)
+    if tokens is not None:
+        token_row = tokens.stride(0)
     if allowed is not None:
         if allowed.dtype is not torch.int32 or allowed.dim() != 2 or allowed.shape[1] < (vocab + 31) // 32:
             raise ValueError(f"allowed must be int32 ({rows}, at least {(vocab + 31) // 32})")
-        allowed = _rows_of(allowed, rows, "allowed")
-    lens = _per_row(rules.token_lens, rows, torch.int32, "token_lens")
-    prompt = _per_row(rules.prompt_lens, rows, torch.int32, "prompt_lens")
-    rep = _per_row(rules.repetition_penalty, rows, torch.float32, "repetition_penalty")
-    pres = _per_row(rules.presence_penalty, rows, torch.float32, "presence_penalty")
-    freq = _per_row(rules.frequency_penalty, rows, torch.float32, "frequency_penalty")
+        allowed = _matrix(allowed, dev, rows, "allowed")
+        mask_row = allowed.stride(0)
     lib = _native.load()
     ws_bytes = lib.plora_logit_rules_workspace(rows, vocab, history, biases)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=logits.device) if ws_bytes else None
     args = _native.LOGIT_RULES_ARGS.pack(
         logits.data_ptr(), row if rows > 1 else vocab, out.data_ptr(), out.stride(0) if rows > 1 else vocab, rows, vocab,
-        dtype_code(logits.dtype), _ptr(tokens), _row_stride(tokens), history, _ptr(lens), _ptr(prompt), _ptr(rep),
-        _ptr(pres), _ptr(freq), _ptr(bias_tokens), _row_stride(bias_tokens), _ptr(bias_values),
-        _row_stride(bias_values), biases, _ptr(allowed), _row_stride(allowed), 4 if width is torch.int32 else 8,
-        _ptr(ws), ws_bytes,
+        dtype_code(logits.dtype), tokens.data_ptr() if tokens is not None else 0, token_row, history, lens_ptr, prompt_ptr,
+        rep_ptr, pres_ptr, freq_ptr, bias_tokens.data_ptr() if biases else 0, bias_row,
+        bias_values.data_ptr() if biases else 0, value_row, biases, allowed.data_ptr() if allowed is not None else 0,
+        mask_row, 4 if width is torch.int32 else 8, ws.data_ptr() if ws_bytes else 0, ws_bytes,
     )
     status = lib.plora_logit_rules(args, _raw_stream(dev))
     if status:
