@@ -229,6 +229,25 @@ def _window(module: nn.Module) -> int:
     return int(window or 0)
 
 
+def _check_attention(module: nn.Module) -> None:
+    """Refuses attention that ``_PagedAttentionForward`` would answer differently:
+    it projects, rotates, and takes a causal softmax of the scaled products."""
+    config = getattr(module, "config", None)
+    own = [n for n, _ in module.named_parameters(recurse=False)] + [n for n, _ in module.named_buffers(recurse=False)]
+    if own:  # such as learned attention sinks
+        raise ValueError(f"an attention module has parameters of its own: {', '.join(own)}")
+    if not getattr(module, "is_causal", True):
+        raise ValueError("an attention module is not causal")
+    if not getattr(module, "use_rope", True):
+        raise ValueError("an attention module does not rotate its queries and keys")
+    for name in ("attn_logit_softcapping", "clip_qkv"):
+        if getattr(module, name, None) is not None or getattr(config, name, None) is not None:
+            raise ValueError(f"an attention module has {name}")
+    types = getattr(config, "layer_types", None)
+    if types is not None and types[module.layer_idx] not in ("full_attention", "sliding_attention"):
+        raise ValueError(f"an attention layer is of type {types[module.layer_idx]!r}")
+
+
 _PROJECTIONS = {"q_proj", "k_proj", "v_proj", "o_proj"}
 
 
@@ -258,6 +277,7 @@ def attach(model: nn.Module, cache: PagedKVCache, inv_freq: torch.Tensor | None 
         raise ValueError(f"the model has {len(modules)} attention modules, the cache {cache.num_layers} layers")
     _, _, kv_heads, _, head_dim = cache.k.shape
     for m in modules:
+        _check_attention(m)
         if int(m.head_dim) != head_dim or m.k_proj.out_features != kv_heads * head_dim:
             raise ValueError(f"an attention module has {m.k_proj.out_features} key features in heads of {m.head_dim}, "
                              f"the cache {kv_heads} heads of {head_dim}")

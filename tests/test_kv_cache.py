@@ -129,6 +129,23 @@ def test_attach_refusals():
         model.attach_kv_cache(_cache())
 
 
+@pytest.mark.parametrize("name,value,match", [
+    ("sinks", torch.nn.Parameter(torch.zeros(4)), "sinks"), ("is_causal", False, "causal"), ("use_rope", 0, "rotate"),
+    ("attn_logit_softcapping", 50.0, "softcapping"), ("config.clip_qkv", 8.0, "clip_qkv"),
+    ("config.layer_types", ["full_attention", "chunked_attention"], "chunked"),
+])
+def test_attach_refuses_other_attention(name, value, match):
+    """Terms that the paged forward leaves out, in any layer."""
+    model = _wrapped(_llama())
+    module = attention_modules(model.base_model)[1]
+    owner = module.config if name.startswith("config.") else module
+    setattr(owner, name.removeprefix("config."), value)
+    forward = module.forward
+    with pytest.raises(ValueError, match=match):
+        model.attach_kv_cache(_cache())
+    assert module.forward == forward  # nothing attached
+
+
 def test_forward_refusals():
     model, cache = _wrapped(_llama()), _cache()
     model.attach_kv_cache(cache)
