@@ -329,8 +329,8 @@ int plora_peft_pack(const char* path, const char* const* modules, int32_t num_mo
  * takes position past_lens[b] + m.  q (rows, max_new, q_heads, head_dim; null:
  * none) and k (.., kv_heads, ..) are rotated, k and v written to their pages,
  * rotated queries to q_out and, if k_out is not null, rotated keys to k_out,
- * both dense; padded tokens (m >= new_lens[b]) are zeros there and leave the
- * cache alone.  The first 2 * pairs elements of a head rotate, element i with
+ * both dense and apart from the inputs and the cache; padded tokens (m >=
+ * new_lens[b]) are zeros there and leave the cache alone.  The first 2 * pairs elements of a head rotate, element i with
  * i + pairs, or 2i with 2i + 1 when interleaved != 0, by position * f_i;
  * phases[i] = round(f_i / (2 pi) * 2^64) mod 2^64, cosines and sines times
  * rotary_scale.  pairs 0: no rotation.  A token whose position has no page in
@@ -339,12 +339,12 @@ int plora_peft_pack(const char* path, const char* const* modules, int32_t num_mo
  * plora_paged_attention: out[b, h] = softmax(scale * q[b, h] . k) v over row
  * b's last min(window, seq_lens[b]) of seq_lens[b] cached tokens (window 0:
  * all of them); zeros where there are none.  out is dense (rows, heads,
- * head_dim).  A token on a page outside [0, num_pages) reads as zeros, and
+ * head_dim); it may be q, but not share a part of its memory.  A token on a page outside [0, num_pages) reads as zeros, and
  * seq_lens beyond the table's reach are clamped to it; the first raises
  * PLORA_DEV_PAGE_RANGE.  Sums in fp32; repeated calls agree bit for bit.  The
  * workspace (plora_paged_attention_workspace bytes, 256-byte aligned; 0 for few
- * short rows and for arguments the call rejects) needs no initialisation; calls that may overlap
- * need one each. */
+ * short rows and for arguments the call rejects) needs no initialisation;
+ * calls that may overlap need one each. */
 
 typedef struct plora_paged_cache {
   void* k_cache;
@@ -397,7 +397,7 @@ int plora_paged_attention(const plora_paged_attention_args* args, void* stream);
  * Each row's own rules on its logits (no counterpart in the reference).
  *
  * logits, out: (rows, vocab) of dtype, *_stride elements between rows; out may
- * be logits.  In fp32, rounded once, in this order:
+ * be logits, but not share a part of its memory.  In fp32, rounded once, in this order:
  *   x > 0 ? x / repetition[b] : x * repetition[b]  for tokens of row b's history,
  *       tokens[b, i], i < token_lens[b] (null: history each);
  *   x - frequency[b] * count - presence[b]         for tokens found count > 0 times
@@ -410,8 +410,7 @@ int plora_paged_attention(const plora_paged_attention_args* args, void* stream);
  * most 65535 rows and 4096 biases a row.  The workspace
  * (plora_logit_rules_workspace bytes, 256-byte aligned; 0 for few rows and for
  * arguments the call rejects; not used in place without a mask) needs no
- * initialisation; calls that may overlap
- * need one each. */
+ * initialisation; calls that may overlap need one each. */
 size_t plora_logit_rules_workspace(int64_t rows, int64_t vocab, int64_t history, int64_t biases);
 
 typedef struct plora_logit_rules_args {

@@ -662,6 +662,21 @@ int token_rows_impl(const void* host_rows, void* device_rows, bool to_host, int6
 }
 
 // ---------------------------------------------------------------- paged cache
+// Whether two byte ranges share memory.
+bool ranges_meet(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
+  const __int128 x = (__int128)reinterpret_cast<uintptr_t>(a), y = (__int128)reinterpret_cast<uintptr_t>(b);
+  return a_bytes > 0 && b_bytes > 0 && x < y + b_bytes && y < x + a_bytes;
+}
+// Whether rows of `width` elements at two addresses share memory without being
+// the same rows.  Rows of one stride may interleave.
+bool rows_meet(const void* a, int64_t a_stride, const void* b, int64_t b_stride, int64_t rows, int64_t width, int64_t el) {
+  if (a == b && (a_stride == b_stride || rows == 1)) return false;
+  if (!ranges_meet(a, ((rows - 1) * a_stride + width) * el, b, ((rows - 1) * b_stride + width) * el)) return false;
+  if (a_stride != b_stride || rows == 1) return true;
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  const int64_t off = (int64_t)((x < y ? y - x : x - y) % (uint64_t)(a_stride * el));
+  return off < width * el || off > (a_stride - width) * el;
+}
 // SMs of a B200: the attention grid, so that its workspace does not depend on the device.
 constexpr int kAttnGrid = 148;
 constexpr int64_t kPagedMaxRows = 1 << 20;
@@ -1263,6 +1278,15 @@ int plora_paged_attention(const plora_paged_attention_args* args, void* stream) 
     return fail(PLORA_ERR_WORKSPACE, "attention workspace %lld < %zu bytes", (long long)args->workspace_size, a.bytes);
   if (reinterpret_cast<uintptr_t>(args->workspace) % 256)
     return fail(PLORA_ERR_INVALID_ARGUMENT, "workspace must be 256-byte aligned");
+  if (args->q_row_stride > INT64_MAX / 16 / rows || args->q_head_stride > INT64_MAX / 16 / heads)
+    return fail(PLORA_ERR_INVALID_ARGUMENT, "size of q overflows");
+  const int64_t el = (int64_t)elem_size(dtype);
+  // in place each query is read before its output is written, and by no other item
+  const bool in_place = q == args->out && (heads == 1 || args->q_head_stride == head_dim) &&
+                        (rows == 1 || args->q_row_stride == (int64_t)heads * head_dim);
+  if (!in_place && ranges_meet(q, ((rows - 1) * args->q_row_stride + (heads - 1) * args->q_head_stride + head_dim) * el,
+                               args->out, rows * heads * head_dim * el))
+    return fail(PLORA_ERR_INVALID_ARGUMENT, "out shares memory with q and is not q");
   DeviceInfo* di = nullptr;
   if ((st = device_info(&di))) return st;
   p.q = q, p.out = args->out, p.seq_lens = args->seq_lens;
@@ -1327,6 +1351,10 @@ int plora_logit_rules(const plora_logit_rules_args* args, void* stream) {
   const uintptr_t el = elem_size(dtype) - 1;
   if ((reinterpret_cast<uintptr_t>(logits) & el) || (reinterpret_cast<uintptr_t>(out) & el))
     return fail(PLORA_ERR_INVALID_ARGUMENT, "logits or out not aligned to its type");
+  if (logits_stride > INT64_MAX / 16 / rows || out_stride > INT64_MAX / 16 / rows)
+    return fail(PLORA_ERR_INVALID_ARGUMENT, "size of logits or out overflows");
+  if (rows_meet(logits, logits_stride, out, out_stride, rows, vocab, (int64_t)elem_size(dtype)))
+    return fail(PLORA_ERR_INVALID_ARGUMENT, "out shares memory with logits and is not logits");
   DeviceInfo* di = nullptr;
   int st = device_info(&di);
   if (st) return st;

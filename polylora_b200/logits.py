@@ -77,7 +77,7 @@ def _vector(t: torch.Tensor, dev: int, rows: int, dtype: torch.dtype, name: str)
 
 def apply_logit_rules(logits: torch.Tensor, rules: LogitRules, out: torch.Tensor | None = None) -> torch.Tensor:
     """``rules`` on logits (B, V), computed in fp32 and rounded once to the
-    logits' dtype; into ``out`` (which may be ``logits``) or a new tensor."""
+    logits' dtype; into ``out`` (``logits``, or memory of its own) or a new tensor."""
     dev = logits.get_device()
     if dev < 0:
         _same_device(dev, logits)

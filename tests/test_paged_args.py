@@ -111,6 +111,33 @@ def test_rules_arguments_rejected_before_cuda(native):
         assert lib.plora_logit_rules_workspace(*bad) == 0
 
 
+def test_outputs_that_share_a_part_of_their_input_are_refused(native):
+    """The ranges are worked out on the host; a call that is taken fails here
+    for want of a GPU, with another status."""
+    lib = native.load()
+
+    def rules(rows, vocab, x, xs, y, ys):
+        return lib.plora_logit_rules(native.LOGIT_RULES_ARGS.pack(
+            x, xs, y, ys, rows, vocab, native.DTYPE_BF16, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, D, 4, 8, 0, 0), None)
+
+    for bad in ((2, 100, D, 100, D + 2, 100), (2, 100, D + 198, 100, D, 100), (2, 100, D, 100, D, 104),
+                (2, 100, D, 250, D + 2 * 151, 250), (3, 100, D, 250, D + 2 * (250 + 99), 250), (1, 100, D, 100, D + 16, 100)):
+        assert rules(*bad) == native.ERR_INVALID_ARGUMENT, bad
+        assert "shares" in native.last_error()
+    for bad in ((2, 100, D, 1 << 62, 2 * D, 100), (2, 100, D, 100, 2 * D, 1 << 62)):
+        assert rules(*bad) == native.ERR_INVALID_ARGUMENT, bad
+    for kw in (dict(out=D + 16), dict(q=D + 2 * 2 * 16 * 64 - 16), dict(qs=(2048, 64)), dict(qs=(1024, 128)),
+               dict(qs=(0, 64)), dict(qs=(1 << 61, 64), out=2 * D)):
+        assert _attend(lib, native, **kw) == native.ERR_INVALID_ARGUMENT, kw
+    if torch.cuda.is_available():
+        return
+    for good in ((2, 100, D, 100, D, 100), (2, 100, D, 100, D + 400, 100), (1, 100, D, 100, D + 200, 100),
+                 (2, 100, D, 250, D + 2 * 150, 250), (3, 100, D, 250, D + 2 * (250 + 100), 250)):
+        assert rules(*good) not in (native.OK, native.ERR_INVALID_ARGUMENT), good
+    for kw in (dict(), dict(out=D + 2 * 2 * 16 * 64), dict(rows=1, qs=(0, 64))):
+        assert _attend(lib, native, **kw) not in (native.OK, native.ERR_INVALID_ARGUMENT), kw
+
+
 def test_cpu_tensors_are_refused():
     kc, table, lens = torch.zeros(1, 1, 4, 8), torch.zeros(1, 1, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
     with pytest.raises(RuntimeError, match="no CPU fallback"):
