@@ -18,7 +18,7 @@
 // own rules.  More rows: the finding first, which leaves lists, and
 // logit_apply_kernel after both.  256 x 128256 bf16 logits, 4096 tokens, 64 biases
 // and a mask: 32 us, of which the copy 25 (5.3 TB/s); 47 us in one kernel whose CTAs
-// do all three.  One row: 5.5 us, the chain of loads and barriers of the finding.
+// do all three.  One row: 4.8 us, the chain of loads and barriers of the finding.
 //
 // The rules are found in two readings of the row's history.  The first sets a bit
 // for each of its tokens; the bits, counted, give each token's place in the list of
@@ -35,6 +35,9 @@ constexpr int kRulesThreads = 256;
 constexpr int kRulesStrip = 128;        // 16-byte chunks that a copying warp takes at a time
 constexpr int kRulesBesideCtas = 148;  // finding CTAs that run beside the copy
 constexpr int kRulesMostPart = 1 << 18; // vocabulary entries of a CTA that finds rules
+// Few rows are cut into parts of no less: a CTA's tables are zeroed and counted in one
+// go.  Uncut and cut: 1 x 128256 bf16 5.6 and 4.8 us, 33 x 50257 fp32 8.3 and 7.2.
+constexpr int kRulesLeastPart = 1 << 14;
 constexpr int kRulesMostSmem = 100 * 1024;
 constexpr int kRulesMaxBiases = 4096;   // entries of a row's bias list
 constexpr int kRulesHeld = 8;           // history entries that a thread reads at once, and of the first keeps
@@ -300,16 +303,26 @@ __global__ void __launch_bounds__(kRulesThreads) logit_find_kernel(const RulesPa
       if (first != j) twice[first] = 1;
     }
     __syncthreads();
+    // A warp adds up a token's biases, looking at 32 entries at a time; one by one, a
+    // token named twice among 300 took 8 us.
+    const int lane = tid & 31;
+    for (int j0 = tid - lane; j0 < p.biases; j0 += kRulesThreads) {
+      uint32_t todo = __ballot_sync(0xffffffffu, j0 + lane < p.biases && twice[j0 + lane]);
+      for (; todo; todo &= todo - 1) {
+        const int j = j0 + __ffs(todo) - 1, token = bias_at[j];
+        float sum = bias_v[j];
+#pragma unroll 4
+        for (int o0 = j0; o0 < p.biases; o0 += 32) {
+          const int o = o0 + lane;
+          uint32_t same = __ballot_sync(0xffffffffu, o > j && o < p.biases && bias_at[o] == token);
+          for (; same; same &= same - 1) sum += bias_v[o0 + __ffs(same) - 1];
+        }
+        if (lane == 0) bias_v[j] = sum;  // read by this warp alone until the barrier
+      }
+    }
+    __syncthreads();
   }
-  auto bias = [&](int r) {
-    const uint32_t j = bias_of[r];
-    if (j == kRulesNone) return 0.f;
-    float sum = bias_v[j];
-    if (twice[j])
-      for (int o = j + 1; o < p.biases; ++o)
-        if (bias_at[o] == token_of[r]) sum += bias_v[o];
-    return sum;
-  };
+  auto bias = [&](int r) { return bias_of[r] == kRulesNone ? 0.f : bias_v[bias_of[r]]; };
 
   if (p.list) {
     const int64_t at = row * gridDim.x + blockIdx.x;

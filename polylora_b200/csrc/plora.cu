@@ -855,8 +855,11 @@ RulesPlan rules_plan(int64_t rows, int64_t vocab, int64_t history, int64_t biase
   const int64_t entries = history + biases;
   a.copy = copy;
   a.find = entries > 0;
-  // the largest part whose tables leave room for a second CTA
-  a.part = (int)std::min<int64_t>(std::max<int64_t>(vocab, 1), kRulesMostPart);
+  // as small a part as keeps all CTAs beside the copy (rows of kRulesLeastPart or less
+  // are not cut), and one whose tables leave room for a second CTA
+  const int64_t cuts = std::max<int64_t>(kRulesBesideCtas / std::max<int64_t>(rows, 1), 1);
+  const int64_t share = std::max<int64_t>(((vocab + cuts - 1) / cuts + 31) & ~31ll, kRulesLeastPart);
+  a.part = (int)std::min({std::max<int64_t>(vocab, 1), share, (int64_t)kRulesMostPart});
   while (a.part > 1024 && rules_smem_bytes(a.part, entries, 0) > kRulesMostSmem) a.part = (a.part / 2 + 31) & ~31;
   a.parts = (int)((vocab + a.part - 1) / a.part);
   a.smem = (size_t)rules_smem_bytes(a.part, entries, (int)biases);
