@@ -15,10 +15,11 @@
 // leaves the memory idle; and the rules are applied to those tokens once the copy
 // is done.  The first two run side by side.  Rows few enough for all of their
 // finding CTAs to wait out the copy: the copy first, and a finding CTA applies its
-// own rules.  More rows: the finding first, which leaves lists, and
-// logit_apply_kernel after both.  256 x 128256 bf16 logits, 4096 tokens, 64 biases
-// and a mask: 32 us, of which the copy 25 (5.3 TB/s); 47 us in one kernel whose CTAs
-// do all three.  One row: 4.8 us, the chain of loads and barriers of the finding.
+// own rules; few rows, cut into small parts: it copies its part too, in one launch.
+// More rows: the finding first, which leaves lists, and logit_apply_kernel after
+// both.  256 x 128256 bf16 logits, 4096 tokens, 64 biases and a mask: 32 us, of which
+// the copy 25 (5.3 TB/s); 47 us in one kernel whose CTAs do all three.  One row: 5.6
+// us, the chain of loads and barriers of the finding.
 //
 // The rules are found in two readings of the row's history.  The first sets a bit
 // for each of its tokens; the bits, counted, give each token's place in the list of
@@ -36,7 +37,8 @@ constexpr int kRulesStrip = 128;        // 16-byte chunks that a copying warp ta
 constexpr int kRulesBesideCtas = 148;  // finding CTAs that run beside the copy
 constexpr int kRulesMostPart = 1 << 18; // vocabulary entries of a CTA that finds rules
 // Few rows are cut into parts of no less: a CTA's tables are zeroed and counted in one
-// go.  Uncut and cut: 1 x 128256 bf16 5.6 and 4.8 us, 33 x 50257 fp32 8.3 and 7.2.
+// go.  Uncut and cut, copied beside: 1 x 128256 bf16 5.6 and 4.8 us, 33 x 50257 fp32 8.3
+// and 7.2.
 constexpr int kRulesLeastPart = 1 << 14;
 constexpr int kRulesMostSmem = 100 * 1024;
 constexpr int kRulesMaxBiases = 4096;   // entries of a row's bias list
@@ -71,6 +73,7 @@ struct RulesParams {
   int32_t history, biases;
   int32_t part;        // vocabulary entries of a CTA that finds rules
   bool beside;         // the finding is launched after the copy, and beside it
+  bool copies;         // a finding CTA copies its part itself
   // lists (null: a finding CTA applies its rules): entries of each (row, part) and how many
   struct RulesEntry* list;
   int32_t* listed;
@@ -122,60 +125,62 @@ struct RulesRow {
   }
 };
 
-// y = x with -infinity where the mask does not allow.  A warp takes a strip of a
-// row, from the row's first 16-byte boundary on, and a lane 16-byte chunks lane,
-// lane + 32, ... of it, all four of them on their way.
+// y = x with -infinity where the mask does not allow, for strip `strip` of `count`
+// elements of a row (from an element that a word of the mask begins with).  A warp
+// takes a strip, counted from the first 16-byte boundary on, and a lane 16-byte
+// chunks lane, lane + 32, ... of it, all four of them on their way.
+template <typename T>
+__device__ __forceinline__ void rules_copy(const T* x, T* y, const uint32_t* mask, int count, int strip, int lane) {
+  constexpr int N = Chunk<T>::N, ROUNDS = kRulesStrip / 32;
+  const int off = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
+  const int head = min(count, off ? N - off : 0), first = head + strip * kRulesStrip * N;
+  if (first >= count && strip != 0) return;
+  auto one = [&](int i) { y[i] = mask && !(mask_bits(mask, i, 1) & 1) ? Chunk<T>::put(-INFINITY) : x[i]; };
+  if ((reinterpret_cast<uintptr_t>(x) & 15) == (reinterpret_cast<uintptr_t>(y) & 15)) {
+    const int chunks = (count - first) / N;  // from here on
+    const uint4* from = reinterpret_cast<const uint4*>(x + first);
+    uint4* to = reinterpret_cast<uint4*>(y + first);
+    uint4 u[ROUNDS];
+#pragma unroll
+    for (int v = 0; v < ROUNDS; ++v)
+      if (lane + v * 32 < chunks) u[v] = from[lane + v * 32];
+    if (mask) {
+      const int i0 = first + lane * N, shift = i0 & 31;  // of the chunk's mask bits in their word, in every round
+      const uint32_t* m = mask + (i0 >> 5);
+      uint32_t w[ROUNDS];
+#pragma unroll
+      for (int v = 0; v < ROUNDS; ++v) w[v] = lane + v * 32 < chunks ? m[v * N] : 0u;
+#pragma unroll
+      for (int v = 0; v < ROUNDS; ++v) {
+        uint32_t keep = w[v] >> shift;
+        if (shift + N > 32 && lane + v * 32 < chunks) keep |= m[v * N + 1] << (32 - shift);  // the rest is in the next word
+        u[v] = rules_masked<T>(u[v], keep);
+      }
+    }
+#pragma unroll
+    for (int v = 0; v < ROUNDS; ++v)
+      if (lane + v * 32 < chunks) to[lane + v * 32] = u[v];
+    // single elements before the first chunk and after the last
+    if (strip == 0 && lane < head) one(lane);
+    const int tail = first + chunks * N;
+    if (chunks <= kRulesStrip && tail + lane < count) one(tail + lane);
+  } else {
+    const int last = min(first + kRulesStrip * N, count);
+#pragma unroll 8
+    for (int i = (strip == 0 ? 0 : first) + lane; i < last; i += 32) one(i);
+  }
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kRulesThreads) logit_copy_kernel(const RulesParams p) {
-  constexpr int N = Chunk<T>::N, ROUNDS = kRulesStrip / 32;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, vocab = (int)p.vocab;
   const int64_t row = blockIdx.y;
-  const int strip = blockIdx.x * (kRulesThreads / 32) + warp;
   // After the finding kernel nothing need be waited for at first: it lets this one
   // start when all of its CTAs have waited for what came before.
   if (p.beside) griddep_wait();
   griddep_launch();
-  const T* x = (const T*)p.x + row * p.x_row;
-  T* y = (T*)p.y + row * p.y_row;
-  const uint32_t* mask = p.allowed ? p.allowed + row * p.mask_row : nullptr;
-  const int off = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
-  const int head = min(vocab, off ? N - off : 0), first = head + strip * kRulesStrip * N;
-  auto one = [&](int i) { y[i] = mask && !(mask_bits(mask, i, 1) & 1) ? Chunk<T>::put(-INFINITY) : x[i]; };
-  if (first < vocab || strip == 0) {
-    if ((reinterpret_cast<uintptr_t>(x) & 15) == (reinterpret_cast<uintptr_t>(y) & 15)) {
-      const int chunks = (vocab - first) / N;  // of the row from here on
-      const uint4* from = reinterpret_cast<const uint4*>(x + first);
-      uint4* to = reinterpret_cast<uint4*>(y + first);
-      uint4 u[ROUNDS];
-#pragma unroll
-      for (int v = 0; v < ROUNDS; ++v)
-        if (lane + v * 32 < chunks) u[v] = from[lane + v * 32];
-      if (mask) {
-        const int i0 = first + lane * N, shift = i0 & 31;  // of the chunk's mask bits in their word, in every round
-        const uint32_t* m = mask + (i0 >> 5);
-        uint32_t w[ROUNDS];
-#pragma unroll
-        for (int v = 0; v < ROUNDS; ++v) w[v] = lane + v * 32 < chunks ? m[v * N] : 0u;
-#pragma unroll
-        for (int v = 0; v < ROUNDS; ++v) {
-          uint32_t keep = w[v] >> shift;
-          if (shift + N > 32 && lane + v * 32 < chunks) keep |= m[v * N + 1] << (32 - shift);  // the rest is in the next word
-          u[v] = rules_masked<T>(u[v], keep);
-        }
-      }
-#pragma unroll
-      for (int v = 0; v < ROUNDS; ++v)
-        if (lane + v * 32 < chunks) to[lane + v * 32] = u[v];
-      // single elements before the first chunk and after the last
-      if (strip == 0 && lane < head) one(lane);
-      const int tail = first + chunks * N;
-      if (chunks <= kRulesStrip && tail + lane < vocab) one(tail + lane);
-    } else {
-      const int last = min(first + kRulesStrip * N, vocab);
-#pragma unroll 8
-      for (int i = (strip == 0 ? 0 : first) + lane; i < last; i += 32) one(i);
-    }
-  }
+  rules_copy<T>((const T*)p.x + row * p.x_row, (T*)p.y + row * p.y_row,
+                p.allowed ? p.allowed + row * p.mask_row : nullptr, (int)p.vocab,
+                blockIdx.x * (kRulesThreads / 32) + (threadIdx.x >> 5), threadIdx.x & 31);
   // this grid's end has to mean the finding kernel's end too, for the kernel that applies its lists
   if (!p.beside && blockIdx.x + 1 == gridDim.x && blockIdx.y + 1 == gridDim.y) griddep_wait();
 }
@@ -238,6 +243,11 @@ __global__ void __launch_bounds__(kRulesThreads) logit_find_kernel(const RulesPa
 #pragma unroll
   for (int k = 0; k < kRulesHeld; ++k) held[k] = -1;
   if (len > 0) read(tid, held);
+  if (p.copies) {  // the barriers up to the applying order it and the copy
+    const uint32_t* mask = p.allowed ? p.allowed + row * p.mask_row + c0 / 32 : nullptr;
+    for (int strip = tid / 32; strip * kRulesStrip * Chunk<T>::N < nc; strip += kRulesThreads / 32)
+      rules_copy<T>((const T*)p.x + row * p.x_row + c0, (T*)p.y + row * p.y_row + c0, mask, nc, strip, tid & 31);
+  }
   __syncthreads();  // the bits are zero
 #pragma unroll
   for (int k = 0; k < kRulesHeld; ++k) touch(held[k]);

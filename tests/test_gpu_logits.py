@@ -108,6 +108,10 @@ CASES = [
     (151, 900, None, 70, True, F32, True),
     (3, 300000, 9000, 20, True, BF, True),    # more than one part of the vocabulary
     (80, 300000, 40, 5, False, BF, True),
+    (33, 50257, 200, 64, True, FH, True),     # small parts: one launch copies and applies
+    (60, 40001, 70, 300, True, BF, True),     # larger ones: two kernels side by side
+    (140, 17000, 30, 600, False, F32, False),
+    (2, 40, 10, 900, True, F32, True),        # each token's biases many times
 ]
 
 
