@@ -8,6 +8,7 @@ The reference has no counterpart (it ends at the base model's output).
 
 from __future__ import annotations
 
+import functools
 from dataclasses import dataclass
 
 import torch
@@ -73,6 +74,11 @@ def _vector(t: torch.Tensor, dev: int, rows: int, dtype: torch.dtype, name: str)
     if t.dim() != 1 or t.shape[0] != rows:
         raise ValueError(f"{name} must have shape ({rows},), got {tuple(t.shape)}")
     return t if t.dtype is dtype and t.is_contiguous() else t.to(dtype).contiguous()
+
+
+@functools.lru_cache(maxsize=1024)  # sizes alone decide it
+def _workspace(rows: int, vocab: int, history: int, biases: int) -> int:
+    return _native.load().plora_logit_rules_workspace(rows, vocab, history, biases)
 
 
 def apply_logit_rules(logits: torch.Tensor, rules: LogitRules, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -148,7 +154,7 @@ def apply_logit_rules(logits: torch.Tensor, rules: LogitRules, out: torch.Tensor
         allowed = _matrix(allowed, dev, rows, "allowed")
         mask_row = allowed.stride(0)
     lib = _native.load()
-    ws_bytes = lib.plora_logit_rules_workspace(rows, vocab, history, biases)
+    ws_bytes = _workspace(rows, vocab, history, biases)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=logits.device) if ws_bytes else None
     args = _native.LOGIT_RULES_ARGS.pack(
         logits.data_ptr(), row if rows > 1 else vocab, out.data_ptr(), out.stride(0) if rows > 1 else vocab, rows, vocab,

@@ -14,6 +14,7 @@ models that bring their own caches.
 
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -61,14 +62,10 @@ def _strides(t: torch.Tensor) -> tuple[int, ...]:
 def _heads(t: torch.Tensor) -> tuple[torch.Tensor, tuple[int, ...], int]:
     """``t`` with dense last dimension and 16-byte aligned rows (a copy where
     it has neither), its strides and its address."""
-    vec = 16 // t.element_size()
-    ptr, st = t.data_ptr(), t.stride()
-    low = ptr // t.element_size()
-    for x in st[:-1]:
-        low |= x
-    if st[-1] == 1 and low % vec == 0:  # the rule, with any dimensions of one
+    ptr, st, size = t.data_ptr(), t.stride(), t.element_size()
+    if st[-1] == 1 and not ((st[0] | st[1] | st[-2]) * size | ptr) & 15:  # the rule, with any dimensions of one
         return t, st, ptr
-    st = _strides(t)
+    st, vec = _strides(t), 16 // size
     if (t.shape[-1] > 1 and st[-1] != 1) or any([s % vec for s in st[:-1]]) or ptr % 16:
         t = t.clone(memory_format=torch.contiguous_format)
         st, ptr = _strides(t), t.data_ptr()
@@ -108,6 +105,13 @@ def _lens(t: torch.Tensor, rows: int, name: str) -> torch.Tensor:
     if t.dim() != 1 or t.shape[0] != rows:
         raise ValueError(f"{name} must have shape ({rows},), got {tuple(t.shape)}")
     return _as(t, torch.int32)
+
+
+# Sizes alone decide it; asking the library takes a microsecond of a call whose kernel takes seven.
+@functools.lru_cache(maxsize=1024)
+def _attention_workspace(rows: int, heads: int, kv_heads: int, dim: int, size: int, max_pages: int, window: int,
+                         dtype: int) -> int:
+    return _native.load().plora_paged_attention_workspace(rows, heads, kv_heads, dim, size, max_pages, window, dtype)
 
 
 # The current stream's raw handle: a Stream object costs 2 us of a call whose kernel takes less than 3.
@@ -243,7 +247,7 @@ def paged_attention(
         raise ValueError("out must be a contiguous tensor of q's shape, dtype and device")
     q, qs, q_ptr = _heads(q)
     code, lib = dtype_code(dtype), _native.load()
-    ws_bytes = lib.plora_paged_attention_workspace(rows, heads, kv_heads, dim, size, max_pages, window, code)
+    ws_bytes = _attention_workspace(rows, heads, kv_heads, dim, size, max_pages, window, code)
     ws = lens.new_empty(ws_bytes // 4) if ws_bytes else None
     args = _native.PAGED_ATTENTION_ARGS.pack(
         k_cache.data_ptr(), v_cache.data_ptr(), k_page, v_page, page_table.data_ptr(), table_row, rows, heads, kv_heads,
