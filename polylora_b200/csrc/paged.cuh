@@ -1019,7 +1019,11 @@ struct AttnMmaCfg {
 // Probabilities enter the second product as a 16-bit number and a 16-bit
 // remainder: with the first alone the sums would be off by as much as the
 // rounding of the result (1.7e-3 becomes 2.3e-3 of a bf16 output); the second
-// costs one more instruction where memory is the bound.
+// costs one more instruction where memory is the bound.  In fp16 the largest
+// probability stands as 2^15, here and in the sum that divides: next to 1 what lies
+// below 2^-25 would be lost, and from the values alone (131071 tokens of 2^-26 are 0.2 %
+// of the sum); so it is what lies below 2^-40.  An infinite value of a token that is attended to
+// gives infinity or NaN.
 //
 // 256 rows of up to 4096 tokens, 32/8 heads of 128, bf16, 2.03 GB: 310 us with plan
 // and join (6.5 TB/s), where the same kernel with a copy instruction a lane took 419;
@@ -1032,6 +1036,7 @@ __global__ void __launch_bounds__(AttnMmaCfg<DP, NT>::kWarps * 32, 1)
   using Tile = AttnTileCfg<2, DP>;
   using T = typename Elem<BF16>::T;
   constexpr int KS = DP / 16, STAGES = Cfg::kStages;
+  constexpr float kUnit = BF16 ? 1.f : 0x1p15f;  // what a probability of 1 stands as
   extern __shared__ __align__(128) unsigned char attn_smem[];
   __shared__ uint64_t bars[TMA ? Cfg::kWarps * STAGES : 1];
   __shared__ int abort_flag;
@@ -1219,8 +1224,8 @@ __global__ void __launch_bounds__(AttnMmaCfg<DP, NT>::kWarps * 32, 1)
         const float m2 = fmaxf(m[nt][j], mx), top = m2 == -INFINITY ? 0.f : m2;
         keep[j] = exp2_fast(m[nt][j] - top);
         m[nt][j] = m2;
-        x[j] = exp2_fast(x[j] - top);
-        x[j + 2] = exp2_fast(x[j + 2] - top);
+        x[j] = exp2_fast(x[j] - top) * kUnit;
+        x[j + 2] = exp2_fast(x[j + 2] - top) * kUnit;
         l[nt][j] = l[nt][j] * keep[j] + x[j] + x[j + 2];  // of this lane's tokens; added over lanes at the end
       }
       if (__any_sync(0xffffffffu, keep[0] != 1.f || keep[1] != 1.f)) {
