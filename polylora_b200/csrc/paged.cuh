@@ -539,8 +539,8 @@ struct AttnWalk {
     return true;
   }
   // Called before each copy of a loader with `left` tiles to start: asks for the
-  // next segment a few tiles ahead (every one but the last is longer), and with
-  // nothing left moves the loader to it.
+  // next segment a few tiles ahead (every one but the last is longer, and nothing is
+  // asked for in that one), and with nothing left moves the loader to it.
   __device__ __forceinline__ bool look_ahead(const AttnParams& p, int left) {
     if (!more) return false;
     if (left == kAttnAsk) ask(p);
@@ -550,8 +550,6 @@ struct AttnWalk {
     if (id >= ids) return false;
     nxt = list.segment(p, id);
     have_nxt = true;
-    // a segment of kAttnAsk tiles or fewer never has that many left after its first
-    if (more && nxt.count <= kAttnAsk) ask(p);
     return true;
   }
   __device__ __forceinline__ void ask(const AttnParams& p) {
