@@ -25,6 +25,7 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
+from .kv_check import check_attention
 from .paged import paged_append, paged_attention, rotary_phases
 
 
@@ -269,7 +270,7 @@ def _rotation(model: nn.Module) -> tuple[torch.Tensor, float]:
 
 
 def attach(model: nn.Module, cache: PagedKVCache, inv_freq: torch.Tensor | None = None,
-           rotary_scale: float | None = None, interleaved: bool = False) -> None:
+           rotary_scale: float | None = None, interleaved: bool = False, check: bool = True) -> None:
     """Gives the model's attention modules their paged forward (see
     ``PolyLoraModel.attach_kv_cache``)."""
     modules = attention_modules(model)
@@ -281,15 +282,22 @@ def attach(model: nn.Module, cache: PagedKVCache, inv_freq: torch.Tensor | None 
         if int(m.head_dim) != head_dim or m.k_proj.out_features != kv_heads * head_dim:
             raise ValueError(f"an attention module has {m.k_proj.out_features} key features in heads of {m.head_dim}, "
                              f"the cache {kv_heads} heads of {head_dim}")
-    if inv_freq is None:
+    given = inv_freq is not None
+    if not given:
         inv_freq, scale = _rotation(model)
     else:
         scale = 1.0
+    if rotary_scale is None:
+        rotary_scale = scale
     phases = rotary_phases(inv_freq)
+    forwards = []
     for layer, m in enumerate(modules):
         original = m.forward.original if isinstance(m.forward, _PagedAttentionForward) else m.forward
-        m.forward = _PagedAttentionForward(m, original, cache, layer, phases, interleaved,
-                                           scale if rotary_scale is None else rotary_scale)
+        forwards.append(_PagedAttentionForward(m, original, cache, layer, phases, interleaved, rotary_scale))
+    if check:
+        check_attention(model, modules, forwards, inv_freq, rotary_scale, given, cache.num_pages * cache.page_size)
+    for m, f in zip(modules, forwards):
+        m.forward = f
 
 
 __all__ = ["PagedBatch", "PagedKVCache", "get_paged_batch", "use_paged_batch"]

@@ -133,14 +133,18 @@ class PolyLoraModel(nn.Module):
                                                   peft_adapter_name=peft_adapter_name)
 
     def attach_kv_cache(self, cache: PagedKVCache, inv_freq: torch.Tensor | None = None,
-                        rotary_scale: float | None = None, interleaved: bool = False) -> None:
+                        rotary_scale: float | None = None, interleaved: bool = False, check: bool = True) -> None:
         """Lets ``forward(..., paged=batch)`` run the base model's attention on
         ``cache``.  For decoders whose attention modules hold q_proj, k_proj,
         v_proj and o_proj and rotate queries and keys (in halves, or as
         neighbouring pairs with ``interleaved``) by ``inv_freq``, by default the
-        model's own rotary embedding's.  Forwards without a batch are unchanged.
-        No counterpart in the reference."""
-        attach(self.base_model, cache, inv_freq, rotary_scale, interleaved)
+        model's own rotary embedding's.  Raises ValueError, with nothing attached,
+        where the paged forward would answer differently: the attention modules
+        are compared with it in forwards of a few random tokens, near and at the
+        farthest position that the cache holds.  ``check=False`` goes without, for
+        a model that such a forward cannot run.  Forwards without a batch are
+        unchanged.  No counterpart in the reference."""
+        attach(self.base_model, cache, inv_freq, rotary_scale, interleaved, check)
 
     def forward(self, *args: Any, adapter_ids: list[str] | None = None, paged: PagedBatch | None = None,
                 logit_rules: LogitRules | None = None, **kwargs: Any) -> Any:
