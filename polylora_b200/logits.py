@@ -47,14 +47,29 @@ class LogitRules:
     def clone(self) -> "LogitRules":
         return LogitRules(**{k: v.clone() if v is not None else None for k, v in vars(self).items()})
 
-    def copy_(self, other: "LogitRules") -> None:
-        """Takes another's values into this one's memory (for a captured call)."""
+    def check_copy(self, other: "LogitRules") -> None:
+        """Raises ValueError where ``copy_`` would not take ``other``'s values as they are."""
         for name, mine in vars(self).items():
             theirs = getattr(other, name)
             if (mine is None) != (theirs is None) or (mine is not None and mine.shape != theirs.shape):
                 raise ValueError(f"{name}: a captured call takes rules of the same kinds and shapes")
+            # what the operator would convert too may be; a token id or a mask may not lose bits
+            if mine is not None and mine.dtype is not _TYPES.get(name) \
+                    and torch.promote_types(mine.dtype, theirs.dtype) is not mine.dtype:
+                raise ValueError(f"{name}: captured as {mine.dtype}, which does not hold every {theirs.dtype}")
+
+    def copy_(self, other: "LogitRules") -> None:
+        """Takes another's values into this one's memory (for a captured call);
+        where one of them is refused, none is taken."""
+        self.check_copy(other)
+        for name, mine in vars(self).items():
             if mine is not None:
-                mine.copy_(theirs, non_blocking=True)
+                mine.copy_(getattr(other, name), non_blocking=True)
+
+
+# What the operator converts lengths and values to.
+_TYPES = {"token_lens": torch.int32, "prompt_lens": torch.int32, "repetition_penalty": torch.float32,
+          "presence_penalty": torch.float32, "frequency_penalty": torch.float32, "bias_values": torch.float32}
 
 
 def _matrix(t: torch.Tensor, dev: int, rows: int, name: str) -> torch.Tensor:

@@ -1,0 +1,41 @@
+"""What the captured copies of rules and batches take, and leave alone.  No GPU."""
+
+import pytest
+import torch
+
+from polylora_b200.logits import LogitRules
+
+
+def _rules(ids=torch.int64, value=1, **kw):
+    r = LogitRules(tokens=torch.full((2, 3), value, dtype=ids), token_lens=torch.full((2,), value, dtype=torch.int32),
+                   repetition_penalty=torch.full((2,), float(value)), bias_tokens=torch.full((2, 4), value, dtype=ids),
+                   bias_values=torch.full((2, 4), float(value)), allowed=torch.full((2, 1), value, dtype=torch.int32))
+    for k, v in kw.items():
+        setattr(r, k, v)
+    return r
+
+
+def _same(a, b):
+    return all((x is None) == (y is None) and (x is None or torch.equal(x, y)) for x, y in zip(vars(a).values(), vars(b).values()))
+
+
+@pytest.mark.parametrize("other", [
+    _rules(value=2),                                                    # int64 ids into int32: 2^32 + 5 would be token 5
+    _rules(torch.int32, 2, bias_tokens=torch.full((2, 4), 2**32 + 5)),
+    _rules(torch.int32, 2, tokens=torch.full((2, 3), 2.0)),
+    _rules(torch.int32, 2, allowed=torch.full((2, 1), 2**40)),
+    _rules(torch.int32, 2, allowed=None),
+    _rules(torch.int32, 2, allowed=torch.full((2, 2), 2, dtype=torch.int32)),
+    _rules(torch.int32, 2, presence_penalty=torch.ones(2)),
+])
+def test_rules_that_are_refused_leave_the_captured_ones_alone(other):
+    mine = _rules(torch.int32)
+    with pytest.raises(ValueError):
+        mine.copy_(other)
+    assert _same(mine, _rules(torch.int32))
+
+
+def test_rules_of_other_types_that_are_taken():
+    mine = _rules(torch.int64)
+    mine.copy_(_rules(torch.int32, 2, token_lens=torch.full((2,), 2), bias_values=torch.full((2, 4), 2.0, dtype=torch.float64)))
+    assert _same(mine, _rules(torch.int64, 2))
