@@ -40,7 +40,7 @@ class PagedBatch:
     new_lens: torch.Tensor    # (B,) int32
     seq_lens: torch.Tensor    # (B,) int32: past + new
     max_new: int              # tokens of a row of the forward's inputs
-    fresh: bool               # no row has a past
+    fresh: bool               # no row has a past (one new token a row runs alike either way)
 
     @property
     def rows(self) -> int:
@@ -50,11 +50,15 @@ class PagedBatch:
         return PagedBatch(self.cache, self.page_table.clone(), self.past_lens.clone(), self.new_lens.clone(),
                           self.seq_lens.clone(), self.max_new, self.fresh)
 
+    def check_copy(self, other: "PagedBatch") -> None:
+        """Raises ValueError where a forward captured with this batch would not run on ``other`` as an eager one does."""
+        if other.cache is not self.cache or other.max_new != self.max_new \
+                or (self.max_new > 1 and other.fresh != self.fresh) or other.page_table.shape != self.page_table.shape:
+            raise ValueError("a captured forward takes batches of its cache, rows, page-table width and new tokens")
+
     def copy_(self, other: "PagedBatch") -> None:
         """Takes another batch's tensors into this one's memory (for a captured forward)."""
-        if other.cache is not self.cache or (other.max_new, other.fresh) != (self.max_new, self.fresh) \
-                or other.page_table.shape != self.page_table.shape:
-            raise ValueError("a captured forward takes batches of its cache, rows, page-table width and new tokens")
+        self.check_copy(other)
         for name in ("page_table", "past_lens", "new_lens", "seq_lens"):
             getattr(self, name).copy_(getattr(other, name), non_blocking=True)
 

@@ -3,6 +3,7 @@
 import pytest
 import torch
 
+from polylora_b200.kv_cache import PagedKVCache
 from polylora_b200.logits import LogitRules
 
 
@@ -39,3 +40,33 @@ def test_rules_of_other_types_that_are_taken():
     mine = _rules(torch.int64)
     mine.copy_(_rules(torch.int32, 2, token_lens=torch.full((2,), 2), bias_values=torch.full((2, 4), 2.0, dtype=torch.float64)))
     assert _same(mine, _rules(torch.int64, 2))
+
+
+def _cache():
+    return PagedKVCache(1, 10, 4, 1, 8, torch.float32, "cpu")
+
+
+def test_one_token_steps_take_first_tokens_and_later_ones():
+    """A step of one token a row computes the same whether rows have a past or not."""
+    c = _cache()
+    first = c.batch(["a", "b"], width=2).clone()
+    later = c.batch(["a", "b"], width=2)
+    assert first.fresh and not later.fresh
+    captured_first, captured_later = first.clone(), later.clone()
+    captured_first.copy_(later)
+    assert captured_first.past_lens.tolist() == [1, 1]
+    c.free("a"), c.free("b")
+    new = c.batch(["x", "y"], width=2)
+    assert new.fresh
+    captured_later.copy_(new)
+    assert captured_later.past_lens.tolist() == [0, 0] and captured_later.seq_lens.tolist() == [1, 1]
+
+
+def test_longer_rows_keep_apart():
+    """Rows of a prompt attend among themselves, later ones over the cache."""
+    c = _cache()
+    prompt = c.batch(["a"], 3, width=3).clone()
+    more = c.batch(["a"], 3, width=3)
+    for one, other in ((prompt, more), (more.clone(), prompt)):
+        with pytest.raises(ValueError):
+            one.copy_(other)
