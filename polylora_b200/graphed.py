@@ -164,13 +164,18 @@ class GraphedForward:
             raise ValueError("a forward captured with a paged batch takes one with every call, others take none")
         if logit_rules is not None and self.rules is None:
             raise ValueError("the forward was captured without logit_rules")
+        # a refused call leaves the batch and the rules of the one before
+        if paged is not None:
+            self.paged.check_copy(paged)
+        if logit_rules is not None:
+            self.rules.check_copy(logit_rules)
+        for k, v in inputs.items():
+            self.static[k].copy_(v, non_blocking=True)
+        ctx = self._host_part(adapter_ids)
         if paged is not None:
             self.paged.copy_(paged)
         if logit_rules is not None:
             self.rules.copy_(logit_rules)
-        for k, v in inputs.items():
-            self.static[k].copy_(v, non_blocking=True)
-        ctx = self._host_part(adapter_ids)
         stream = torch.cuda.current_stream(self.device)
         if ctx.ready_event is not None:
             stream.wait_event(ctx.ready_event)

@@ -3,6 +3,7 @@
 import pytest
 import torch
 
+from polylora_b200.graphed import GraphedForward
 from polylora_b200.kv_cache import PagedKVCache
 from polylora_b200.logits import LogitRules
 
@@ -70,3 +71,29 @@ def test_longer_rows_keep_apart():
     for one, other in ((prompt, more), (more.clone(), prompt)):
         with pytest.raises(ValueError):
             one.copy_(other)
+
+
+def _captured(paged, rules, refuse):
+    """A captured forward's host side, without its graph."""
+    step = GraphedForward.__new__(GraphedForward)
+    step.paged, step.rules, step.static = paged, rules, {}
+
+    def host_part(adapter_ids):
+        raise refuse
+
+    step._host_part = host_part
+    return step
+
+
+def test_refused_calls_leave_batch_and_rules_alone():
+    c = _cache()
+    batch, rules = c.batch(["a", "b"], width=2), _rules(torch.int32)
+    later = c.batch(["a", "b"], width=2)
+    for paged, new, match in (
+            (later, _rules(value=2), "bias_tokens|tokens"),                # rules refused, the batch is not taken
+            (c.batch(["a", "b"], width=3), _rules(torch.int32, 2), "width"),  # the batch refused, the rules are not
+            (later, _rules(torch.int32, 2), "no such adapter")):           # both well, but the adapters are not
+        step = _captured(batch.clone(), rules.clone(), ValueError("no such adapter"))
+        with pytest.raises(ValueError, match=match):
+            step(["x", "y"], paged=paged, logit_rules=new)
+        assert step.paged.past_lens.tolist() == [0, 0] and _same(step.rules, rules)
