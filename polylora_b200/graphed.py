@@ -110,6 +110,8 @@ class GraphedForward:
 
     def __init__(self, model: Any, adapter_ids: list[str], warmup: int = 2, output=None,
                  paged: PagedBatch | None = None, logit_rules: LogitRules | None = None, **inputs: torch.Tensor):
+        if paged is not None and "attention_mask" in inputs:
+            raise ValueError("a paged batch carries its rows' lengths: pass no attention_mask")
         self.model = model
         self.paged = paged.clone() if paged is not None else None
         self.rules = logit_rules.clone() if logit_rules is not None else None

@@ -153,6 +153,8 @@ class PolyLoraModel(nn.Module):
         them.  ``logit_rules``: applied in place to the output's logits, of one
         token per row.  Neither has a counterpart in the reference."""
         if paged is not None:
+            if len(args) > 1:  # a decoder's second argument is its mask
+                raise ValueError("inputs of a paged forward after the first go by name")
             if kwargs.get("attention_mask") is not None:
                 raise ValueError("a paged batch carries its rows' lengths: pass no attention_mask")
             kwargs.setdefault("use_cache", False)

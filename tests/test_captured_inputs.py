@@ -97,3 +97,18 @@ def test_refused_calls_leave_batch_and_rules_alone():
         with pytest.raises(ValueError, match=match):
             step(["x", "y"], paged=paged, logit_rules=new)
         assert step.paged.past_lens.tolist() == [0, 0] and _same(step.rules, rules)
+
+
+def test_masks_that_a_paged_forward_would_not_look_at():
+    from test_kv_cache import _llama, _wrapped
+    from test_kv_cache import _cache as cache_of_llama
+
+    model, c = _wrapped(_llama()), cache_of_llama()
+    model.attach_kv_cache(c)
+    batch, ids, mask = c.batch(["a", "b"], 3), torch.zeros(2, 3, dtype=torch.long), torch.ones(2, 3)
+    with pytest.raises(ValueError, match="attention_mask"):
+        GraphedForward(model, ["__base__"] * 2, paged=batch, input_ids=ids, attention_mask=mask)
+    with pytest.raises(ValueError, match="by name"):
+        model(ids, mask, paged=batch)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU fallback"):
+        model(ids, paged=batch)
