@@ -16,6 +16,7 @@ from __future__ import annotations
 
 import contextlib
 import dataclasses
+import inspect
 from typing import Any, Iterator
 
 import torch
@@ -151,12 +152,21 @@ class PolyLoraModel(nn.Module):
         """``paged`` (see ``attach_kv_cache``): the new tokens of each row, right
         padded to ``paged.max_new``, are appended to their sequences and attend to
         them.  ``logit_rules``: applied in place to the output's logits, of one
-        token per row.  Neither has a counterpart in the reference."""
+        token per row.  A forward of several tokens a row has such logits with
+        ``logits_to_keep=1``, of the last column, which is padding in all but the
+        longest rows: of right-padded prompts take each row's last logits and apply
+        the rules to those (``apply_logit_rules``).  Neither has a counterpart in the
+        reference."""
         if paged is not None:
             if len(args) > 1:  # a decoder's second argument is its mask
                 raise ValueError("inputs of a paged forward after the first go by name")
             if kwargs.get("attention_mask") is not None:
                 raise ValueError("a paged batch carries its rows' lengths: pass no attention_mask")
+            if logit_rules is not None and paged.max_new > 1 and isinstance(kwargs.get("logits_to_keep", 0), int) \
+                    and not kwargs.get("logits_to_keep", 0) \
+                    and "logits_to_keep" in inspect.signature(self.base_model.forward).parameters:
+                raise ValueError(f"logit_rules apply to the logits of one token per row, the output has {paged.max_new}: "
+                                 "apply them to each row's last logits")  # before anything is appended
             kwargs.setdefault("use_cache", False)
         with use_paged_batch(paged) if paged is not None else contextlib.nullcontext():
             if adapter_ids is None:

@@ -112,3 +112,26 @@ def test_masks_that_a_paged_forward_would_not_look_at():
         model(ids, mask, paged=batch)
     with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU fallback"):
         model(ids, paged=batch)
+
+
+def test_rules_for_several_tokens_are_refused_before_the_forward(monkeypatch):
+    from transformers import LlamaConfig, LlamaForCausalLM
+
+    from test_kv_cache import _wrapped
+    from test_kv_cache import _cache as cache_of_llama
+
+    base = LlamaForCausalLM(LlamaConfig(vocab_size=50, hidden_size=64, intermediate_size=64, num_hidden_layers=2,
+                                        num_attention_heads=4, num_key_value_heads=2, max_position_embeddings=64)).eval()
+    model, c = _wrapped(base), cache_of_llama()
+    model.attach_kv_cache(c)
+    appended = []
+    monkeypatch.setattr("polylora_b200.kv_cache.paged_append", lambda *a, **k: appended.append(a) or 1 / 0)
+    ids, rules = torch.zeros(2, 3, dtype=torch.long), LogitRules()
+    with torch.no_grad():
+        for kw in ({}, dict(logits_to_keep=0)):
+            with pytest.raises(ValueError, match="one token per row"):
+                model(input_ids=ids, paged=c.batch(["a", "b"], 3), logit_rules=rules, **kw)
+        assert not appended
+        for kw, n in ((dict(logits_to_keep=1), 3), ({}, 1)):  # one token's logits: the forward begins
+            with pytest.raises(ZeroDivisionError):
+                model(input_ids=ids[:, :n], paged=c.batch(["a", "b"], n), logit_rules=rules, **kw)
