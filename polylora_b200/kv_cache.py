@@ -171,6 +171,9 @@ class PagedKVCache:
         return PagedBatch(self, dev[:rows * width].view(rows, width), lens[0], lens[1], lens[2], max_new, not any(past))
 
 
+_MOST_ROWS = 1 << 20  # of a call of paged_attention
+
+
 class _PagedAttentionForward:
     """The forward of an attention module under a PagedBatch."""
 
@@ -207,8 +210,13 @@ class _PagedAttentionForward:
             step = torch.arange(new, dtype=torch.int32, device=q.device)
             live = step < batch.new_lens[:, None]
             lens = torch.where(live, batch.past_lens[:, None] + step + 1, 0).view(-1)
-            out = paged_attention(q.view(rows * new, -1, d), kc, vc, batch.page_table.repeat_interleave(new, 0), lens,
-                                  scale=self.scale, window=self.window)
+            q = q.view(rows * new, -1, d)
+            out = torch.empty_like(q)
+            for first in range(0, rows * new, _MOST_ROWS):
+                part = slice(first, min(first + _MOST_ROWS, rows * new))
+                row = torch.arange(part.start, part.stop, device=q.device) // new
+                paged_attention(q[part], kc, vc, batch.page_table[row], lens[part], scale=self.scale, window=self.window,
+                                out=out[part])
         return m.o_proj(out.reshape(rows, new, -1)), None
 
     def _prompt(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> torch.Tensor:
