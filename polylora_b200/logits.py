@@ -105,7 +105,7 @@ def apply_logit_rules(logits: torch.Tensor, rules: LogitRules, out: torch.Tensor
     if dev != _current_device():
         with torch.cuda.device(dev):
             return apply_logit_rules(logits, rules, out)
-    _no_grad(logits)
+    _no_grad(logits, rules.repetition_penalty, rules.presence_penalty, rules.frequency_penalty, rules.bias_values)
     if logits.dim() != 2:
         raise ValueError("logits must be (B, V)")
     rows, vocab = logits.shape

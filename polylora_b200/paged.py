@@ -18,6 +18,7 @@ import functools
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native
 from .sgmv import _as, _require_cuda, dtype_code
@@ -38,10 +39,15 @@ def rotary_phases(inv_freq: torch.Tensor) -> torch.Tensor:
 
 
 def _no_grad(*tensors: torch.Tensor | None) -> None:
+    """Refuses tensors whose gradients or tangents would be lost without a word."""
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
                 raise RuntimeError("the paged-cache and logit operators have no gradient: call them under torch.no_grad()")
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError("the paged-cache and logit operators have no gradient, and a tensor carries a tangent")
 
 
 def _same_device(index: int, *tensors: torch.Tensor) -> None:
@@ -153,7 +159,7 @@ def paged_append(
         with torch.cuda.device(dev):
             return paged_append(q, k, v, k_cache, v_cache, page_table, past_lens, new_lens, phases=phases,
                                 interleaved=interleaved, rotary_scale=rotary_scale, return_keys=return_keys)
-    _no_grad(q, k, v)
+    _no_grad(q, k, v, k_cache, v_cache)
     shape, dtype = k.shape, k.dtype
     if len(shape) != 4 or v.shape != shape:
         raise ValueError("q must be (B, M, heads, D), k and v (B, M, kv_heads, D)")
@@ -231,7 +237,7 @@ def paged_attention(
     if dev != _current_device():
         with torch.cuda.device(dev):
             return paged_attention(q, k_cache, v_cache, page_table, seq_lens, scale=scale, window=window, out=out)
-    _no_grad(q)
+    _no_grad(q, k_cache, v_cache)
     shape, dtype = q.shape, q.dtype
     if len(shape) != 3:
         raise ValueError("q must be (B, heads, D)")
