@@ -330,18 +330,20 @@ int plora_peft_pack(const char* path, const char* const* modules, int32_t num_mo
  * none) and k (.., kv_heads, ..) are rotated, k and v written to their pages,
  * rotated queries to q_out and, if k_out is not null, rotated keys to k_out,
  * both dense and apart from the inputs and the cache; padded tokens (m >=
- * new_lens[b]) are zeros there and leave the cache alone.  The first 2 * pairs elements of a head rotate, element i with
- * i + pairs, or 2i with 2i + 1 when interleaved != 0, by position * f_i;
+ * new_lens[b]) are zeros there and leave the cache alone.  The first 2 * pairs
+ * elements of a head rotate, element i with i + pairs, or 2i with 2i + 1 when
+ * interleaved != 0, by position * f_i;
  * phases[i] = round(f_i / (2 pi) * 2^64) mod 2^64, cosines and sines times
- * rotary_scale.  pairs 0: no rotation.  A token whose position has no page in
+ * rotary_scale.  pairs 0: no rotation.  k_cache and v_cache may interleave page
+ * by page, but not share memory.  A token whose position has no page in
  * [0, num_pages) is not cached and raises PLORA_DEV_PAGE_RANGE.
  *
  * plora_paged_attention: out[b, h] = softmax(scale * q[b, h] . k) v over row
  * b's last min(window, seq_lens[b]) of seq_lens[b] cached tokens (window 0:
  * all of them); zeros where there are none.  out is dense (rows, heads,
- * head_dim); it may be q, but not share a part of its memory.  A token on a page outside [0, num_pages) reads as zeros, and
- * seq_lens beyond the table's reach are clamped to it; the first raises
- * PLORA_DEV_PAGE_RANGE.  Sums in fp32; repeated calls agree bit for bit.  The
+ * head_dim); it may be q, but not share a part of its memory.  A token on a page
+ * outside [0, num_pages) reads as zeros, and seq_lens beyond the table's reach are
+ * clamped to it; the first raises PLORA_DEV_PAGE_RANGE.  Sums in fp32; repeated calls agree bit for bit.  The
  * workspace (plora_paged_attention_workspace bytes, 256-byte aligned; 0 for few
  * short rows and for arguments the call rejects) needs no initialisation;
  * calls that may overlap need one each. */

@@ -1227,6 +1227,11 @@ int plora_paged_append(const plora_paged_append_args* args, void* stream) {
   if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(args->q_out) ||
       !aligned16(args->k_out))
     return fail(PLORA_ERR_INVALID_ARGUMENT, "token pointers must be 16-byte aligned");
+  // halves of one buffer's pages interleave; keys and values in one place would not both last
+  const int64_t page_elems = c.kv_heads * c.page_size * c.head_dim, el = (int64_t)elem_size(dtype);
+  if (c.k_cache == c.v_cache ||
+      rows_meet(c.k_cache, c.k_page_stride, c.v_cache, c.v_page_stride, c.num_pages, page_elems, el))
+    return fail(PLORA_ERR_INVALID_ARGUMENT, "k_cache and v_cache share memory");
   DeviceInfo* di = nullptr;
   if ((st = device_info(&di))) return st;
   p.q = q, p.k = k, p.v = v, p.q_out = args->q_out, p.k_out = args->k_out;

@@ -150,7 +150,8 @@ def paged_append(
     times ``rotary_scale``.  k_cache and v_cache are updated in place.  Returns
     the rotated queries and, with ``return_keys``, the rotated keys (padded
     tokens zero); None for what was not given or asked for.  Rows of one call
-    must not write to the same page."""
+    must not write to the same page, nor keys and values to the same memory (their
+    pages may interleave)."""
     dev = k.get_device()
     if dev < 0 or not (v.get_device() == k_cache.get_device() == v_cache.get_device() == page_table.get_device()
                        == past_lens.get_device() == dev):
