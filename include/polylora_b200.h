@@ -343,10 +343,11 @@ int plora_peft_pack(const char* path, const char* const* modules, int32_t num_mo
  * all of them); zeros where there are none.  out is dense (rows, heads,
  * head_dim); it may be q, but not share a part of its memory.  A token on a page
  * outside [0, num_pages) reads as zeros, and seq_lens beyond the table's reach are
- * clamped to it; the first raises PLORA_DEV_PAGE_RANGE.  Sums in fp32; repeated calls agree bit for bit.  The
- * workspace (plora_paged_attention_workspace bytes, 256-byte aligned; 0 for few
- * short rows and for arguments the call rejects) needs no initialisation;
- * calls that may overlap need one each. */
+ * clamped to it; the first raises PLORA_DEV_PAGE_RANGE.  An infinite value of a
+ * token that is attended to gives infinity or NaN.  Sums in fp32; repeated calls
+ * agree bit for bit.  The workspace (plora_paged_attention_workspace bytes, 256-byte
+ * aligned; 0 for few short rows and for arguments the call rejects) needs no
+ * initialisation; calls that may overlap need one each. */
 
 typedef struct plora_paged_cache {
   void* k_cache;
@@ -399,7 +400,8 @@ int plora_paged_attention(const plora_paged_attention_args* args, void* stream);
  * Each row's own rules on its logits (no counterpart in the reference).
  *
  * logits, out: (rows, vocab) of dtype, *_stride elements between rows; out may
- * be logits, but not share a part of its memory.  In fp32, rounded once, in this order:
+ * be logits, but not share a part of its memory.  In fp32, rounded once, in this
+ * order:
  *   x > 0 ? x / repetition[b] : x * repetition[b]  for tokens of row b's history,
  *       tokens[b, i], i < token_lens[b] (null: history each);
  *   x - frequency[b] * count - presence[b]         for tokens found count > 0 times

@@ -158,7 +158,7 @@ class PolyLoraModel(nn.Module):
         the rules to those (``apply_logit_rules``).  Neither has a counterpart in the
         reference."""
         if paged is not None:
-            if len(args) > 1:  # a decoder's second argument is its mask
+            if any(a is not None for a in args[1:]):  # a decoder's second argument is its mask
                 raise ValueError("inputs of a paged forward after the first go by name")
             if kwargs.get("attention_mask") is not None:
                 raise ValueError("a paged batch carries its rows' lengths: pass no attention_mask")

@@ -110,8 +110,10 @@ def test_masks_that_a_paged_forward_would_not_look_at():
         GraphedForward(model, ["__base__"] * 2, paged=batch, input_ids=ids, attention_mask=mask)
     with pytest.raises(ValueError, match="by name"):
         model(ids, mask, paged=batch)
-    with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU fallback"):
-        model(ids, paged=batch)
+    with torch.no_grad():
+        for args in ((ids,), (ids, None)):
+            with pytest.raises(RuntimeError, match="no CPU fallback"):
+                model(*args, paged=batch)
 
 
 def test_rules_for_several_tokens_are_refused_before_the_forward(monkeypatch):
