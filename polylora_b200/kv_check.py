@@ -189,10 +189,12 @@ def check_attention(model: nn.Module, modules: list[nn.Module], forwards: list[A
     state = [(m, dict(m.__dict__), dict(m._buffers)) for m in rotary]  # some renew their frequencies in a forward
 
     def run(start: int, new: int, whole: bool) -> None:
-        ids = torch.randint(0, weight.shape[0], (1, new), generator=torch.Generator().manual_seed(new))
+        # tokens from the middle of the vocabulary: special ones lie at its ends
+        vocab = weight.shape[0]
+        ids = vocab // 8 + torch.randint(0, max(vocab // 2, 1), (1, new), generator=torch.Generator().manual_seed(new))
         if whole:  # twice, apart from the first token
             ids = ids.repeat(2, 1)
-            ids[1, 0] = (ids[1, 0] + 1) % weight.shape[0]
+            ids[1, 0] = (ids[1, 0] + 1) % vocab
         for p in probes:
             p.start, p.stop, p.seen = start, False, False
         probes[-1].stop = not whole
